@@ -78,8 +78,9 @@ def draw(rng):
         else:
             heads = rng.choice([4, 5, 8, 16, 32])
             kv = rng.choice([g for g in (1, heads // 4, heads // 2, heads, heads, heads) if g >= 1 and heads % g == 0])
+            # (a gradient through a single state is zero, and says nothing: training draws start at sixteen)
             tq = 1 if (op == "cross" and rng.random() < 0.3) else _log_int(rng, 2, 4096)
-            c = {"op": op, "B": _log_int(rng, 1, 64), "Tq": tq, "Tk": _log_int(rng, 1, 4096), "heads": heads, "kv_heads": kv,
+            c = {"op": op, "B": _log_int(rng, 1, 64), "Tq": tq, "Tk": _log_int(rng, 16 if op == "cross_train" else 1, 4096), "heads": heads, "kv_heads": kv,
                  "d": rng.choice([32, 40, 64, 80, 96, 128, 160]), "t": t, "lens": rng.random() < 0.6, "mask": rng.random() < 0.4}
             if c["B"] * heads * tq * c["Tk"] > 600e6 or c["B"] * c["Tk"] * kv * c["d"] > 3e8:
                 continue
