@@ -608,6 +608,24 @@ int tfmq_fisher_loss(tfmq_handle h, const float* pred, const float* tgt, const f
 /* y += a*x */
 int tfmq_axpy(tfmq_handle h, float* y, const float* x, float a, size_t n, void* stream);
 
+/* ---- K17: Linears on e4m3 (8-bit float) operands with one fp32 scale per block of 128 ------------------------------------------
+ * A block with largest magnitude a (at least 2^-100) stores q = e4m3(fl32(x * fl32(448 / a))), round half even, and s = fl32(a / 448); a NaN or
+ * an infinity makes its block NaN.  dtype codes: 0 fp32, 1 fp16, 2 bf16.  Kb = ceil(K / 128), Kp = 128 Kb (stored rows are zero padded to Kp).
+ *
+ * tfmq_quantize_fp8: x [M][K] with row stride ld (elements), unit column stride, any alignment.
+ *   by_column = 0: q [M][Kp],                  s [Kb][M]: one scale per row and 128 columns
+ *   by_column = 1: q [K][128 ceil(M / 128)],   s [ceil(M / 128)][K]: one scale per column and 128 rows, stored transposed */
+int tfmq_quantize_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, int by_column, uint8_t* q, float* s, void* stream);
+/* w fp32 [N][K] contiguous -> q [N][Kp], its transpose qt [K][128 ceil(N / 128)], s [ceil(N / 128)][Kb]: one scale per 128 x 128 */
+int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint8_t* q, uint8_t* qt, float* s, void* stream);
+/* y[m][n] = sum_kb sa[kb][m] sb(n, kb) (sum_{k in kb} a[m][k] b[n][k]) + bias[n], y [M][N] contiguous of y_dtype, fp32 sums;
+ * a [M][128 Kb], b [N][128 Kb], 16-byte aligned.  sb(n, kb) = sb[(n / 128) * sbn + kb * sbk], or (sb_row, y fp32 only) sb[kb * N + n]. */
+int tfmq_gemm_fp8(tfmq_handle h, const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, long sbn, long sbk, int sb_row,
+                  const float* bias, void* y, int y_dtype, long M, int N, int Kb, void* stream);
+/* the same product for few rows (M <= 1024) in one launch: x is quantised on the way in (bit-identical operands) */
+int tfmq_linear_fp8_small(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* w, const float* ws, const float* bias,
+                          void* y, int y_dtype, int N, void* stream);
+
 /* ---- K16: the exchange step of the sharded calibration: RCCL over xGMI, one rank per GPU.
  * Replaces linklink.allreduce / dist_helper.allaverage (linklink/__init__.py:6-13, linklink/dist_helper.py:33-36) at
  * their call sites: the SUM of a reconstruction unit's gradients every Adam iteration (quant/reconstruction.py:72-75,

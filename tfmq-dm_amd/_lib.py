@@ -185,6 +185,10 @@ _SIGS = {
     "tfmq_upsample2x_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "tfmq_kl_softmax_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, C.c_long, c_int, c_int, c_int, c_void_p, c_void_p]),
     "tfmq_fisher_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_int, c_size_t, c_void_p, c_void_p, c_void_p]),
+    "tfmq_quantize_fp8": (c_int, [c_void_p, c_void_p, c_int, C.c_long, c_int, C.c_long, c_int, c_void_p, c_void_p, c_void_p]),
+    "tfmq_pack_w_fp8": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tfmq_gemm_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.c_long, C.c_long, c_int, c_void_p, c_void_p, c_int, C.c_long, c_int, c_int, c_void_p]),
+    "tfmq_linear_fp8_small": (c_int, [c_void_p, c_void_p, c_int, C.c_long, c_int, C.c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "tfmq_graph_begin": (c_int, [c_void_p, c_void_p]),
     "tfmq_graph_end": (c_int, [c_void_p, c_void_p, C.POINTER(c_int)]),
     "tfmq_graph_launch": (c_int, [c_void_p, c_int, c_void_p]),

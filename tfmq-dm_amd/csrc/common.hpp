@@ -92,6 +92,18 @@ struct GemmP {
     }                                                                                \
   } while (0)
 
+// Makes the handle's device current for the length of a call (a caller may hold tensors of another device than its current one).
+struct DeviceGuard {
+  int prev = -1;
+  bool switched = false;
+  explicit DeviceGuard(tfmq_handle h) {
+    if (h && hipGetDevice(&prev) == hipSuccess && prev != h->device) switched = hipSetDevice(h->device) == hipSuccess;
+  }
+  ~DeviceGuard() {
+    if (switched) (void)hipSetDevice(prev);
+  }
+};
+
 static inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 // ---------------------------------------------------------------- device helpers

@@ -1737,3 +1737,194 @@ def fisher_loss(pred: torch.Tensor, tgt: torch.Tensor, fgrad: torch.Tensor, mode
     dot = torch.empty(N, dtype=torch.float64, device=pred.device) if mode == FISHER_FULL else None
     handle(d).call("fisher_loss", _p(pred), _p(tgt), _p(fgrad), _p(g), N, pred.numel() // N, int(mode), int(denom), _p(dot), _p(loss), _stream(d))
     return loss, g
+
+
+# ------------------------------------------------------------------------------ K17: 8-bit float Linears, one scale per block of 128
+_DT_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _dt_code(t: torch.Tensor, name: str) -> int:
+    c = _DT_CODE.get(t.dtype)
+    if c is None:
+        raise TfmqError(f"{name}: expected fp32, fp16 or bf16, got {t.dtype}")
+    return c
+
+
+def _rows2d(x: torch.Tensor, name: str):
+    """x [..., K] as rows: (M, K, row stride in elements).  Any leading shape whose rows lie one stride apart (a column slice of a wider
+    tensor included); unit column stride."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise TfmqError(f"{name}: expected [..., K] with K >= 1, got {tuple(x.shape)}")
+    K, M = x.shape[-1], x.numel() // x.shape[-1]
+    if M == 0:
+        return 0, K, K
+    if K > 1 and x.stride(-1) != 1:
+        raise TfmqError(f"{name}: the last dimension must have unit stride")
+    ld, span = None, None
+    for n, st in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+        if n == 1:
+            continue
+        if ld is None:
+            ld, span = st, n * st
+        elif st != span:
+            raise TfmqError(f"{name}: the leading dimensions must collapse into rows of one stride (got strides {tuple(x.stride())})")
+        else:
+            span = n * st
+    ld = K if ld is None else ld
+    if ld < K:
+        raise TfmqError(f"{name}: rows overlap (row stride {ld} < {K})")
+    return M, K, ld
+
+
+def _same_device(d: int, **tensors):
+    for n, t in tensors.items():
+        if t is not None and _dev(t) != d:
+            raise TfmqError(f"{n}: on cuda:{_dev(t)}, the call is on cuda:{d}")
+
+
+class QuantFp8:
+    """Activations in e4m3 with one fp32 scale per row and block of 128 channels (quantize_fp8).  q: uint8 [M, 128 * ceil(K / 128)] (the e4m3
+    bytes, zero padded), scale: fp32 [ceil(K / 128), M]; the value of (m, k) is q[m, k] * scale[k // 128, m]."""
+
+    def __init__(self, q, scale, shape, dtype):
+        self.q, self.scale, self.shape, self.dtype = q, scale, tuple(shape), dtype
+
+
+class PackedFp8:
+    """A Linear's weight [N, K] in e4m3 with one fp32 scale per 128 x 128 block, laid out once (pack_w_fp8 / load_w_fp8).  q: uint8
+    [N, 128 * ceil(K / 128)]; qt: its transpose [K, 128 * ceil(N / 128)], which the gradient with respect to x reads; scale [ceil(N / 128),
+    ceil(K / 128)] and its transpose; bias fp32 [N] or None."""
+
+    def __init__(self, q, qt, scale, bias, N, K):
+        self.q, self.qt, self.scale, self.bias, self.N, self.K = q, qt, scale, bias, N, K
+        self.scale_t = scale.t().contiguous()
+
+
+def quantize_fp8(x: torch.Tensor) -> QuantFp8:
+    """x [..., K] fp32 / fp16 / bf16 -> e4m3 with one scale per row and block of 128 channels: the block's largest magnitude a (at least
+    2^-100) gives s = a / 448, the stored value is e4m3(x * (448 / a)), all in fp32, round half even.  NaN and infinities make their block NaN.
+    A result may be passed to linear_fp8 in place of x, for several Linears that read the same tokens."""
+    d = _dev(x)
+    dt = _dt_code(x, "quantize_fp8")
+    M, K, ld = _rows2d(x, "quantize_fp8")
+    Kb = (K + 127) // 128
+    q = _alloc(M, Kb * 128, dtype=torch.uint8, device=x.device)
+    s = _alloc(Kb, M, dtype=torch.float32, device=x.device)
+    if M:
+        handle(d).call("quantize_fp8", _p(x), dt, M, K, ld, 0, _p(q), _p(s), _stream(d))
+    return QuantFp8(q, s, x.shape, x.dtype)
+
+
+def _quant_cols_fp8(x: torch.Tensor, name: str):
+    """x as rows [M, K] -> (q [K, 128 * ceil(M / 128)], s [ceil(M / 128), K]): one scale per column and block of 128 rows, transposed."""
+    d = _dev(x)
+    M, K, ld = _rows2d(x, name)
+    Mb = (M + 127) // 128
+    q = _alloc(K, Mb * 128, dtype=torch.uint8, device=x.device)
+    s = _alloc(Mb, K, dtype=torch.float32, device=x.device)
+    handle(d).call("quantize_fp8", _p(x), _dt_code(x, name), M, K, ld, 1, _p(q), _p(s), _stream(d))
+    return q, s
+
+
+def _bias_f32(bias, N: int, d: int, name: str):
+    if bias is None:
+        return None
+    if tuple(bias.shape) != (N,):
+        raise TfmqError(f"{name}: bias must be [{N}], got {tuple(bias.shape)}")
+    _same_device(d, bias=bias)
+    return bias.detach().float().contiguous()
+
+
+def pack_w_fp8(w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> PackedFp8:
+    """Quantise a Linear's weight [N, K] (fp32 / fp16 / bf16) to e4m3 with one scale per 128 x 128 block; both orders of the bytes are laid
+    out here, once."""
+    d = _dev(w)
+    _dt_code(w, "pack_w_fp8")
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
+        raise TfmqError(f"pack_w_fp8: expected [N, K], got {tuple(w.shape)}")
+    N, K = w.shape
+    w = w.detach().float().contiguous()
+    Nb, Kb = (N + 127) // 128, (K + 127) // 128
+    q = torch.empty(N, Kb * 128, dtype=torch.uint8, device=w.device)
+    qt = torch.empty(K, Nb * 128, dtype=torch.uint8, device=w.device)
+    s = torch.empty(Nb, Kb, dtype=torch.float32, device=w.device)
+    handle(d).call("pack_w_fp8", _p(w), N, K, _p(q), _p(qt), _p(s), _stream(d))
+    return PackedFp8(q, qt, s, _bias_f32(bias, N, d, "pack_w_fp8"), N, K)
+
+
+def load_w_fp8(q: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor] = None) -> PackedFp8:
+    """A weight that is stored in this form already: q float8_e4m3fn [N, K], scale fp32 [ceil(N / 128), ceil(K / 128)], weight = q * scale."""
+    d = _dev(q)
+    if q.dtype != torch.float8_e4m3fn or q.dim() != 2 or q.shape[0] < 1 or q.shape[1] < 1:
+        raise TfmqError(f"load_w_fp8: expected float8_e4m3fn [N, K], got {q.dtype} {tuple(q.shape)}")
+    N, K = q.shape
+    Nb, Kb = (N + 127) // 128, (K + 127) // 128
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (Nb, Kb):
+        raise TfmqError(f"load_w_fp8: scale must be fp32 [{Nb}, {Kb}], got {scale.dtype} {tuple(scale.shape)}")
+    _same_device(d, scale=scale)
+    b = q.contiguous().view(torch.uint8)
+    q8 = torch.zeros(N, Kb * 128, dtype=torch.uint8, device=q.device)
+    qt = torch.zeros(K, Nb * 128, dtype=torch.uint8, device=q.device)
+    q8[:, :K].copy_(b)
+    qt[:, :N].copy_(b.t())
+    return PackedFp8(q8, qt, scale.detach().clone(), _bias_f32(bias, N, d, "load_w_fp8"), N, K)
+
+
+# rows up to which one launch that quantises on the way in beats quantise + tiled product
+_FP8_SMALL_M = 32
+
+
+def _fp8_product(x, w, ws, bias, N: int, K: int, out_dtype, name: str) -> torch.Tensor:
+    """x (tensor or QuantFp8) [..., K] times the packed rows w [N, Kp] with block scales ws [ceil(N / 128), Kb]."""
+    quantised = isinstance(x, QuantFp8)
+    src = x.q if quantised else x
+    d = _dev(src)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DT_CODE:
+        raise TfmqError(f"{name}: output type must be fp32, fp16 or bf16, got {out_dtype}")
+    if x.shape[-1] != K:
+        raise TfmqError(f"{name}: x has {x.shape[-1]} channels, the weight {K}")
+    _same_device(d, weight=w)
+    if not quantised:
+        dt = _dt_code(x, name)
+        M, _, ld = _rows2d(x, name)
+    else:
+        M = src.shape[0]
+    y = _alloc(tuple(x.shape[:-1]) + (N,), dtype=out_dtype, device=src.device)
+    if M == 0:
+        return y
+    h = handle(d)
+    if not quantised and M <= _FP8_SMALL_M:
+        h.call("linear_fp8_small", _p(x), dt, M, K, ld, _p(w), _p(ws), _p(bias), _p(y), _DT_CODE[out_dtype], N, _stream(d))
+        return y
+    xq = x if quantised else quantize_fp8(x)
+    h.call("gemm_fp8", _p(xq.q), _p(xq.scale), _p(w), _p(ws), ws.shape[1], 1, 0, _p(bias), _p(y), _DT_CODE[out_dtype], M, N, ws.shape[1], _stream(d))
+    return y
+
+
+def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = x W^T + bias on e4m3 operands, one scale per 128 channels of a row of x and per 128 x 128 of W, fp32 sums, rounded once to out_dtype
+    (default: x's).  x: [..., K] fp32 / fp16 / bf16 (quantised here as quantize_fp8 does) or a QuantFp8."""
+    return _fp8_product(x, pw.q, pw.scale, pw.bias, pw.N, pw.K, out_dtype, "linear_fp8")
+
+
+def linear_fp8_bwd(x: torch.Tensor, gy: torch.Tensor, pw: PackedFp8, want_gx: bool = True, want_gw: bool = True):
+    """Gradients of linear_fp8 with the same operand form: gx = gy W (gy quantised per row and 128 outputs, the weight's own bytes) in gy's type,
+    gw = gy^T x (both quantised down their columns, one scale per 128 tokens) in fp32.  -> (gx [..., K] | None, gw [N, K] | None).  The rounding
+    of the forward's operands is passed straight through; the bias gradient is gy summed over its rows."""
+    d = _dev(gy)
+    _same_device(d, x=x, weight=pw.q)
+    if x.shape[-1] != pw.K or gy.shape[-1] != pw.N or x.shape[:-1] != gy.shape[:-1]:
+        raise TfmqError(f"linear_fp8_bwd: x {tuple(x.shape)} and gy {tuple(gy.shape)} do not fit a weight [{pw.N}, {pw.K}]")
+    _dt_code(x, "linear_fp8_bwd"), _dt_code(gy, "linear_fp8_bwd")
+    gx = _fp8_product(gy, pw.qt, pw.scale_t, None, pw.K, pw.N, None, "linear_fp8_bwd") if want_gx else None
+    gw = None
+    if want_gw:
+        gw = _alloc(pw.N, pw.K, dtype=torch.float32, device=gy.device)
+        if gy.numel() == 0:
+            gw.zero_()
+            return gx, gw
+        gq, gs = _quant_cols_fp8(gy, "linear_fp8_bwd")
+        xq, xs = _quant_cols_fp8(x, "linear_fp8_bwd")
+        handle(d).call("gemm_fp8", _p(gq), _p(gs), _p(xq), _p(xs), 0, 0, 1, None, _p(gw), 0, pw.N, pw.K, gs.shape[0], _stream(d))
+    return gx, gw
