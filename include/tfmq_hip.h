@@ -626,6 +626,38 @@ int tfmq_gemm_fp8(tfmq_handle h, const uint8_t* a, const float* sa, const uint8_
 int tfmq_linear_fp8_small(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* w, const float* ws, const float* bias,
                           void* y, int y_dtype, int N, void* stream);
 
+/* ---- K18: cross attention of Tq query tokens to Tk states of an encoder (ldm/modules/attention.py:168-194 with `context` and `mask`), fp16 / bf16,
+ * per-item lengths, a key mask, H query heads over G shared key / value heads ---------------------------------------------------------
+ * q [B][Tq][H d], k / v [B][Tk][G d]: batch and token strides in elements (multiples of 8, 16-byte aligned rows), unit channel stride; o / dq
+ * contiguous [B][Tq][H d], dk / dv contiguous [B][Tk][G d], lse fp32 [B][H][Tq].  d % 8 == 0, d <= 160.  Query head h reads key head h / (H / G).
+ * A key is kept if its index is below kv_lens[b] (null: Tk) and mask[b][key] != 0 (null: all); a query row from q_lens[b] on, and a row that
+ * keeps no key, is zero with lse = -inf, and its gradients are zero.  What masked places hold (NaN, infinities) is never read into a sum. */
+typedef struct tfmq_xattn_desc {
+  int32_t dtype;                 /* 1 fp16, 2 bf16 */
+  int32_t B, H, G, Tq, Tk, d;
+  float scale;                   /* > 0 */
+  const void *q, *k, *v;
+  int64_t q_bs, q_ts, k_bs, k_ts, v_bs, v_ts;
+  const int32_t *q_lens, *kv_lens;
+  const uint8_t* mask;
+  int64_t mask_bs;
+  void* o;                       /* forward: written; backward: read */
+  int64_t o_bs, o_ts;            /* backward: strides of o */
+  float* lse;                    /* forward: written unless null; backward: read */
+  const void* go;                /* backward: upstream gradient [B][Tq][H d] */
+  int64_t go_bs, go_ts;
+  void *dq, *dk, *dv;
+  float* ws;
+  int32_t nsplit;
+} tfmq_xattn_desc;
+/* slices of the key axis that suit a forward call (1: none).  ws: nsplit * B * H * Tq * (d + 2) floats when nsplit > 1 */
+int tfmq_xattn_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk);
+int tfmq_xattn_fwd(tfmq_handle h, const tfmq_xattn_desc* a, void* stream);
+/* dq, dk, dv from q, k, v, o, lse, go.  nsplit: slices of the rows in the dk / dv sums; ws: (2 B H Tq rounded up to 4) floats, and
+ * nsplit * 2 * B * Tk * G * d more when nsplit > 1.  Deterministic. */
+int tfmq_xattn_bwd_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk, int d);
+int tfmq_xattn_bwd(tfmq_handle h, const tfmq_xattn_desc* a, void* stream);
+
 /* ---- K16: the exchange step of the sharded calibration: RCCL over xGMI, one rank per GPU.
  * Replaces linklink.allreduce / dist_helper.allaverage (linklink/__init__.py:6-13, linklink/dist_helper.py:33-36) at
  * their call sites: the SUM of a reconstruction unit's gradients every Adam iteration (quant/reconstruction.py:72-75,

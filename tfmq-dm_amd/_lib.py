@@ -89,6 +89,20 @@ class ChainDesc(C.Structure):
     ]
 
 
+class XattnDesc(C.Structure):
+    """tfmq_xattn_desc"""
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("G", C.c_int32), ("Tq", C.c_int32), ("Tk", C.c_int32), ("d", C.c_int32),
+        ("scale", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_bs", C.c_int64), ("q_ts", C.c_int64), ("k_bs", C.c_int64), ("k_ts", C.c_int64), ("v_bs", C.c_int64), ("v_ts", C.c_int64),
+        ("q_lens", c_void_p), ("kv_lens", c_void_p), ("mask", c_void_p), ("mask_bs", C.c_int64),
+        ("o", c_void_p), ("o_bs", C.c_int64), ("o_ts", C.c_int64), ("lse", c_void_p),
+        ("go", c_void_p), ("go_bs", C.c_int64), ("go_ts", C.c_int64),
+        ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("ws", c_void_p), ("nsplit", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/tfmq_hip.h
 _SIGS = {
     "tfmq_abi_version": (c_int, []),
@@ -189,6 +203,10 @@ _SIGS = {
     "tfmq_pack_w_fp8": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "tfmq_gemm_fp8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.c_long, C.c_long, c_int, c_void_p, c_void_p, c_int, C.c_long, c_int, c_int, c_void_p]),
     "tfmq_linear_fp8_small": (c_int, [c_void_p, c_void_p, c_int, C.c_long, c_int, C.c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "tfmq_xattn_splits": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int]),
+    "tfmq_xattn_fwd": (c_int, [c_void_p, C.POINTER(XattnDesc), c_void_p]),
+    "tfmq_xattn_bwd_splits": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "tfmq_xattn_bwd": (c_int, [c_void_p, C.POINTER(XattnDesc), c_void_p]),
     "tfmq_graph_begin": (c_int, [c_void_p, c_void_p]),
     "tfmq_graph_end": (c_int, [c_void_p, c_void_p, C.POINTER(c_int)]),
     "tfmq_graph_launch": (c_int, [c_void_p, c_int, c_void_p]),

@@ -1,0 +1,170 @@
+// Shared pieces of the cross attention kernels (attention_cross_fwd.hip, attention_cross_bwd.hip): operand types, the tile staging and the
+// transposed fragment reads.
+//
+// Rows and heads: the R = (H / G) Tq query rows that share key head g of item b are one row space, row r = query r % Tq of head g H / G + r / Tq,
+// so shared key heads cost nothing extra and a one-token call still fills a fragment with its H / G heads.
+#pragma once
+#include "conv_common.hpp"
+#include <type_traits>
+
+namespace xattn {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Vec8;
+template <> struct Vec8<_Float16> { using type = v8h; };
+template <> struct Vec8<__bf16> { using type = v8b; };
+
+__device__ __forceinline__ v16f mfma16(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v16f mfma16(v8b a, v8b b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v16f zero16() {
+  v16f z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+  return z;
+}
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+struct View {          // [B][T][heads * d] with unit channel stride; element strides
+  const void* p;
+  long bs, ts;
+};
+
+struct XattnP {
+  View q, k, v, o, go;
+  const float* lse_in;
+  void *y, *dk, *dv;                 // forward: o; backward: dq, dk, dv; contiguous
+  float *lse, *delta, *part;         // [B][H][Tq] each; split partials
+  const int32_t *q_lens, *kv_lens;   // [B] or null
+  const uint8_t* mask;               // [B][Tk] (row stride mask_bs) or null
+  long mask_bs;
+  int B, H, G, rep, Tq, Tk, d;
+  long R;                            // rep * Tq
+  float scale;
+  int nrb, nsplit;                   // row (or key) blocks, slices of the other axis
+};
+
+__device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int T) { return lens ? min(max(lens[b], 0), T) : T; }
+
+// a fragment register r of half hh holds row 8 (r >> 2) + 4 hh + (r & 3) of a 32-row product
+__device__ __forceinline__ constexpr int crow(int r, int hh) { return 8 * (r >> 2) + 4 * hh + (r & 3); }
+
+// scores S^T of 64 keys (two products): those of dropped keys become -inf
+__device__ __forceinline__ void drop_keys(v16f (&s)[2], unsigned long long keep, int hh) {
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const unsigned bits = static_cast<unsigned>(keep >> (32 * kt)) >> (4 * hh);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[kt][r] = ((bits >> crow(r, 0)) & 1) ? s[kt][r] : -INFINITY;
+  }
+}
+
+// ---- a tile of NROW rows x D channels: global -> registers -> LDS (rows of STRIDE bytes).  Rows outside `ok` and channels from d on are zeros, so
+// what a masked place holds (NaN included) never reaches a product.
+template <typename T, int D, int NROW, int STRIDE, int NT = 256>
+struct Tile {
+  static constexpr int DP = D / 8, N = NROW * DP, PT = (N + NT - 1) / NT;
+  uint4 reg[PT];
+  template <typename RowOff>          // RowOff(row) -> element offset of a row, < 0: zeros
+  __device__ __forceinline__ void load(const T* base, int d, RowOff off) {
+#pragma unroll
+    for (int it = 0; it < PT; ++it) {
+      const int idx = static_cast<int>(threadIdx.x) + it * NT, row = idx / DP, pc = idx - row * DP;
+      const long o = (N % NT == 0 || idx < N) && pc * 8 < d ? off(row) : -1;
+      reg[it] = o >= 0 ? *reinterpret_cast<const uint4*>(base + o + pc * 8) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* lds) const {
+#pragma unroll
+    for (int it = 0; it < PT; ++it) {
+      const int idx = static_cast<int>(threadIdx.x) + it * NT, row = idx / DP, pc = idx - row * DP;
+      if (N % NT == 0 || idx < N) *reinterpret_cast<uint4*>(lds + row * STRIDE + pc * 16) = reg[it];
+    }
+  }
+};
+
+// rows [row0, row0 + 32) of a tile as an operand, channels [16 ks, +16): lane j = row, half hh = 8 of the 16 channels
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type frag_rows(const unsigned char* lds, int stride, int row, int ks, int hh) {
+  return *reinterpret_cast<const typename Vec8<T>::type*>(lds + row * stride + (ks * 16 + hh * 8) * 2);
+}
+
+// The tile transposed: channels [32 t, +32) as the operand's rows, tile rows [r0, +16) as its 16 reduction steps, in the order in which a lane
+// of the other operand holds a product's registers (half hh: rows r0 + 4 hh + (0 .. 3), then r0 + 8 + 4 hh + (0 .. 3)).  ds_read_b64_tr_b16 hands lane
+// i of 16 the i-th of 16 channels of four rows; the channel groups are dealt so that operand row 8 a + 4 h + c is channel 32 t + 16 h + 4 a + c:
+// register r of half hh of the result is channel 32 t + 16 hh + r, 16 consecutive ones a lane.
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type frag_cols(const unsigned char* lds, int stride, int r0, int t, int lane) {
+  const int L = lane & 15, gg = (lane >> 4) & 1, hh = lane >> 5, cg = L & 3;
+  const unsigned char* p = lds + (r0 + 4 * hh + (L >> 2)) * stride + (t * 32 + 16 * (cg & 1) + 8 * gg + 4 * (cg >> 1)) * 2;
+  using P = __attribute__((address_space(3))) v4s*;
+  const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p));
+  const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 8 * stride));
+  v8s w;
+  w[0] = a[0]; w[1] = a[1]; w[2] = a[2]; w[3] = a[3]; w[4] = b[0]; w[5] = b[1]; w[6] = b[2]; w[7] = b[3];
+  return __builtin_bit_cast(typename Vec8<T>::type, w);
+}
+
+// registers 8 u .. 8 u + 7 of a product, rounded, as the operand of the reduction step that frag_cols feeds with rows 16 u ...
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type frag_regs(const v16f& s, int u) {
+  typename Vec8<T>::type f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = static_cast<T>(s[8 * u + e]);
+  return f;
+}
+
+// what a row that is not there (or has no query) leaves: zeros, whatever its lanes computed
+template <int N>
+__device__ __forceinline__ void zero_unless(bool ok, v16f (&a)[N]) {
+  if (!ok) {
+#pragma unroll
+    for (int t = 0; t < N; ++t) a[t] = zero16();
+  }
+}
+
+// 16 consecutive channels of one row (those below d; d % 8 == 0)
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int c0, int d, const v16f& v, float f) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    if (c0 + 8 * g >= d) continue;
+    typename Vec8<T>::type w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(v[8 * g + e] * f);
+    *reinterpret_cast<typename Vec8<T>::type*>(row + c0 + 8 * g) = w;
+  }
+}
+
+constexpr int nks(int D) { return (D + 15) / 16; }
+constexpr int nrt(int D) { return (D + 31) / 32; }
+// LDS row strides (bytes).  Row fragments want an odd number of 16-byte units, transposed ones four rows 64 bytes apart modulo the 256 bytes of the
+// banks; where a tile is read both ways the stride is the next odd multiple of 16 whose bank step is within 4 of that.
+constexpr int stride_rows(int D) { return D * 2 + 16; }
+constexpr int stride_cols(int D) { return (nrt(D) | 1) * 64; }
+constexpr int stride_both(int D) {
+  int s = D * 2;
+  for (;; s += 16) {
+    const int m = (s / 4) % 64;
+    if ((s / 16) % 2 == 1 && s >= nrt(D) * 64 && (m == 12 || m == 20 || m == 44 || m == 52)) return s;
+  }
+}
+
+// head dims run in the smallest of these that holds them
+template <typename F>
+int for_head_dim(int d, F f) {
+  if (d <= 32) return f(std::integral_constant<int, 32>{});
+  if (d <= 48) return f(std::integral_constant<int, 48>{});
+  if (d <= 64) return f(std::integral_constant<int, 64>{});
+  if (d <= 80) return f(std::integral_constant<int, 80>{});
+  if (d <= 96) return f(std::integral_constant<int, 96>{});
+  if (d <= 128) return f(std::integral_constant<int, 128>{});
+  return f(std::integral_constant<int, 160>{});
+}
+
+}  // namespace xattn

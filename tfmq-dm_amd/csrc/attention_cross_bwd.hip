@@ -1,0 +1,390 @@
+// Gradients of the cross attention (attention_cross_fwd.hip): with p_ij = exp(scale q_i k_j - lse_i), dp_ij = go_i v_j and D_i = sum_c o_ic go_ic,
+//     ds_ij = p_ij (dp_ij - D_i),   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij go_i.
+//
+// Two kernels recompute p from the saved lse, each with its sums in registers and no atomics: k_xattn_dq walks the keys of 128 rows (a lane owns a row,
+// as in the forward), k_xattn_dkv walks the rows of 128 keys (a lane owns a key; shared key heads sum over their query heads because those are
+// further rows).  Seven products instead of the five of a fused pass, for results that are the same bits every time.  Where few key blocks face
+// many rows -- 77 states under 4096 tokens -- the rows are cut into slices whose fp32 sums are added in order.
+//
+// fp16 range: ds has the size of go p, far below fp16's normal numbers when a loss is averaged over many tokens.  The ds operand is therefore
+// carried with a power of two that brings go's largest magnitude (of the row in dq, of the slice's rows in dkv) to 1 ... 2, and p in dv with 2^12;
+// both are exact and taken out of the fp32 sums.  bf16 has the range.
+#include "attention_cross.hpp"
+
+using namespace xattn;
+
+namespace {
+
+template <typename T> constexpr bool is_f16() { return std::is_same<T, _Float16>::value; }
+
+// 2^-exponent of a magnitude (1 for zero; finite for every input)
+__device__ __forceinline__ int inv_exponent(float a) {
+  const int e = static_cast<int>((__float_as_uint(a) >> 23) & 255);
+  return e == 0 ? 0 : 127 - min(max(e, 27), 227);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
+  constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_both(D), VS = stride_rows(D);
+  using V8 = typename Vec8<T>::type;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* sK = smem;
+  unsigned char* sV = smem + 64 * KS;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
+  const int id = xcd_tile_id();
+  const int rb = id % p.nrb, bg = id / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
+  const long row = static_cast<long>(rb) * 128 + wid * 32 + j;
+  const int hi = static_cast<int>(row / p.Tq), i = static_cast<int>(row - static_cast<long>(hi) * p.Tq);
+  const long brow = (static_cast<long>(b) * p.H + g * p.rep) * p.Tq + row;          // row of [B][H][Tq]
+  const bool in = row < p.R, ok = in && i < qlen;
+  const int head = g * p.rep + hi;
+
+  V8 qf[NKS], gf[NKS];
+  float dl = 0.0f, gm = 0.0f;
+  {
+    const long hc = static_cast<long>(head) * p.d;
+    const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.bs + i * p.q.ts + hc;
+    const T* grow = static_cast<const T*>(p.go.p) + b * p.go.bs + i * p.go.ts + hc;
+    const T* orow = static_cast<const T*>(p.o.p) + b * p.o.bs + i * p.o.ts + hc;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = ks * 16 + hh * 8;
+      uint4 a = make_uint4(0, 0, 0, 0), w = a, z = a;
+      if (ok && c < p.d) {
+        a = *reinterpret_cast<const uint4*>(qrow + c);
+        w = *reinterpret_cast<const uint4*>(grow + c);
+        z = *reinterpret_cast<const uint4*>(orow + c);
+      }
+      qf[ks] = __builtin_bit_cast(V8, a);
+      gf[ks] = __builtin_bit_cast(V8, w);
+      const V8 of = __builtin_bit_cast(V8, z);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = static_cast<float>(gf[ks][e]);
+        dl = __builtin_fmaf(static_cast<float>(of[e]), x, dl);
+        gm = fmaxf(gm, fabsf(x));
+      }
+    }
+  }
+  dl += __shfl_xor(dl, 32, 64);
+  gm = fmaxf(gm, __shfl_xor(gm, 32, 64));
+  float lse2 = INFINITY;
+  if (ok) {
+    const float v = p.lse_in[brow];
+    lse2 = v == -INFINITY ? INFINITY : v * LOG2E;
+  }
+  if (in && hh == 0) {
+    p.delta[brow] = dl;
+    p.delta[static_cast<long>(p.B) * p.H * p.Tq + brow] = gm;
+  }
+  const int fe = is_f16<T>() ? inv_exponent(gm) : 0;
+  const float sh = lse2 - static_cast<float>(fe);
+
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
+  const uint8_t* mb = p.mask ? p.mask + b * p.mask_bs : nullptr;
+  auto keep_bit = [&](int t) { const int key = t * 64 + lane; return key < klen && (!mb || mb[key] != 0); };
+  const int nt = (klen + 63) / 64;
+  Tile<T, D, 64, KS> tk;
+  Tile<T, D, 64, VS> tv;
+  unsigned long long cur = 0, nxt = 0;
+  auto fetch = [&](int t, unsigned long long m) {
+    auto live = [&](int r) { return (m >> r) & 1; };
+    tk.load(kb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.k.ts : -1L; });
+    tv.load(vb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.v.ts : -1L; });
+  };
+  const float c2 = p.scale * LOG2E;
+  v16f acc[NRT];
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) acc[t] = zero16();
+  if (nt > 0) {
+    cur = __ballot(keep_bit(0));
+    fetch(0, cur);
+  }
+  for (int t = 0; t < nt; ++t) {
+    __syncthreads();
+    tk.store(sK);
+    tv.store(sV);
+    __syncthreads();
+    nxt = 0;
+    if (t + 1 < nt) {
+      nxt = __ballot(keep_bit(t + 1));
+      fetch(t + 1, nxt);
+    }
+    if (cur != 0) {
+      v16f s[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        s[kt] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) s[kt] = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s[kt]);
+      }
+      if (cur != ~0ull) drop_keys(s, cur, hh);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        v16f dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) dp = mfma16(frag_rows<T>(sV, VS, kt * 32 + j, ks, hh), gf[ks], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], c2, -sh)) * (dp[r] - dl);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const V8 df = frag_regs<T>(s[u >> 1], u & 1);
+#pragma unroll
+        for (int t2 = 0; t2 < NRT; ++t2) acc[t2] = mfma16(frag_cols<T>(sK, KS, u * 16, t2, lane), df, acc[t2]);
+      }
+    }
+    cur = nxt;
+  }
+  if (!in) return;
+  zero_unless(ok, acc);
+  const float f = p.scale * __builtin_amdgcn_exp2f(static_cast<float>(-fe));
+  T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, acc[t], f);
+}
+
+template <int D> constexpr int dkv_rows() { return D <= 64 ? 64 : 32; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
+  constexpr int NKS = nks(D), NRT = nrt(D), S = stride_both(D), NR = dkv_rows<D>();
+  using V8 = typename Vec8<T>::type;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* sQ = smem;
+  unsigned char* sG = smem + NR * S;
+  float* sL = reinterpret_cast<float*>(smem + 2 * NR * S);          // lse (base 2) of the tile's rows, +inf: not a row
+  float* sD = sL + NR;
+  float* sM = sD + NR;                                              // 4 floats: the waves' maxima
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
+  const int id = xcd_tile_id();
+  const int sp = id % p.nsplit, kbk = (id / p.nsplit) % p.nrb;
+  const int bg = id / p.nsplit / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
+  const int key = kbk * 128 + wid * 32 + j;
+  const bool keep = key < klen && (!p.mask || p.mask[b * p.mask_bs + key] != 0);
+  const bool work = __any(keep);
+  const long brow0 = (static_cast<long>(b) * p.H + g * p.rep) * p.Tq;          // the row space of (b, g) inside [B][H][Tq]
+  const float* gmax = p.delta + static_cast<long>(p.B) * p.H * p.Tq + brow0;
+
+  const int nt = static_cast<int>((p.R + NR - 1) / NR), per = (nt + p.nsplit - 1) / p.nsplit;
+  const int t0 = sp * per;
+  int t1 = min(nt, t0 + per);
+  if (kbk * 128 >= klen || qlen == 0) t1 = t0;          // nothing to sum: zeros are written below
+
+  V8 kf[NKS], vf[NKS];
+  {
+    const T* krow = static_cast<const T*>(p.k.p) + b * p.k.bs + key * p.k.ts + static_cast<long>(g) * p.d;
+    const T* vrow = static_cast<const T*>(p.v.p) + b * p.v.bs + key * p.v.ts + static_cast<long>(g) * p.d;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = ks * 16 + hh * 8;
+      uint4 a = make_uint4(0, 0, 0, 0), w = a;
+      if (keep && c < p.d) {
+        a = *reinterpret_cast<const uint4*>(krow + c);
+        w = *reinterpret_cast<const uint4*>(vrow + c);
+      }
+      kf[ks] = __builtin_bit_cast(V8, a);
+      vf[ks] = __builtin_bit_cast(V8, w);
+    }
+  }
+  constexpr float PSHIFT = is_f16<T>() ? 12.0f : 0.0f;
+  float ff = 1.0f, unf = 1.0f;          // the power of two in ds, relative to the one in p, and what takes it out again
+  if (is_f16<T>() && t0 < t1) {
+    float mx = 0.0f;
+    for (long r = static_cast<long>(t0) * NR + tid; r < min(p.R, static_cast<long>(t1) * NR); r += 256) mx = fmaxf(mx, gmax[r]);
+    mx = wave_reduce_max(mx);
+    if (lane == 0) sM[wid] = mx;
+    __syncthreads();
+    const int fe = inv_exponent(fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3])));
+    ff = __builtin_amdgcn_exp2f(static_cast<float>(fe) - PSHIFT);
+    unf = __builtin_amdgcn_exp2f(static_cast<float>(-fe));
+  }
+  Tile<T, D, NR, S> tq, tg;
+  float rl = INFINITY, rd = 0.0f;
+  auto fetch = [&](int t) {
+    const long r0 = static_cast<long>(t) * NR;
+    auto at = [&](int r, const View& v) -> long {
+      const long row = r0 + r;
+      if (row >= p.R) return -1;
+      const int hi = static_cast<int>(row / p.Tq), i = static_cast<int>(row - static_cast<long>(hi) * p.Tq);
+      return i < qlen ? i * v.ts + static_cast<long>(hi) * p.d : -1;
+    };
+    const long hc = b * p.q.bs + static_cast<long>(g) * p.rep * p.d, gc = b * p.go.bs + static_cast<long>(g) * p.rep * p.d;
+    tq.load(static_cast<const T*>(p.q.p) + hc, p.d, [&](int r) { return at(r, p.q); });
+    tg.load(static_cast<const T*>(p.go.p) + gc, p.d, [&](int r) { return at(r, p.go); });
+    if (tid < NR) {
+      const long row = r0 + tid;
+      rl = INFINITY;
+      rd = 0.0f;
+      if (row < p.R && static_cast<int>(row % p.Tq) < qlen) {
+        const float v = p.lse_in[brow0 + row];
+        rl = v == -INFINITY ? INFINITY : v * LOG2E;
+        rd = p.delta[brow0 + row];
+      }
+    }
+  };
+  const float c2 = p.scale * LOG2E;
+  v16f ak[NRT], av[NRT];
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) ak[t] = zero16(), av[t] = zero16();
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    tq.store(sQ);
+    tg.store(sG);
+    if (tid < NR) sL[tid] = rl - PSHIFT, sD[tid] = rd;
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    if (work) {
+#pragma unroll
+      for (int half = 0; half < NR / 32; ++half) {
+        v16f s = zero16(), dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) s = mfma16(frag_rows<T>(sQ, S, half * 32 + j, ks, hh), kf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) dp = mfma16(frag_rows<T>(sG, S, half * 32 + j, ks, hh), vf[ks], dp);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const float4 L = *reinterpret_cast<const float4*>(sL + half * 32 + 8 * a + 4 * hh);
+          const float4 dd = *reinterpret_cast<const float4*>(sD + half * 32 + 8 * a + 4 * hh);
+          const float lv[4] = {L.x, L.y, L.z, L.w}, dv[4] = {dd.x, dd.y, dd.z, dd.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int r = 4 * a + c;
+            const float pr = keep ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lv[c])) : 0.0f;
+            s[r] = pr;
+            dp[r] = pr * (dp[r] - dv[c]) * ff;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const V8 pf = frag_regs<T>(s, u), df = frag_regs<T>(dp, u);
+#pragma unroll
+          for (int t2 = 0; t2 < NRT; ++t2) {
+            av[t2] = mfma16(frag_cols<T>(sG, S, half * 32 + u * 16, t2, lane), pf, av[t2]);
+            ak[t2] = mfma16(frag_cols<T>(sQ, S, half * 32 + u * 16, t2, lane), df, ak[t2]);
+          }
+        }
+      }
+    }
+  }
+  if (key >= p.Tk) return;
+  const float fk = p.scale * unf, fv = is_f16<T>() ? 1.0f / 4096.0f : 1.0f;
+  const long krow = (static_cast<long>(b) * p.Tk + key) * p.G + g;
+  if (p.nsplit > 1) {
+    const long n = static_cast<long>(p.B) * p.Tk * p.G * p.d;
+    float* pk = p.part + 2 * sp * n + krow * p.d;
+#pragma unroll
+    for (int t = 0; t < NRT; ++t)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int c = t * 32 + 16 * hh + 4 * q4;
+        if (c >= p.d) continue;
+        *reinterpret_cast<float4*>(pk + c) = make_float4(ak[t][4 * q4] * fk, ak[t][4 * q4 + 1] * fk, ak[t][4 * q4 + 2] * fk, ak[t][4 * q4 + 3] * fk);
+        *reinterpret_cast<float4*>(pk + n + c) = make_float4(av[t][4 * q4] * fv, av[t][4 * q4 + 1] * fv, av[t][4 * q4 + 2] * fv, av[t][4 * q4 + 3] * fv);
+      }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) {
+    store16<T>(static_cast<T*>(p.dk) + krow * p.d, t * 32 + 16 * hh, p.d, ak[t], fk);
+    store16<T>(static_cast<T*>(p.dv) + krow * p.d, t * 32 + 16 * hh, p.d, av[t], fv);
+  }
+}
+
+// dk and dv: the slices' sums in order; 8 channels a thread
+template <typename T>
+__global__ __launch_bounds__(256) void k_xattn_sum(XattnP p, long n) {
+  const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= 2 * n) return;
+  float a[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a[e] = 0.0f;
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float4* q = reinterpret_cast<const float4*>(p.part + 2 * s * n + i);
+    const float4 x = q[0], y = q[1];
+    a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w; a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+  }
+  typename Vec8<T>::type w;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(a[e]);
+  T* out = i < n ? static_cast<T*>(p.dk) + i : static_cast<T*>(p.dv) + (i - n);
+  *reinterpret_cast<typename Vec8<T>::type*>(out) = w;
+}
+
+template <typename T>
+int launch_bwd(tfmq_handle h, XattnP p, hipStream_t st) {
+  return for_head_dim(p.d, [&](auto dc) {
+    constexpr int D = decltype(dc)::value;
+    auto kq = &k_xattn_dq<T, D>;
+    auto kk = &k_xattn_dkv<T, D>;
+    constexpr int sq = 64 * (stride_both(D) + stride_rows(D)), sk = 2 * dkv_rows<D>() * (stride_both(D) + 4) + 16;
+    TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kq), hipFuncAttributeMaxDynamicSharedMemorySize, sq));
+    TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kk), hipFuncAttributeMaxDynamicSharedMemorySize, sk));
+    XattnP a = p;
+    a.nrb = ceil_div(p.R, 128);
+    const long nq = static_cast<long>(p.B) * p.G * a.nrb;
+    XattnP c = p;
+    c.nrb = ceil_div(p.Tk, 128);
+    const long nk = static_cast<long>(p.B) * p.G * c.nrb * p.nsplit;
+    TFMQ_CHECK_ARG(h, nq < (1L << 31) && nk < (1L << 31), "xattn_bwd: too many workgroups");
+    hipLaunchKernelGGL(kq, dim3(static_cast<unsigned>(nq)), dim3(256), sq, st, a);
+    TFMQ_LAUNCH_CHECK(h);
+    hipLaunchKernelGGL(kk, dim3(static_cast<unsigned>(nk)), dim3(256), sk, st, c);
+    TFMQ_LAUNCH_CHECK(h);
+    if (p.nsplit > 1) {
+      const long n = static_cast<long>(p.B) * p.Tk * p.G * p.d;
+      hipLaunchKernelGGL((k_xattn_sum<T>), dim3(static_cast<unsigned>((2 * n / 8 + 255) / 256)), dim3(256), 0, st, p, n);
+      TFMQ_LAUNCH_CHECK(h);
+    }
+    return TFMQ_OK;
+  });
+}
+
+}  // namespace
+
+// Slices of the rows in the dk / dv kernel: only where its key blocks leave CUs idle; at least two row tiles a slice.
+extern "C" int tfmq_xattn_bwd_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk, int d) {
+  if (!h || B <= 0 || H <= 0 || G <= 0 || H % G || Tq <= 0 || Tk <= 0) return 1;
+  const long blocks = static_cast<long>(B) * G * ceil_div(Tk, 128), R = static_cast<long>(H / G) * Tq;
+  const long want = 2L * h->cu_count;
+  if (blocks * 2 > want) return 1;
+  const long most = (R + 127) / 128, n = want / blocks;
+  (void)d;
+  return static_cast<int>(n < 1 ? 1 : n < most ? n : most);
+}
+
+extern "C" int tfmq_xattn_bwd(tfmq_handle h, const tfmq_xattn_desc* a, void* stream) {
+  TFMQ_CHECK_ARG(h, h && a, "xattn_bwd: null pointer");
+  DeviceGuard guard(h);
+  TFMQ_CHECK_ARG(h, a->B > 0 && a->H > 0 && a->G > 0 && a->H % a->G == 0 && a->Tq > 0 && a->Tk > 0 && a->d > 0 && a->d <= 160 && a->d % 8 == 0,
+                 "xattn_bwd: bad shape");
+  TFMQ_CHECK_ARG(h, a->dtype == 1 || a->dtype == 2, "xattn_bwd: fp16 or bf16");
+  TFMQ_CHECK_ARG(h, a->q && a->k && a->v && a->o && a->go && a->lse && a->dq && a->dk && a->dv && a->ws, "xattn_bwd: null tensor");
+  TFMQ_CHECK_ARG(h, a->nsplit >= 1, "xattn_bwd: bad slice count");
+  XattnP p{};
+  p.q = {a->q, a->q_bs, a->q_ts};
+  p.k = {a->k, a->k_bs, a->k_ts};
+  p.v = {a->v, a->v_bs, a->v_ts};
+  p.o = {a->o, a->o_bs, a->o_ts};
+  p.go = {a->go, a->go_bs, a->go_ts};
+  p.lse_in = a->lse;
+  p.y = a->dq;
+  p.dk = a->dk;
+  p.dv = a->dv;
+  p.q_lens = a->q_lens;
+  p.kv_lens = a->kv_lens;
+  p.mask = a->mask;
+  p.mask_bs = a->mask_bs;
+  p.B = a->B; p.H = a->H; p.G = a->G; p.rep = a->H / a->G; p.Tq = a->Tq; p.Tk = a->Tk; p.d = a->d;
+  p.R = static_cast<long>(p.rep) * p.Tq;
+  p.scale = a->scale;
+  p.nsplit = a->nsplit;
+  const long rows = static_cast<long>(p.B) * p.H * p.Tq;
+  p.delta = a->ws;
+  p.part = a->ws + (2 * rows + 3) / 4 * 4;
+  return a->dtype == 1 ? launch_bwd<_Float16>(h, p, as_stream(stream)) : launch_bwd<__bf16>(h, p, as_stream(stream));
+}

@@ -1,0 +1,246 @@
+// Cross attention of Tq query tokens to Tk states of an encoder, per-item lengths, a key mask and shared key heads (CrossAttention.forward with
+// `context` and `mask`, ldm/modules/attention.py:168-194; there a fully masked row attends to everything evenly, here it is zero):
+//     o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j - lse_i),  lse_i = log sum_j exp(scale q_i k_j)   over the kept keys j.
+//
+// One pass over the keys with the running maximum and sum.  A wave owns 32 rows as the COLUMNS of S^T = K Q^T: a lane has one row, its maximum and
+// sum are registers, and the probabilities are already the operand that O^T = V^T P^T wants.  K and V tiles of 64 keys are loaded into registers
+// while the previous tile is multiplied, and stored to LDS row-major; V is read transposed by ds_read_b64_tr_b16.  Scores, statistics and sums are fp32;
+// the probabilities are rounded to the operand type for the second product (they are <= 1, the sum takes them unrounded).
+#include "attention_cross.hpp"
+
+using namespace xattn;
+
+namespace {
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
+  constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_rows(D), VS = stride_cols(D);
+  using V8 = typename Vec8<T>::type;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* sK = smem;
+  unsigned char* sV = smem + 64 * KS;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
+  const int id = xcd_tile_id();
+  const int sp = id % p.nsplit, rb = (id / p.nsplit) % p.nrb;
+  const int bg = id / p.nsplit / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
+
+  const long row = static_cast<long>(rb) * 128 + wid * 32 + j;
+  const int hi = static_cast<int>(row / p.Tq), i = static_cast<int>(row - static_cast<long>(hi) * p.Tq);
+  const bool ok = row < p.R && i < qlen;
+  const int head = g * p.rep + hi;
+  V8 qf[NKS];
+  {
+    const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.bs + i * p.q.ts + static_cast<long>(head) * p.d;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = ks * 16 + hh * 8;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (ok && c < p.d) w = *reinterpret_cast<const uint4*>(qrow + c);
+      qf[ks] = __builtin_bit_cast(V8, w);
+    }
+  }
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
+  const uint8_t* mb = p.mask ? p.mask + b * p.mask_bs : nullptr;
+  auto keep_bit = [&](int t) { const int key = t * 64 + lane; return key < klen && (!mb || mb[key] != 0); };
+
+  const int nt = (klen + 63) / 64, per = (nt + p.nsplit - 1) / p.nsplit;
+  const int t0 = sp * per, t1 = min(nt, t0 + per);
+  Tile<T, D, 64, KS> tk;
+  Tile<T, D, 64, VS> tv;
+  unsigned long long cur = 0, nxt = 0;
+  auto fetch = [&](int t, unsigned long long m) {
+    auto live = [&](int r) { return (m >> r) & 1; };
+    tk.load(kb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.k.ts : -1L; });
+    tv.load(vb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.v.ts : -1L; });
+  };
+  const float c2 = p.scale * LOG2E;
+  float m = -INFINITY, l = 0.0f;
+  v16f o[NRT];
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) o[t] = zero16();
+
+  if (t0 < t1) {
+    cur = __ballot(keep_bit(t0));
+    fetch(t0, cur);
+  }
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();                   // every wave is through with the previous tile
+    tk.store(sK);
+    tv.store(sV);
+    __syncthreads();
+    nxt = 0;
+    if (t + 1 < t1) {
+      nxt = __ballot(keep_bit(t + 1));
+      fetch(t + 1, nxt);
+    }
+    if (cur != 0) {
+      v16f s[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        s[kt] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) s[kt] = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s[kt]);
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kt][r] *= c2;
+      if (cur != ~0ull) drop_keys(s, cur, hh);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - mu);
+      m = mn;
+      float rs = 0.0f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kt][r] = __builtin_amdgcn_exp2f(s[kt][r] - mu);
+          rs += s[kt][r];
+        }
+      l = __builtin_fmaf(l, alpha, rs);
+      if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int t2 = 0; t2 < NRT; ++t2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[t2][r] *= alpha;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const V8 pf = frag_regs<T>(s[u >> 1], u & 1);
+#pragma unroll
+        for (int t2 = 0; t2 < NRT; ++t2) o[t2] = mfma16(frag_cols<T>(sV, VS, u * 16, t2, lane), pf, o[t2]);
+      }
+    }
+    cur = nxt;
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (row >= p.R) return;
+  zero_unless(ok, o);
+  const long orow = (static_cast<long>(b) * p.H + head) * p.Tq + i;          // row of [B][H][Tq]
+  if (p.nsplit > 1) {
+    // slice sp's sums against its own maximum: [slice][row][d] and {m, l} behind them
+    float* po = p.part + (static_cast<long>(sp) * p.B * p.H * p.Tq + orow) * p.d;
+#pragma unroll
+    for (int t = 0; t < NRT; ++t) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int c = t * 32 + 16 * hh + 4 * q4;
+        if (c < p.d) *reinterpret_cast<float4*>(po + c) = make_float4(o[t][4 * q4], o[t][4 * q4 + 1], o[t][4 * q4 + 2], o[t][4 * q4 + 3]);
+      }
+    }
+    if (hh == 0) {
+      float* ml = p.part + static_cast<long>(p.nsplit) * p.B * p.H * p.Tq * p.d + (static_cast<long>(sp) * p.B * p.H * p.Tq + orow) * 2;
+      ml[0] = ok ? m : -INFINITY;
+      ml[1] = ok ? l : 0.0f;
+    }
+    return;
+  }
+  const float inv = ok && l != 0.0f ? 1.0f / l : 0.0f;
+  T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
+#pragma unroll
+  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, o[t], inv);
+  if (p.lse && hh == 0) p.lse[orow] = ok && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+}
+
+// joins the slices of a row: 16 lanes a row, four (eight) channels a lane and step
+template <typename T>
+__global__ __launch_bounds__(256) void k_xattn_join(XattnP p) {
+  const long rows = static_cast<long>(p.B) * p.H * p.Tq;
+  const long r = static_cast<long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int c16 = threadIdx.x & 15;
+  if (r >= rows) return;
+  const float* ml = p.part + static_cast<long>(p.nsplit) * rows * p.d;
+  float M = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, ml[(s * rows + r) * 2]);
+  const float mu = M == -INFINITY ? 0.0f : M;
+  float l = 0.0f;
+  for (int s = 0; s < p.nsplit; ++s) l = __builtin_fmaf(ml[(s * rows + r) * 2 + 1], __builtin_amdgcn_exp2f(ml[(s * rows + r) * 2] - mu), l);
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const long bh = r / p.Tq;
+  const int i = static_cast<int>(r - bh * p.Tq), b = static_cast<int>(bh / p.H), head = static_cast<int>(bh - static_cast<long>(b) * p.H);
+  T* y = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
+  for (int c = c16 * 8; c < p.d; c += 128) {
+    float a[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = 0.0f;
+    for (int s = 0; s < p.nsplit; ++s) {
+      const float w = __builtin_amdgcn_exp2f(ml[(s * rows + r) * 2] - mu);
+      const float4* po = reinterpret_cast<const float4*>(p.part + (s * rows + r) * p.d + c);
+      const float4 x = po[0], z = po[1];
+      a[0] = __builtin_fmaf(x.x, w, a[0]); a[1] = __builtin_fmaf(x.y, w, a[1]); a[2] = __builtin_fmaf(x.z, w, a[2]); a[3] = __builtin_fmaf(x.w, w, a[3]);
+      a[4] = __builtin_fmaf(z.x, w, a[4]); a[5] = __builtin_fmaf(z.y, w, a[5]); a[6] = __builtin_fmaf(z.z, w, a[6]); a[7] = __builtin_fmaf(z.w, w, a[7]);
+    }
+    typename Vec8<T>::type w8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w8[e] = static_cast<T>(a[e] * inv);
+    *reinterpret_cast<typename Vec8<T>::type*>(y + c) = w8;
+  }
+  if (p.lse && c16 == 0) p.lse[r] = l != 0.0f ? (M + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+}
+
+template <typename T>
+int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
+  return for_head_dim(p.d, [&](auto dc) {
+    constexpr int D = decltype(dc)::value;
+    auto kern = &k_xattn_fwd<T, D>;
+    constexpr int smem = 64 * (stride_rows(D) + stride_cols(D));
+    TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+    p.nrb = ceil_div(p.R, 128);
+    const long nb = static_cast<long>(p.B) * p.G * p.nrb * p.nsplit;
+    TFMQ_CHECK_ARG(h, nb < (1L << 31), "xattn_fwd: too many workgroups");
+    hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nb)), dim3(256), smem, st, p);
+    TFMQ_LAUNCH_CHECK(h);
+    if (p.nsplit > 1) {
+      hipLaunchKernelGGL((k_xattn_join<T>), dim3(static_cast<unsigned>((static_cast<long>(p.B) * p.H * p.Tq + 15) / 16)), dim3(256), 0, st, p);
+      TFMQ_LAUNCH_CHECK(h);
+    }
+    return TFMQ_OK;
+  });
+}
+
+}  // namespace
+
+// Slices of the key axis of a forward call: only where the rows alone leave CUs idle; at least two tiles of 64 keys a slice.
+extern "C" int tfmq_xattn_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk) {
+  if (!h || B <= 0 || H <= 0 || G <= 0 || H % G || Tq <= 0 || Tk <= 0) return 1;
+  const long blocks = static_cast<long>(B) * G * ceil_div(static_cast<long>(H / G) * Tq, 128);
+  const long want = 3L * h->cu_count;
+  if (blocks * 2 > want) return 1;
+  const long most = (Tk + 127) / 128;
+  const long n = want / blocks;
+  return static_cast<int>(n < 1 ? 1 : n < most ? n : most);
+}
+
+extern "C" int tfmq_xattn_fwd(tfmq_handle h, const tfmq_xattn_desc* a, void* stream) {
+  TFMQ_CHECK_ARG(h, h && a, "xattn_fwd: null pointer");
+  DeviceGuard guard(h);
+  TFMQ_CHECK_ARG(h, a->B > 0 && a->H > 0 && a->G > 0 && a->H % a->G == 0 && a->Tq > 0 && a->Tk >= 0 && a->d > 0 && a->d <= 160 && a->d % 8 == 0,
+                 "xattn_fwd: bad shape");
+  TFMQ_CHECK_ARG(h, a->dtype == 1 || a->dtype == 2, "xattn_fwd: fp16 or bf16");
+  TFMQ_CHECK_ARG(h, a->q && (a->Tk == 0 || (a->k && a->v)) && a->o, "xattn_fwd: null tensor");
+  TFMQ_CHECK_ARG(h, a->nsplit >= 1 && (a->nsplit == 1 || a->ws), "xattn_fwd: slices need a workspace");
+  XattnP p{};
+  p.q = {a->q, a->q_bs, a->q_ts};
+  p.k = {a->k, a->k_bs, a->k_ts};
+  p.v = {a->v, a->v_bs, a->v_ts};
+  p.y = a->o;
+  p.lse = a->lse;
+  p.part = a->ws;
+  p.q_lens = a->q_lens;
+  p.kv_lens = a->kv_lens;
+  p.mask = a->mask;
+  p.mask_bs = a->mask_bs;
+  p.B = a->B; p.H = a->H; p.G = a->G; p.rep = a->H / a->G; p.Tq = a->Tq; p.Tk = a->Tk; p.d = a->d;
+  p.R = static_cast<long>(p.rep) * p.Tq;
+  p.scale = a->scale;
+  p.nsplit = a->nsplit;
+  return a->dtype == 1 ? launch_fwd<_Float16>(h, p, as_stream(stream)) : launch_fwd<__bf16>(h, p, as_stream(stream));
+}

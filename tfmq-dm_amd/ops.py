@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._lib import ChainDesc, ConvDesc, FfDesc, GnDesc, QSel, TfmqError
+from ._lib import ChainDesc, ConvDesc, FfDesc, GnDesc, QSel, TfmqError, XattnDesc
 from ._lib import handle as _lib_handle
 
 NULL = None
@@ -1928,3 +1928,110 @@ def linear_fp8_bwd(x: torch.Tensor, gy: torch.Tensor, pw: PackedFp8, want_gx: bo
         xq, xs = _quant_cols_fp8(x, "linear_fp8_bwd")
         handle(d).call("gemm_fp8", _p(gq), _p(gs), _p(xq), _p(xs), 0, 0, 1, None, _p(gw), 0, pw.N, pw.K, gs.shape[0], _stream(d))
     return gx, gw
+
+
+# ------------------------------------------------------------------------------ K18: cross attention to an encoder's states
+def _xattn_view(t: torch.Tensor, T: int, C_: int, B: int, dtype, name: str):
+    """(pointer, batch stride, token stride) of a [B, T, C] operand: unit channel stride, rows 16-byte aligned."""
+    if tuple(t.shape) != (B, T, C_):
+        raise TfmqError(f"{name}: expected [{B}, {T}, {C_}], got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TfmqError(f"{name}: expected {dtype}, got {t.dtype}")
+    bs = t.stride(0) if B > 1 else 0
+    ts = t.stride(1) if T > 1 else 0
+    if t.numel() and (t.stride(2) != 1 or bs % 8 or ts % 8 or t.data_ptr() % 16):
+        raise TfmqError(f"{name}: needs unit channel stride and 16-byte aligned rows (strides {tuple(t.stride())}, address % 16 = {t.data_ptr() % 16})")
+    return t.data_ptr(), bs, ts
+
+
+def _xattn_desc(q, k, v, heads: int, scale: float, kv_heads, q_lens, kv_lens, mask, name: str):
+    d_ = _dev(q)
+    _same_device(d_, k=k, v=v, q_lens=q_lens, kv_lens=kv_lens, mask=mask)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TfmqError(f"{name}: fp16 or bf16 operands (fp32: attention_f32_fwd), got {q.dtype}")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise TfmqError(f"{name}: q, k, v must be [B, T, heads * d]")
+    B, Tq, Cq = q.shape
+    Tk = k.shape[1]
+    G = heads if kv_heads is None else int(kv_heads)
+    if heads < 1 or G < 1 or Cq % heads or heads % G:
+        raise TfmqError(f"{name}: {Cq} channels do not split into {heads} heads over {G} key heads")
+    d = Cq // heads
+    if d % 8 or not 0 < d <= 160:
+        raise TfmqError(f"{name}: head dim {d} (a multiple of 8, at most 160)")
+    scale = float(scale)
+    if not (0.0 < scale < float("inf")):
+        raise TfmqError(f"{name}: scale must be positive and finite, got {scale}")
+    a = XattnDesc()
+    a.dtype, a.B, a.H, a.G, a.Tq, a.Tk, a.d, a.scale = _DT_CODE[q.dtype], B, heads, G, Tq, Tk, d, scale
+    a.q, a.q_bs, a.q_ts = _xattn_view(q, Tq, Cq, B, q.dtype, name + " q")
+    a.k, a.k_bs, a.k_ts = _xattn_view(k, Tk, G * d, B, q.dtype, name + " k")
+    a.v, a.v_bs, a.v_ts = _xattn_view(v, Tk, G * d, B, q.dtype, name + " v")
+    for n, t in (("q_lens", q_lens), ("kv_lens", kv_lens)):
+        if t is not None:
+            if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+                raise TfmqError(f"{name}: {n} must be contiguous int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+            setattr(a, n, t.data_ptr())
+    if mask is not None:
+        if mask.dtype != torch.bool or tuple(mask.shape) != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
+            raise TfmqError(f"{name}: mask must be bool [{B}, {Tk}] (True: attend) with unit key stride, got {mask.dtype} {tuple(mask.shape)}")
+        a.mask, a.mask_bs = mask.data_ptr(), mask.stride(0)
+    return d_, a
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, scale: float, kv_heads: Optional[int] = None,
+                    q_lens: Optional[torch.Tensor] = None, kv_lens: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                    want_lse: bool = False):
+    """softmax(scale q k^T) v of Tq query tokens over Tk states of an encoder (CrossAttention.forward with `context` and `mask`,
+    ldm/modules/attention.py:168-194).  q [B, Tq, heads * d], k / v [B, Tk, kv_heads * d] fp16 or bf16, views with unit channel stride and 16-byte
+    aligned rows (the halves of a fused k | v projection, a batch expanded with stride 0); d a multiple of 8, at most 160.  Query head h reads
+    key head h // (heads // kv_heads).
+
+    kv_lens: int32 [B], item b's first kv_lens[b] states are real (values outside [0, Tk] are clamped).  mask: bool [B, Tk], True: attend (both
+    may be given: a key needs both).  q_lens: int32 [B], rows from q_lens[b] on are not computed.  A row that keeps no key, or lies behind
+    q_lens, is zero (the reference's masked_fill with the lowest value averages all states instead).  Nothing a dropped key or row holds, NaN
+    and infinities included, reaches a result.  Lengths and mask are read by the kernels on the current stream.
+
+    -> o [B, Tq, heads * d], or (o, lse fp32 [B, heads, Tq]) with lse = log sum exp(scale q k^T) over the kept keys, -inf where there is none."""
+    d_, a = _xattn_desc(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, "cross_attention")
+    o = _alloc(tuple(q.shape), dtype=q.dtype, device=q.device)
+    lse = _alloc(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device) if want_lse else None
+    if q.numel() == 0 or a.Tk == 0:
+        o.zero_()
+        if want_lse:
+            lse.fill_(float("-inf"))
+        return (o, lse) if want_lse else o
+    h = handle(d_)
+    a.nsplit = h.lib.tfmq_xattn_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk)
+    ws = _alloc(a.nsplit * a.B * a.H * a.Tq * (a.d + 2), dtype=torch.float32, device=q.device) if a.nsplit > 1 else None
+    a.o, a.lse, a.ws = o.data_ptr(), (lse.data_ptr() if want_lse else None), (ws.data_ptr() if ws is not None else None)
+    h.call("xattn_fwd", C.byref(a), _stream(d_))
+    return (o, lse) if want_lse else o
+
+
+def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, g_o: torch.Tensor, heads: int,
+                        scale: float, kv_heads: Optional[int] = None, q_lens: Optional[torch.Tensor] = None,
+                        kv_lens: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
+    """-> (dq, dk, dv) of cross_attention for the upstream gradient g_o [B, Tq, heads * d], given its o and lse; contiguous, in the operands'
+    type.  dk / dv of shared key heads are summed over their query heads; dropped keys and rows have zeros; a k or v that was expanded over the
+    batch gets its gradient per item.  The same bits on every call."""
+    d_, a = _xattn_desc(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, "cross_attention_bwd")
+    _same_device(d_, o=o, lse=lse, g_o=g_o)
+    a.o, a.o_bs, a.o_ts = _xattn_view(o, a.Tq, a.H * a.d, a.B, q.dtype, "cross_attention_bwd o")
+    a.go, a.go_bs, a.go_ts = _xattn_view(g_o, a.Tq, a.H * a.d, a.B, q.dtype, "cross_attention_bwd g_o")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Tq) or not lse.is_contiguous():
+        raise TfmqError(f"cross_attention_bwd: lse must be contiguous fp32 [{a.B}, {a.H}, {a.Tq}], got {lse.dtype} {tuple(lse.shape)}")
+    dq = _alloc(tuple(q.shape), dtype=q.dtype, device=q.device)
+    dk = _alloc(tuple(k.shape), dtype=q.dtype, device=q.device)
+    dv = _alloc(tuple(v.shape), dtype=q.dtype, device=q.device)
+    if q.numel() == 0 or a.Tk == 0:
+        for t in (dq, dk, dv):
+            t.zero_()
+        return dq, dk, dv
+    h = handle(d_)
+    a.nsplit = h.lib.tfmq_xattn_bwd_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk, a.d)
+    rows = (2 * a.B * a.H * a.Tq + 3) // 4 * 4
+    ws = _alloc(rows + (2 * a.nsplit * dk.numel() if a.nsplit > 1 else 0), dtype=torch.float32, device=q.device)
+    a.lse, a.dq, a.dk, a.dv, a.ws = lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr()
+    h.call("xattn_bwd", C.byref(a), _stream(d_))
+    return dq, dk, dv
