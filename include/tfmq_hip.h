@@ -618,13 +618,17 @@ int tfmq_axpy(tfmq_handle h, float* y, const float* x, float a, size_t n, void* 
 int tfmq_quantize_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, int by_column, uint8_t* q, float* s, void* stream);
 /* w fp32 [N][K] contiguous -> q [N][Kp], its transpose qt [K][128 ceil(N / 128)], s [ceil(N / 128)][Kb]: one scale per 128 x 128 */
 int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint8_t* q, uint8_t* qt, float* s, void* stream);
-/* y[m][n] = sum_kb sa[kb][m] sb(n, kb) (sum_{k in kb} a[m][k] b[n][k]) + bias[n], y [M][N] contiguous of y_dtype, fp32 sums;
- * a [M][128 Kb], b [N][128 Kb], 16-byte aligned.  sb(n, kb) = sb[(n / 128) * sbn + kb * sbk], or (sb_row, y fp32 only) sb[kb * N + n]. */
-int tfmq_gemm_fp8(tfmq_handle h, const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, long sbn, long sbk, int sb_row,
-                  const float* bias, void* y, int y_dtype, long M, int N, int Kb, void* stream);
-/* the same product for few rows (M <= 1024) in one launch: x is quantised on the way in (bit-identical operands) */
-int tfmq_linear_fp8_small(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* w, const float* ws, const float* bias,
-                          void* y, int y_dtype, int N, void* stream);
+/* y[m][n] = sum_kb sx[kb][m] sw(n / 128, kb) (sum_{k in kb} qx[m][k] qw[n][k]) + bias[n], y [M][N] contiguous of y_dtype (16-byte aligned), fp32 sums.
+ * x [M][K] of dtype, row stride ld, is quantised here; or x = NULL and xq / xs as tfmq_quantize_fp8 leaves them.  w as tfmq_pack_w_fp8 leaves it; the
+ * scale of (column block nb, k block kb) at ws[nb * ws_n + kb * ws_k].  work: tfmq_linear_fp8_ws_bytes (0 for up to 32 rows: one launch). */
+size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K);
+int tfmq_linear_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* xq, const float* xs, const uint8_t* w,
+                    const float* ws, long ws_n, long ws_k, const float* bias, void* y, int y_dtype, int N, void* work, void* stream);
+/* gx [M][K] (of gy's type) = product of gy, quantised by rows, with the transposed weight wt (tfmq_pack_w_fp8's qt; ws its s [ceil(N / 128)][Kb]);
+ * gw fp32 [N][K] = sum over tokens, both operands quantised by columns.  Either output may be NULL.  Deterministic. */
+size_t tfmq_linear_fp8_bwd_ws_bytes(tfmq_handle h, long M, int N, int K, int want_gx, int want_gw);
+int tfmq_linear_fp8_bwd(tfmq_handle h, const void* x, int x_dtype, long x_ld, const void* gy, int gy_dtype, long gy_ld, long M, int N, int K,
+                        const uint8_t* wt, const float* ws, void* gx, float* gw, void* work, void* stream);
 
 /* ---- K18: cross attention of Tq query tokens to Tk states of an encoder (ldm/modules/attention.py:168-194 with `context` and `mask`), fp16 / bf16,
  * per-item lengths, a key mask, H query heads over G shared key / value heads ---------------------------------------------------------

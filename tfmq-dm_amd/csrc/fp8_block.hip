@@ -95,40 +95,91 @@ __global__ __launch_bounds__(256) void k_quant_rows(const typename Elem<DT>::typ
   }
 }
 
-// ---- columns: x [M][K] -> q [K][Mp] with one scale per column and block of 128 rows, s [Mb][K].  A workgroup takes 128 rows x 64 columns:
-// thread (column c = tid & 63, row quarter tid >> 6) holds 32 values, the column's maximum meets in LDS, the bytes are transposed through LDS
-// and leave as 128-byte rows.
-template <int DT>
-__global__ __launch_bounds__(256) void k_quant_cols(const typename Elem<DT>::type* __restrict__ x, long M, int K, long ld, uint8_t* __restrict__ q,
-                                                    float* __restrict__ s, long Mp) {
-  __shared__ unsigned amax[4][64];
-  __shared__ __attribute__((aligned(16))) unsigned bytes[64][33];
-  const int nkt = (K + 63) / 64;
-  const long mb = blockIdx.x / nkt;
-  const int k0 = static_cast<int>(blockIdx.x % nkt) * 64;
-  const int c = threadIdx.x & 63, qr = threadIdx.x >> 6;
-  const int k = k0 + c;
-  float v[32];
-  unsigned a = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const long m = mb * 128 + qr * 32 + i;
-    v[i] = (k < K && m < M) ? static_cast<float>(x[m * ld + k]) : 0.0f;
-    a = max(a, mag_bits(v[i]));
+// ---- columns: x [M][K] -> qc [K][Mp] with one scale per column and block of 128 rows, sc [Mb][K]; the row form (q, s as above) from the same
+// values where it is wanted too, so that an upstream gradient, which both products read, is read once.  A workgroup takes 128 rows x 128 columns, a
+// thread 8 x 8 of them; the columns' maxima meet in LDS, the bytes are transposed through LDS and leave as 128-byte rows.  HBM-bound.
+struct QuantTileP {
+  const void* x;
+  int dt, vec;                 // type code; rows 16-byte aligned and K % 8 == 0
+  long M, ld;
+  int K, Kb;
+  uint8_t *q, *qc;
+  float *s, *sc;               // q, s null: columns only
+};
+__device__ __forceinline__ void load8_any(const QuantTileP& p, long row, int c, float (&v)[8]) {
+  if (p.dt == DT_F32) {
+    const float* x = static_cast<const float*>(p.x) + row;
+    p.vec ? load8<DT_F32, true>(x, c, p.K, v) : load8<DT_F32, false>(x, c, p.K, v);
+  } else if (p.dt == DT_F16) {
+    const _Float16* x = static_cast<const _Float16*>(p.x) + row;
+    p.vec ? load8<DT_F16, true>(x, c, p.K, v) : load8<DT_F16, false>(x, c, p.K, v);
+  } else {
+    const __bf16* x = static_cast<const __bf16*>(p.x) + row;
+    p.vec ? load8<DT_BF16, true>(x, c, p.K, v) : load8<DT_BF16, false>(x, c, p.K, v);
   }
-  amax[qr][c] = a;
-  __syncthreads();
-  a = max(max(amax[0][c], amax[1][c]), max(amax[2][c], amax[3][c]));
-  const float2 sc = block_scale(a);
-  if (qr == 0 && k < K) s[mb * K + k] = sc.y;
+}
+__device__ __forceinline__ void quant_tile(const QuantTileP& p, int t) {
+  __shared__ unsigned amax[16][128];
+  __shared__ __attribute__((aligned(16))) unsigned bytes[128][33];
+  const long mb = t / p.Kb, Mp = (p.M + 127) / 128 * 128;
+  const int kb = t % p.Kb;
+  const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, k = kb * 128 + cg * 8;
+  const long m0 = mb * 128 + rg * 8;
+  float v[8][8];
+  unsigned cm[8] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bytes[c][qr * 8 + i] = pack4_f8(v[4 * i] * sc.x, v[4 * i + 1] * sc.x, v[4 * i + 2] * sc.x, v[4 * i + 3] * sc.x);
+  for (int r = 0; r < 8; ++r) {
+    if (m0 + r < p.M) {
+      load8_any(p, (m0 + r) * p.ld, k, v[r]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[r][e] = 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cm[e] = max(cm[e], mag_bits(v[r][e]));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax[rg][cg * 8 + e] = cm[e];
+  if (p.q) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      unsigned a = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = max(a, mag_bits(v[r][e]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) a = max(a, static_cast<unsigned>(__shfl_xor(static_cast<int>(a), o, 16)));
+      const float2 sc = block_scale(a);
+      if (m0 + r < p.M) {
+        uint2 w;
+        w.x = pack4_f8(v[r][0] * sc.x, v[r][1] * sc.x, v[r][2] * sc.x, v[r][3] * sc.x);
+        w.y = pack4_f8(v[r][4] * sc.x, v[r][5] * sc.x, v[r][6] * sc.x, v[r][7] * sc.x);
+        *reinterpret_cast<uint2*>(p.q + ((m0 + r) * p.Kb + kb) * 128 + cg * 8) = w;
+        if (cg == 0) p.s[static_cast<long>(kb) * p.M + m0 + r] = sc.y;
+      }
+    }
+  }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int e = 0; e < 8; ++e) {
+    unsigned a = 0;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) a = max(a, amax[g][cg * 8 + e]);
+    const float2 sc = block_scale(a);
+    if (rg == 0 && k + e < p.K) p.sc[mb * p.K + k + e] = sc.y;
+    bytes[cg * 8 + e][rg * 2] = pack4_f8(v[0][e] * sc.x, v[1][e] * sc.x, v[2][e] * sc.x, v[3][e] * sc.x);
+    bytes[cg * 8 + e][rg * 2 + 1] = pack4_f8(v[4][e] * sc.x, v[5][e] * sc.x, v[6][e] * sc.x, v[7][e] * sc.x);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
     const int idx = threadIdx.x + i * 256, row = idx >> 5, w = idx & 31;
-    if (k0 + row < K) *reinterpret_cast<unsigned*>(q + static_cast<long>(k0 + row) * Mp + mb * 128 + w * 4) = bytes[row][w];
+    if (kb * 128 + row < p.K) *reinterpret_cast<unsigned*>(p.qc + static_cast<long>(kb * 128 + row) * Mp + mb * 128 + w * 4) = bytes[row][w];
   }
+}
+// one launch for up to two tensors (n0 tiles of the first)
+__global__ __launch_bounds__(256) void k_quant_cols(QuantTileP a, QuantTileP b, int n0) {
+  const int t = blockIdx.x;
+  quant_tile(t < n0 ? a : b, t < n0 ? t : t - n0);
 }
 
 // ---- weights: w fp32 [N][K] -> q [N][Kp] and its transpose qt [K][Np], s [Nb][Kb]; one workgroup per 128 x 128 block, run once per layer
@@ -201,6 +252,7 @@ struct GemmF8P {
   long M;
   int N, Kb;
   int tm, tn;                  // tiles along M, N
+  int nslice;                  // slices of the Kb blocks: slice s writes fp32 partials at y + s * M * N
 };
 
 // one 16-byte piece of a 128-byte operand row lives at slot (piece ^ key(row)): 8 consecutive lanes of a fragment read hit 8 different slots
@@ -234,179 +286,286 @@ __device__ __forceinline__ void store_run(typename Elem<YDT>::type* p, const flo
 
 // The product.  The MFMA computes W_tile X_tile^T, so a lane owns ONE row m of the output (its scale is one register) and its 16 accumulators are
 // columns n; the rows of W enter the fragment in the order n = 16 h + 4 a + c for fragment row 8 a + 4 h + c, so those 16 columns are consecutive.
-// Operand tiles of one block (128 bytes a row) travel by LDS-DMA into two stages, the next one in flight while this one is multiplied.
-template <int BM, int BN, int WM, int WN, int YDT, bool SBROW>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_gemm_f8(GemmF8P p) {
+// Operand tiles of one block (128 bytes a row) travel by LDS-DMA into two stages, the next one in flight while this one is multiplied.  A workgroup
+// walks over its tiles (or, sliced, one K range of a tile) as one sequence of blocks: the next tile's first stage is under way while the results of
+// this one are rounded and stored.
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), WPS) void k_gemm_f8(GemmF8P p) {
   constexpr int NWM = BM / WM, NWN = BN / WN, NW = NWM * NWN, TM = WM / 32, TN = WN / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int STAGE = (BM + BN) * 128;
   using YT = typename Elem<YDT>::type;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  using F = Frag<YDT == DT_F32>;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & 31, hh = lane >> 5;
   const int wm = wid % NWM, wn = wid / NWM;
-  const int tile = xcd_tile_id();
-  const long m0 = static_cast<long>(tile % p.tm) * BM;
-  const int n0 = (tile / p.tm) * BN;
   const long Kp = static_cast<long>(p.Kb) * 128;
+  const int ntile = p.tm * p.tn;
+  float* sS = reinterpret_cast<float*>(smem + 2 * STAGE) + wid * WN;          // SBROW: this wave's column scales of a block
 
-  // ---- LDS-DMA plan: instruction i of a wave moves 8 rows x 128 bytes; rows [0, BN) of a stage are W, [BN, BN + BM) X
+  // ---- LDS-DMA plan: instruction i of a wave moves 8 rows x 128 bytes; rows [0, BN) of a stage are W, [BN, BN + BM) X; a wave moves one of them
   constexpr int NI = (BM + BN) / 8 / NW;
-  static_assert((BM + BN) % (8 * NW) == 0 && BN % 8 == 0, "whole rows per wave instruction");
-  const uint8_t* src[NI];
+  static_assert((BM + BN) % (8 * NW) == 0 && BN % (8 * NI) == 0, "whole rows per wave instruction, one operand per wave");
+  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem)) + wid * NI * 1024;
+  const bool is_w = wid * NI * 8 < BN;
+  unsigned voff[NI];
+  const uint8_t* src = nullptr;
+  long m0 = 0;
+  int n0 = 0;
+  auto place = [&](int tile) {
+    // neighbouring workgroups of an XCD share rows and columns: groups of 8 row tiles walk the columns
+    const int gsz = 8 * p.tn, grp = tile / gsz, first = grp * 8, rows = min(p.tm - first, 8), in = tile - grp * gsz;
+    m0 = static_cast<long>(first + in % rows) * BM;
+    n0 = (in / rows) * BN;
+    src = uniform_ptr(is_w ? p.b + n0 * Kp : p.a + m0 * Kp);
+    const unsigned last = __builtin_amdgcn_readfirstlane(static_cast<int>(is_w ? p.N - 1 - n0 : min(static_cast<long>(BM), p.M - m0) - 1));
+    const int r0 = (is_w ? wid : wid - BN / (8 * NI)) * NI * 8 + (lane >> 3);
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int row = (wid * NI + i) * 8 + (lane >> 3), slot = lane & 7;
-    if (row < BN) {
-      const int n = min(n0 + row, p.N - 1);
-      src[i] = p.b + static_cast<long>(n) * Kp + ((slot ^ key_w(row)) << 4);
-    } else {
-      const int r = row - BN;
-      const long m = min(m0 + r, p.M - 1);
-      src[i] = p.a + m * Kp + ((slot ^ key_x(r)) << 4);
+    for (int i = 0; i < NI; ++i) {
+      const int r = r0 + 8 * i;
+      voff[i] = min(static_cast<unsigned>(r), last) * static_cast<unsigned>(Kp) + (((lane & 7) ^ (is_w ? key_w(r) : key_x(r))) << 4);
+      asm volatile("" : "+v"(voff[i]));          // kept, not recomputed for every block
     }
-  }
-  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem));
-  auto fetch = [&](int kb, int st) {
-#pragma unroll
-    for (int i = 0; i < NI; ++i) glds16(src[i] + static_cast<long>(kb) * 128, __builtin_amdgcn_readfirstlane(lds0 + st * STAGE + (wid * NI + i) * 1024));
   };
-  long mrow[TM];
+  auto fetch = [&](int kb, int st) {
+    const uint8_t* base = uniform_ptr(src + static_cast<long>(kb) * 128);
+    const unsigned dst = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE);
 #pragma unroll
-  for (int t = 0; t < TM; ++t) mrow[t] = min(m0 + wm * WM + t * 32 + j, p.M - 1);
-  const int nbase = n0 + wn * WN;
-
-  v16f acc[TN][TM];
-#pragma unroll
-  for (int u = 0; u < TN; ++u)
-#pragma unroll
-    for (int t = 0; t < TM; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[u][t][r] = 0.0f;
-
-  float sx[TM], sxn[TM] = {};
+    for (int i = 0; i < NI; ++i)
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff[i]), "s"(base), "s"(dst + i * 1024) : "memory", "m0");
+  };
+  // this workgroup's slice of the blocks, and its tiles
+  const int sl = p.nslice > 1 ? static_cast<int>(blockIdx.x) % p.nslice : 0;
+  const int per = (p.Kb + p.nslice - 1) / p.nslice, k_lo = sl * per, k_hi = min(p.Kb, k_lo + per);
+  int tile = p.nslice > 1 ? static_cast<int>(blockIdx.x) / p.nslice : xcd_tile_id();
+  const int stride = p.nslice > 1 ? ntile : static_cast<int>(gridDim.x);
+  if (tile >= ntile) return;
   const int nb_last = (p.N - 1) >> 7;
+  static_assert(!SBROW || WN == 64, "a lane per column");
+  static_assert(128 % WN == 0 && BN % 128 == 0, "a wave's columns share a scale");
+
+  float sx[TM], sxn[TM] = {}, sbn = 0.0f;          // row scales (times the column block's) of this block; what has been asked for of the next
+  auto scales = [&](int kb) {
+    const float* row = p.sa + static_cast<long>(kb) * p.M;
 #pragma unroll
-  for (int t = 0; t < TM; ++t) sx[t] = p.sa[mrow[t]];
-  fetch(0, 0);
-  for (int kb = 0; kb < p.Kb; ++kb) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                 // this stage has arrived for every wave, and every wave is through with the other one
-    if (kb + 1 < p.Kb) {
+    for (int t = 0; t < TM; ++t) sxn[t] = row[min(m0 + wm * WM + t * 32 + j, p.M - 1)];
+    // (a wave's columns lie in one block of 128.  The scales travel a block ahead and are first touched behind the wait for the stage: a use, or a
+    // load, between the LDS-DMA and that wait would wait for the LDS-DMA)
+    sbn = SBROW ? p.sb[static_cast<long>(kb) * p.N + min(n0 + wn * WN + lane, p.N - 1)]
+                : p.sb[static_cast<long>(min((n0 + wn * WN) >> 7, nb_last)) * p.sbn + kb * p.sbk];
+  };
+  // fragment addresses inside a stage: four 16-byte pieces of a row (the sub-tiles are immediates)
+  const int rw = wn * WN + 16 * ((j >> 2) & 1) + 4 * (j >> 3) + (j & 3), rx = wm * WM + j;          // fragment row j of W holds row rw
+  unsigned pw[4], px[4];
 #pragma unroll
-      for (int t = 0; t < TM; ++t) sxn[t] = p.sa[static_cast<long>(kb + 1) * p.M + mrow[t]];
-      fetch(kb + 1, (kb + 1) & 1);
-    }
-    const unsigned char* sW = smem + (kb & 1) * STAGE;
-    const unsigned char* sX = sW + BN * 128;
-    using F = Frag<YDT == DT_F32>;
-    F xf[TM][2];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) {
-      const int r = wm * WM + t * 32 + j;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint4 w = *reinterpret_cast<const uint4*>(sX + r * 128 + (((s * 4 + hh * 2 + e) ^ key_x(r)) << 4));
-          xf[t][s].set(4 * e, w.x); xf[t][s].set(4 * e + 1, w.y); xf[t][s].set(4 * e + 2, w.z); xf[t][s].set(4 * e + 3, w.w);
-        }
-        xf[t][s].done();
-      }
-    }
+  for (int q = 0; q < 4; ++q) {
+    const int piece = (q >> 1) * 4 + hh * 2 + (q & 1);
+    pw[q] = rw * 128 + ((piece ^ key_w(rw)) << 4);
+    px[q] = BN * 128 + rx * 128 + ((piece ^ key_x(rx)) << 4);
+  }
+  v16f acc[TN][TM];
+  // one block of a stage: products into acc
+  auto block = [&](int st) {
+    const unsigned char* S = smem + st * STAGE;
+    F wf[TN][2];
+    float swr[SBROW ? TN : 1][16];
 #pragma unroll
     for (int u = 0; u < TN; ++u) {
-      const int i = 16 * ((j >> 2) & 1) + 4 * (j >> 3) + (j & 3);          // fragment row j holds this row of the 32
-      const int r = wn * WN + u * 32 + i;
-      F wf[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint4 w = *reinterpret_cast<const uint4*>(sW + r * 128 + (((s * 4 + hh * 2 + e) ^ key_w(r)) << 4));
-          wf[s].set(4 * e, w.x); wf[s].set(4 * e + 1, w.y); wf[s].set(4 * e + 2, w.z); wf[s].set(4 * e + 3, w.w);
-        }
-        wf[s].done();
+      for (int q = 0; q < 4; ++q) {
+        const uint4 w = *reinterpret_cast<const uint4*>(S + pw[q] + u * 32 * 128);
+        F& f = wf[u][q >> 1];
+        f.set(4 * (q & 1), w.x); f.set(4 * (q & 1) + 1, w.y); f.set(4 * (q & 1) + 2, w.z); f.set(4 * (q & 1) + 3, w.w);
       }
-      float sw = 0.0f, swr[16];
+      wf[u][0].done();
+      wf[u][1].done();
       if constexpr (SBROW) {
 #pragma unroll
-        for (int r2 = 0; r2 < 16; ++r2) swr[r2] = p.sb[static_cast<long>(kb) * p.N + min(nbase + u * 32 + 16 * hh + r2, p.N - 1)];
-      } else {
-        sw = p.sb[static_cast<long>(min((nbase + u * 32) >> 7, nb_last)) * p.sbn + kb * p.sbk];
-      }
-#pragma unroll
-      for (int t = 0; t < TM; ++t) {
-        v16f z;
-#pragma unroll
-        for (int r2 = 0; r2 < 16; ++r2) z[r2] = 0.0f;
-        const v16f d = F::mul(wf[1], xf[t][1], F::mul(wf[0], xf[t][0], z));
-        if constexpr (SBROW) {
-#pragma unroll
-          for (int r2 = 0; r2 < 16; ++r2) acc[u][t][r2] = __builtin_fmaf(d[r2], sx[t] * swr[r2], acc[u][t][r2]);
-        } else {
-          const float f = sx[t] * sw;
-#pragma unroll
-          for (int r2 = 0; r2 < 16; ++r2) acc[u][t][r2] = __builtin_fmaf(d[r2], f, acc[u][t][r2]);
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const float4 v = *reinterpret_cast<const float4*>(sS + u * 32 + 16 * hh + 4 * q4);
+          swr[u][4 * q4] = v.x; swr[u][4 * q4 + 1] = v.y; swr[u][4 * q4 + 2] = v.z; swr[u][4 * q4 + 3] = v.w;
         }
       }
     }
 #pragma unroll
-    for (int t = 0; t < TM; ++t) sx[t] = sxn[t];
+    for (int t = 0; t < TM; ++t) {
+      F xf[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint4 w = *reinterpret_cast<const uint4*>(S + px[q] + t * 32 * 128);
+        F& f = xf[q >> 1];
+        f.set(4 * (q & 1), w.x); f.set(4 * (q & 1) + 1, w.y); f.set(4 * (q & 1) + 2, w.z); f.set(4 * (q & 1) + 3, w.w);
+      }
+      xf[0].done();
+      xf[1].done();
+#pragma unroll
+      for (int u = 0; u < TN; ++u) {
+        const v16f z = {};
+        const v16f d = F::mul(wf[u][1], xf[1], F::mul(wf[u][0], xf[0], z));
+        if constexpr (SBROW) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[u][t][r] = __builtin_fmaf(d[r], sx[t] * swr[u][r], acc[u][t][r]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[u][t][r] = __builtin_fmaf(d[r], sx[t], acc[u][t][r]);
+        }
+      }
+    }
+  };
+
+  place(tile);
+  scales(min(k_lo, p.Kb - 1));
+  if (k_lo < k_hi) fetch(k_lo, 0);
+  int st = 0;
+  bool stores = false;          // the last tile's stores (at least TM TN 2 instructions a wave) may still be under way
+  for (; tile < ntile; tile += stride) {
+#pragma unroll
+    for (int u = 0; u < TN; ++u)
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[u][t][r] = 0.0f;
+    const long mt = m0;
+    const int nbase = n0 + wn * WN;
+    const bool full = (p.N * sizeof(YT)) % 16 == 0 && m0 + BM <= p.M && n0 + BN <= p.N;
+    for (int kb = k_lo; kb < k_hi; ++kb) {
+      if (stores) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TM * TN * (YDT == DT_F32 ? 4 : 2)) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      stores = false;
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+        sx[t] = SBROW ? sxn[t] : sxn[t] * sbn;
+        asm volatile("" : "+v"(sx[t]));          // here, not behind the next LDS-DMA
+      }
+      if constexpr (SBROW) sS[lane] = sbn;
+      LDS_BARRIER();                   // this stage has arrived for every wave, and every wave is through with the other one
+      if (kb + 1 < k_hi) {
+        scales(kb + 1);
+        fetch(kb + 1, st ^ 1);
+      } else if (tile + stride < ntile) {
+        place(tile + stride);
+        scales(k_lo);
+        fetch(k_lo, st ^ 1);
+      }
+      block(st);
+      st ^= 1;
+    }
+    // ---- lane (row m, half hh) holds columns u * 32 + 16 hh + (0 .. 15): out through LDS (this wave's part of the stage just multiplied), 32 rows x
+    // 128 bytes at a time, so that the stores are whole lines
+    YT* out = reinterpret_cast<YT*>(p.y) + (p.nslice > 1 ? static_cast<long>(sl) * p.M * p.N : 0);
+    constexpr int CW = 128 / static_cast<int>(sizeof(YT)), UC = CW / 32, SR = 144, PE = 16 / static_cast<int>(sizeof(YT));
+    static_assert(NW * 32 * SR <= STAGE, "the waves' store buffers fit a stage");
+    const bool vec = (p.N * sizeof(YT)) % 16 == 0;
+    LDS_BARRIER();                     // every wave is through with that stage
+    unsigned char* sO = smem + (st ^ 1) * STAGE + wid * 32 * SR;
+#pragma unroll
+    for (int c = 0; c < WN / CW; ++c) {
+      const int nc = nbase + c * CW;
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+#pragma unroll
+        for (int u = 0; u < UC; ++u) {
+          float v[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[r] = acc[c * UC + u][t][r];
+          if (p.bias) {
+            const int nl = nc + u * 32 + 16 * hh;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] += p.bias[min(nl + r, p.N - 1)];
+          }
+          store_run<YDT>(reinterpret_cast<YT*>(sO + j * SR) + u * 32 + 16 * hh, v, 16, true);
+        }
+        const long mb = mt + wm * WM + t * 32;
+        if (vec) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 3), pc = lane & 7;
+            const uint4 w = *reinterpret_cast<const uint4*>(sO + r * SR + pc * 16);
+            if (full || (mb + r < p.M && nc + pc * PE < p.N)) *reinterpret_cast<uint4*>(out + (mb + r) * p.N + nc + pc * PE) = w;
+          }
+        } else {
+#pragma unroll 1
+          for (int e = lane; e < 32 * CW; e += 64) {
+            const int r = e / CW, n = e % CW;
+            if (mb + r < p.M && nc + n < p.N) out[(mb + r) * p.N + nc + n] = reinterpret_cast<const YT*>(sO + r * SR)[n];
+          }
+        }
+      }
+    }
+    stores = full;
   }
-  // ---- lane (row m, half hh) holds columns u * 32 + 16 hh + (0 .. 15)
-  const bool vec = (p.N * sizeof(YT)) % 16 == 0;
-#pragma unroll
-  for (int t = 0; t < TM; ++t) {
-    const long m = m0 + wm * WM + t * 32 + j;
-    if (m >= p.M) continue;
-#pragma unroll
-    for (int u = 0; u < TN; ++u) {
-      const int n = nbase + u * 32 + 16 * hh;
-      const int cnt = min(16, p.N - n);
-      if (cnt <= 0) continue;
-      float v[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = acc[u][t][r] + ((p.bias && r < cnt) ? p.bias[n + r] : 0.0f);
-      store_run<YDT>(reinterpret_cast<YT*>(p.y) + m * p.N + n, v, cnt, vec);
+}
+
+// slices of the K axis, added in order; four outputs a thread
+__global__ __launch_bounds__(256) void k_sum_slices(const float* __restrict__ part, float* __restrict__ y, long n, int nslice) {
+  const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  if (n % 4 == 0) {
+    float4 a = make_float4(0, 0, 0, 0);
+    for (int s = 0; s < nslice; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(part + s * n + i);
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    *reinterpret_cast<float4*>(y + i) = a;
+  } else {
+    for (long e = i; e < min(n, i + 4); ++e) {
+      float a = 0.0f;
+      for (int s = 0; s < nslice; ++s) a += part[s * n + e];
+      y[e] = a;
     }
   }
 }
 
-template <int BM, int BN, int WM, int WN, int YDT, bool SBROW>
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
 int launch_gemm(tfmq_handle h, GemmF8P p, hipStream_t st) {
-  constexpr int smem = 2 * (BM + BN) * 128;
-  auto kern = &k_gemm_f8<BM, BN, WM, WN, YDT, SBROW>;
+  constexpr int NW = (BM / WM) * (BN / WN), smem = 2 * (BM + BN) * 128 + (SBROW ? NW * WN * 4 : 0);
+  auto kern = &k_gemm_f8<BM, BN, WM, WN, YDT, SBROW, WPS>;
   TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
   p.tm = ceil_div(p.M, BM);
   p.tn = ceil_div(p.N, BN);
-  const long nb = static_cast<long>(p.tm) * p.tn;
-  TFMQ_CHECK_ARG(h, nb < (1L << 31), "gemm_fp8: too many tiles");
-  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nb)), dim3(64 * (BM / WM) * (BN / WN)), smem, st, p);
+  const long nt = static_cast<long>(p.tm) * p.tn;
+  TFMQ_CHECK_ARG(h, nt * 8 < (1L << 31), "gemm_fp8: too many tiles");
+  const long room = static_cast<long>(h->cu_count) * (4 * WPS / NW);          // resident workgroups
+  const long nb = p.nslice > 1 ? nt * p.nslice : (nt < room ? nt : room);
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nb)), dim3(64 * NW), smem, st, p);
   TFMQ_LAUNCH_CHECK(h);
   return TFMQ_OK;
 }
 
-template <int DT>
-int launch_quant_rows(tfmq_handle h, const void* x, long M, int K, long ld, uint8_t* q, float* s, hipStream_t st) {
-  using T = typename Elem<DT>::type;
+bool rows_aligned(const void* x, int dtype, int K, long ld) {
+  return K % 8 == 0 && (ld * (dtype == DT_F32 ? 4 : 2)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+}
+// by type code and alignment: f(integral_constant<dtype>, bool_constant<vec>)
+template <typename F>
+int for_input(const void* x, int dtype, int K, long ld, F f) {
+  const bool vec = rows_aligned(x, dtype, K, ld);
+  auto pick = [&](auto d) { return vec ? f(d, std::true_type{}) : f(d, std::false_type{}); };
+  if (dtype == DT_F32) return pick(std::integral_constant<int, DT_F32>{});
+  return dtype == DT_F16 ? pick(std::integral_constant<int, DT_F16>{}) : pick(std::integral_constant<int, DT_BF16>{});
+}
+QuantTileP quant_tiles(const void* x, int dtype, long M, int K, long ld, uint8_t* q, float* s, uint8_t* qc, float* sc) {
+  return QuantTileP{x, dtype, rows_aligned(x, dtype, K, ld), M, ld, K, (K + 127) / 128, q, qc, s, sc};
+}
+
+int launch_quant_cols(tfmq_handle h, const QuantTileP& a, const QuantTileP* b, hipStream_t st) {
+  auto tiles = [](const QuantTileP& p) { return (p.M + 127) / 128 * p.Kb; };
+  const long na = tiles(a), n = na + (b ? tiles(*b) : 0);
+  TFMQ_CHECK_ARG(h, n < (1L << 31), "quantize_fp8: too many blocks");
+  hipLaunchKernelGGL(k_quant_cols, dim3(static_cast<unsigned>(n)), dim3(256), 0, st, a, b ? *b : a, static_cast<int>(na));
+  TFMQ_LAUNCH_CHECK(h);
+  return TFMQ_OK;
+}
+
+int launch_quant_rows(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, uint8_t* q, float* s, hipStream_t st) {
   const int Kb = (K + 127) / 128;
   const long nt = (M + 15) / 16 * Kb;
   const unsigned grid = static_cast<unsigned>(nt < 65536 ? nt : 65536);
-  const bool vec = K % 8 == 0 && (ld * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  if (vec) hipLaunchKernelGGL((k_quant_rows<DT, true>), dim3(grid), dim3(256), 0, st, static_cast<const T*>(x), M, K, ld, q, s, Kb);
-  else hipLaunchKernelGGL((k_quant_rows<DT, false>), dim3(grid), dim3(256), 0, st, static_cast<const T*>(x), M, K, ld, q, s, Kb);
-  TFMQ_LAUNCH_CHECK(h);
-  return TFMQ_OK;
-}
-
-template <int DT>
-int launch_quant_cols(tfmq_handle h, const void* x, long M, int K, long ld, uint8_t* q, float* s, hipStream_t st) {
-  using T = typename Elem<DT>::type;
-  const long Mb = (M + 127) / 128, nb = Mb * ((K + 63) / 64);
-  TFMQ_CHECK_ARG(h, nb < (1L << 31), "quantize_fp8: too many blocks");
-  hipLaunchKernelGGL((k_quant_cols<DT>), dim3(static_cast<unsigned>(nb)), dim3(256), 0, st, static_cast<const T*>(x), M, K, ld, q, s, Mb * 128);
-  TFMQ_LAUNCH_CHECK(h);
-  return TFMQ_OK;
+  return for_input(x, dtype, K, ld, [&](auto d, auto v) {
+    using T = typename Elem<decltype(d)::value>::type;
+    hipLaunchKernelGGL((k_quant_rows<decltype(d)::value, decltype(v)::value>), dim3(grid), dim3(256), 0, st, static_cast<const T*>(x), M, K, ld, q, s, Kb);
+    TFMQ_LAUNCH_CHECK(h);
+    return TFMQ_OK;
+  });
 }
 
 // ---- few rows (M <= 32 a workgroup): one launch, W read once straight into the fragments, the activations quantised on the way in.  Eight waves
@@ -417,7 +576,8 @@ struct SmallF8P {
   long ld;
   int M, K;
   const uint8_t* w;
-  const float* ws;             // [Nb][Kb]
+  const float* ws;             // scale of (column block, k block) at ws[n * ws_n + k * ws_k]
+  long ws_n, ws_k;
   const float* bias;
   void* y;
   int N, Kb;
@@ -432,7 +592,7 @@ __global__ __launch_bounds__(512) void k_linear_f8_small(SmallF8P p) {
   const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32;
   const T* xrow = static_cast<const T*>(p.x) + static_cast<long>(min(m0 + j, p.M - 1)) * p.ld;
   const uint8_t* wrow = p.w + static_cast<long>(min(n0 + j, p.N - 1)) * p.Kb * 128;
-  const float* wsc = p.ws + static_cast<long>(n0 >> 7) * p.Kb;
+  const float* wsc = p.ws + static_cast<long>(n0 >> 7) * p.ws_n;
   v16f acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
@@ -442,7 +602,7 @@ __global__ __launch_bounds__(512) void k_linear_f8_small(SmallF8P p) {
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int e = 0; e < 2; ++e) wv[2 * s + e] = *reinterpret_cast<const uint4*>(wrow + kb * 128 + s * 64 + hh * 32 + e * 16);
-    const float sw = wsc[kb];
+    const float sw = wsc[kb * p.ws_k];
     float v[2][4][8];
     unsigned a = 0;
 #pragma unroll
@@ -495,38 +655,95 @@ __global__ __launch_bounds__(512) void k_linear_f8_small(SmallF8P p) {
   }
 }
 
-template <int DT>
-int launch_small(tfmq_handle h, const SmallF8P& p, int y_dtype, hipStream_t st) {
-  using T = typename Elem<DT>::type;
+int launch_small(tfmq_handle h, const SmallF8P& p, int dtype, int y_dtype, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>((p.N + 31) / 32), static_cast<unsigned>((p.M + 31) / 32));
-  const bool vec = p.K % 8 == 0 && (p.ld * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
-  auto go = [&](auto v, auto y) { hipLaunchKernelGGL((k_linear_f8_small<DT, decltype(v)::value, decltype(y)::value>), grid, dim3(512), 0, st, p); };
-  auto pick = [&](auto y) { vec ? go(std::true_type{}, y) : go(std::false_type{}, y); };
-  if (y_dtype == DT_F32) pick(std::integral_constant<int, DT_F32>{});
-  else if (y_dtype == DT_F16) pick(std::integral_constant<int, DT_F16>{});
-  else pick(std::integral_constant<int, DT_BF16>{});
-  TFMQ_LAUNCH_CHECK(h);
-  return TFMQ_OK;
+  return for_input(p.x, dtype, p.K, p.ld, [&](auto d, auto v) {
+    auto go = [&](auto y) { hipLaunchKernelGGL((k_linear_f8_small<decltype(d)::value, decltype(v)::value, decltype(y)::value>), grid, dim3(512), 0, st, p); };
+    if (y_dtype == DT_F32) go(std::integral_constant<int, DT_F32>{});
+    else if (y_dtype == DT_F16) go(std::integral_constant<int, DT_F16>{});
+    else go(std::integral_constant<int, DT_BF16>{});
+    TFMQ_LAUNCH_CHECK(h);
+    return TFMQ_OK;
+  });
 }
+
+// ---- which kernel multiplies.  Tiles of 256 x 256 where they fill the card in whole rounds (at least three quarters of the last one), else 128 x 128.
+bool big_tiles(tfmq_handle h, long M, int N) {
+  const long nt = static_cast<long>(ceil_div(M, 256)) * ceil_div(N, 256), cu = h->cu_count;
+  return nt >= cu && nt * 4 >= (nt + cu - 1) / cu * cu * 3;
+}
+int launch_product(tfmq_handle h, const GemmF8P& p, int y_dtype, hipStream_t st) {
+  if (y_dtype == DT_F32) return launch_gemm<128, 128, 64, 64, DT_F32, false, 2>(h, p, st);
+  if (big_tiles(h, p.M, p.N))
+    return y_dtype == DT_F16 ? launch_gemm<256, 256, 128, 64, DT_F16, false, 2>(h, p, st) : launch_gemm<256, 256, 128, 64, DT_BF16, false, 2>(h, p, st);
+  return y_dtype == DT_F16 ? launch_gemm<128, 128, 64, 64, DT_F16, false, 2>(h, p, st) : launch_gemm<128, 128, 64, 64, DT_BF16, false, 2>(h, p, st);
+}
+// slices of the token axis of a weight gradient [N][K]: its tiles alone leave CUs idle, every slice costs a write and a read of the result in fp32
+int grad_slices(tfmq_handle h, long M, int N, int K) {
+  const long nt = static_cast<long>(ceil_div(N, 128)) * ceil_div(K, 128), Mb = (M + 127) / 128;
+  const long n = h->cu_count / nt;
+  return static_cast<int>(n < 1 ? 1 : n < Mb ? n : Mb);
+}
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+constexpr long SMALL_M = 32;          // rows up to which one launch that quantises on the way in beats two
+
+// the buffers of a call inside its workspace; sizes in bytes
+struct Carve {
+  char* p;
+  size_t at = 0;
+  template <typename T>
+  T* take(size_t n) {
+    T* r = reinterpret_cast<T*>(p + at);
+    at += up256(n * sizeof(T));
+    return r;
+  }
+};
+struct LinWs {
+  uint8_t* q;
+  float* s;
+  LinWs(Carve& c, long M, int K) {
+    const long Kb = (K + 127) / 128;
+    q = c.take<uint8_t>(static_cast<size_t>(M) * Kb * 128);
+    s = c.take<float>(static_cast<size_t>(M) * Kb);
+  }
+};
+struct BwdWs {
+  uint8_t *gq = nullptr, *gc, *xc;
+  float *gs = nullptr, *gcs, *xcs, *part = nullptr;
+  int slices;
+  BwdWs(Carve& c, tfmq_handle h, long M, int N, int K, bool gx, bool gw) {
+    const long Mb = (M + 127) / 128, Nb = (N + 127) / 128;
+    if (gx && (gw || M > SMALL_M)) {
+      gq = c.take<uint8_t>(static_cast<size_t>(M) * Nb * 128);
+      gs = c.take<float>(static_cast<size_t>(M) * Nb);
+    }
+    if (!gw) return;
+    gc = c.take<uint8_t>(static_cast<size_t>(N) * Mb * 128);
+    gcs = c.take<float>(static_cast<size_t>(N) * Mb);
+    xc = c.take<uint8_t>(static_cast<size_t>(K) * Mb * 128);
+    xcs = c.take<float>(static_cast<size_t>(K) * Mb);
+    slices = grad_slices(h, M, N, K);
+    if (slices > 1) part = c.take<float>(static_cast<size_t>(slices) * N * K);
+  }
+};
+bool shape_ok(long M, int N, int K) { return M > 0 && N > 0 && K > 0 && K <= (1 << 22) && N <= (1 << 22) && M <= (1L << 30); }
+bool type_ok(int t) { return t >= 0 && t <= 2; }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
 extern "C" int tfmq_quantize_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, int by_column, uint8_t* q, float* s, void* stream) {
   DeviceGuard guard(h);
   TFMQ_CHECK_ARG(h, h && x && q && s, "quantize_fp8: null pointer");
-  TFMQ_CHECK_ARG(h, M > 0 && K > 0 && ld >= K && dtype >= 0 && dtype <= 2, "quantize_fp8: bad shape or type");
-  hipStream_t st = as_stream(stream);
-  if (by_column) {
-    if (dtype == DT_F32) return launch_quant_cols<DT_F32>(h, x, M, K, ld, q, s, st);
-    return dtype == DT_F16 ? launch_quant_cols<DT_F16>(h, x, M, K, ld, q, s, st) : launch_quant_cols<DT_BF16>(h, x, M, K, ld, q, s, st);
-  }
-  if (dtype == DT_F32) return launch_quant_rows<DT_F32>(h, x, M, K, ld, q, s, st);
-  return dtype == DT_F16 ? launch_quant_rows<DT_F16>(h, x, M, K, ld, q, s, st) : launch_quant_rows<DT_BF16>(h, x, M, K, ld, q, s, st);
+  TFMQ_CHECK_ARG(h, shape_ok(M, 1, K) && ld >= K && type_ok(dtype), "quantize_fp8: bad shape or type");
+  TFMQ_CHECK_ARG(h, aligned16(q), "quantize_fp8: q must be 16-byte aligned");
+  if (!by_column) return launch_quant_rows(h, x, dtype, M, K, ld, q, s, as_stream(stream));
+  return launch_quant_cols(h, quant_tiles(x, dtype, M, K, ld, nullptr, nullptr, q, s), nullptr, as_stream(stream));
 }
 
 extern "C" int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint8_t* q, uint8_t* qt, float* s, void* stream) {
   DeviceGuard guard(h);
-  TFMQ_CHECK_ARG(h, h && w && q && qt && s && N > 0 && K > 0, "pack_w_fp8: bad argument");
+  TFMQ_CHECK_ARG(h, h && w && q && qt && s && shape_ok(1, N, K), "pack_w_fp8: bad argument");
   const long nb = static_cast<long>((N + 127) / 128) * ((K + 127) / 128);
   TFMQ_CHECK_ARG(h, nb < (1L << 31), "pack_w_fp8: too many blocks");
   hipLaunchKernelGGL(k_pack_w_f8, dim3(static_cast<unsigned>(nb)), dim3(256), 0, as_stream(stream), w, N, K, q, qt, s);
@@ -534,30 +751,72 @@ extern "C" int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint
   return TFMQ_OK;
 }
 
-extern "C" int tfmq_gemm_fp8(tfmq_handle h, const uint8_t* a, const float* sa, const uint8_t* b, const float* sb, long sbn, long sbk, int sb_row,
-                             const float* bias, void* y, int y_dtype, long M, int N, int Kb, void* stream) {
-  DeviceGuard guard(h);
-  TFMQ_CHECK_ARG(h, h && a && sa && b && sb && y, "gemm_fp8: null pointer");
-  TFMQ_CHECK_ARG(h, M > 0 && N > 0 && Kb > 0 && y_dtype >= 0 && y_dtype <= 2, "gemm_fp8: bad shape or type");
-  TFMQ_CHECK_ARG(h, !sb_row || y_dtype == DT_F32, "gemm_fp8: a scale per column comes with an fp32 output");
-  TFMQ_CHECK_ARG(h, reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(b) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0,
-                 "gemm_fp8: operands and output must be 16-byte aligned");
-  GemmF8P p{a, b, sa, sb, sbn, sbk, bias, y, M, N, Kb, 0, 0};
-  hipStream_t st = as_stream(stream);
-  if (sb_row) return launch_gemm<128, 128, 64, 64, DT_F32, true>(h, p, st);
-  if (y_dtype == DT_F32) return launch_gemm<128, 128, 64, 64, DT_F32, false>(h, p, st);
-  if (y_dtype == DT_F16) return launch_gemm<128, 128, 64, 64, DT_F16, false>(h, p, st);
-  return launch_gemm<128, 128, 64, 64, DT_BF16, false>(h, p, st);
+extern "C" size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K) {
+  if (!h || !shape_ok(M, N, K) || M <= SMALL_M) return 0;
+  Carve c{nullptr};
+  LinWs w(c, M, K);
+  return c.at;
 }
 
-extern "C" int tfmq_linear_fp8_small(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* w, const float* ws, const float* bias,
-                                     void* y, int y_dtype, int N, void* stream) {
+extern "C" int tfmq_linear_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* xq, const float* xs, const uint8_t* w,
+                               const float* ws, long ws_n, long ws_k, const float* bias, void* y, int y_dtype, int N, void* work, void* stream) {
   DeviceGuard guard(h);
-  TFMQ_CHECK_ARG(h, h && x && w && ws && y, "linear_fp8_small: null pointer");
-  TFMQ_CHECK_ARG(h, M > 0 && M <= 1024 && N > 0 && K > 0 && ld >= K && dtype >= 0 && dtype <= 2 && y_dtype >= 0 && y_dtype <= 2,
-                 "linear_fp8_small: bad shape (at most 1024 rows) or type");
-  TFMQ_CHECK_ARG(h, reinterpret_cast<uintptr_t>(w) % 16 == 0, "linear_fp8_small: weights must be 16-byte aligned");
-  const SmallF8P p{x, ld, static_cast<int>(M), K, w, ws, bias, y, N, (K + 127) / 128};
-  if (dtype == DT_F32) return launch_small<DT_F32>(h, p, y_dtype, as_stream(stream));
-  return dtype == DT_F16 ? launch_small<DT_F16>(h, p, y_dtype, as_stream(stream)) : launch_small<DT_BF16>(h, p, y_dtype, as_stream(stream));
+  TFMQ_CHECK_ARG(h, h && (x || (xq && xs)) && w && ws && y, "linear_fp8: null pointer");
+  TFMQ_CHECK_ARG(h, shape_ok(M, N, K) && type_ok(y_dtype) && (!x || (ld >= K && type_ok(dtype))), "linear_fp8: bad shape or type");
+  TFMQ_CHECK_ARG(h, aligned16(w) && aligned16(xq) && aligned16(y) && aligned16(work), "linear_fp8: operands, output and workspace must be 16-byte aligned");
+  hipStream_t st = as_stream(stream);
+  const int Kb = (K + 127) / 128;
+  if (x && M <= SMALL_M) return launch_small(h, SmallF8P{x, ld, static_cast<int>(M), K, w, ws, ws_n, ws_k, bias, y, N, Kb}, dtype, y_dtype, st);
+  if (x) {
+    TFMQ_CHECK_ARG(h, work, "linear_fp8: more than 32 rows need a workspace");
+    Carve c{static_cast<char*>(work)};
+    const LinWs b(c, M, K);
+    const int rc = launch_quant_rows(h, x, dtype, M, K, ld, b.q, b.s, st);
+    if (rc != TFMQ_OK) return rc;
+    xq = b.q;
+    xs = b.s;
+  }
+  return launch_product(h, GemmF8P{xq, w, xs, ws, ws_n, ws_k, bias, y, M, N, Kb, 0, 0, 1}, y_dtype, st);
+}
+
+extern "C" size_t tfmq_linear_fp8_bwd_ws_bytes(tfmq_handle h, long M, int N, int K, int want_gx, int want_gw) {
+  if (!h || !shape_ok(M, N, K)) return 0;
+  Carve c{nullptr};
+  BwdWs w(c, h, M, N, K, want_gx != 0, want_gw != 0);
+  return c.at;
+}
+
+extern "C" int tfmq_linear_fp8_bwd(tfmq_handle h, const void* x, int x_dtype, long x_ld, const void* gy, int gy_dtype, long gy_ld, long M, int N, int K,
+                                   const uint8_t* wt, const float* ws, void* gx, float* gw, void* work, void* stream) {
+  DeviceGuard guard(h);
+  TFMQ_CHECK_ARG(h, h && gy && (gx || gw) && (!gx || (wt && ws)) && (!gw || x), "linear_fp8_bwd: null pointer");
+  TFMQ_CHECK_ARG(h, shape_ok(M, N, K) && gy_ld >= N && type_ok(gy_dtype) && (!gw || (x_ld >= K && type_ok(x_dtype))), "linear_fp8_bwd: bad shape or type");
+  TFMQ_CHECK_ARG(h, aligned16(wt) && aligned16(gx) && aligned16(gw) && aligned16(work), "linear_fp8_bwd: operands, outputs and workspace must be 16-byte aligned");
+  hipStream_t st = as_stream(stream);
+  const int Nb = (N + 127) / 128, Kb = (K + 127) / 128;
+  Carve c{static_cast<char*>(work)};
+  const BwdWs b(c, h, M, N, K, gx != nullptr, gw != nullptr);
+  TFMQ_CHECK_ARG(h, c.at == 0 || work, "linear_fp8_bwd: null workspace");
+  int rc = TFMQ_OK;
+  if (gw) {
+    const QuantTileP qx = quant_tiles(x, x_dtype, M, K, x_ld, nullptr, nullptr, b.xc, b.xcs);
+    rc = launch_quant_cols(h, quant_tiles(gy, gy_dtype, M, N, gy_ld, b.gq, b.gs, b.gc, b.gcs), &qx, st);
+  } else if (b.gq) {
+    rc = launch_quant_rows(h, gy, gy_dtype, M, N, gy_ld, b.gq, b.gs, st);
+  }
+  if (rc != TFMQ_OK) return rc;
+  if (gx) {          // the weight's blocks seen from its columns: scale (n block, k block) at ws[n block][k block]
+    rc = b.gq ? launch_product(h, GemmF8P{b.gq, wt, b.gs, ws, 1, Kb, nullptr, gx, M, K, Nb, 0, 0, 1}, gy_dtype, st)
+              : launch_small(h, SmallF8P{gy, gy_ld, static_cast<int>(M), N, wt, ws, 1, Kb, nullptr, gx, K, Nb}, gy_dtype, gy_dtype, st);
+    if (rc != TFMQ_OK) return rc;
+  }
+  if (gw) {
+    const int Mb = static_cast<int>((M + 127) / 128);
+    rc = launch_gemm<128, 128, 64, 64, DT_F32, true, 2>(h, GemmF8P{b.gc, b.xc, b.gcs, b.xcs, 0, 0, nullptr, b.part ? b.part : gw, N, K, Mb, 0, 0, b.slices}, st);
+    if (rc != TFMQ_OK || !b.part) return rc;
+    const long n = static_cast<long>(N) * K;
+    hipLaunchKernelGGL(k_sum_slices, dim3(static_cast<unsigned>((n + 1023) / 1024)), dim3(256), 0, st, b.part, gw, n, b.slices);
+    TFMQ_LAUNCH_CHECK(h);
+  }
+  return rc;
 }

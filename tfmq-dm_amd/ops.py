@@ -1793,11 +1793,10 @@ class QuantFp8:
 class PackedFp8:
     """A Linear's weight [N, K] in e4m3 with one fp32 scale per 128 x 128 block, laid out once (pack_w_fp8 / load_w_fp8).  q: uint8
     [N, 128 * ceil(K / 128)]; qt: its transpose [K, 128 * ceil(N / 128)], which the gradient with respect to x reads; scale [ceil(N / 128),
-    ceil(K / 128)] and its transpose; bias fp32 [N] or None."""
+    ceil(K / 128)]; bias fp32 [N] or None."""
 
     def __init__(self, q, qt, scale, bias, N, K):
         self.q, self.qt, self.scale, self.bias, self.N, self.K = q, qt, scale, bias, N, K
-        self.scale_t = scale.t().contiguous()
 
 
 def quantize_fp8(x: torch.Tensor) -> QuantFp8:
@@ -1870,63 +1869,56 @@ def load_w_fp8(q: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor
     return PackedFp8(q8, qt, scale.detach().clone(), _bias_f32(bias, N, d, "load_w_fp8"), N, K)
 
 
-# rows up to which one launch that quantises on the way in beats quantise + tiled product
-_FP8_SMALL_M = 32
-
-
-def _fp8_product(x, w, ws, bias, N: int, K: int, out_dtype, name: str) -> torch.Tensor:
-    """x (tensor or QuantFp8) [..., K] times the packed rows w [N, Kp] with block scales ws [ceil(N / 128), Kb]."""
+def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = x W^T + bias on e4m3 operands, one scale per 128 channels of a row of x and per 128 x 128 of W, fp32 sums, rounded once to out_dtype
+    (default: x's).  x: [..., K] fp32 / fp16 / bf16 (quantised here as quantize_fp8 does) or a QuantFp8."""
     quantised = isinstance(x, QuantFp8)
     src = x.q if quantised else x
     d = _dev(src)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _DT_CODE:
-        raise TfmqError(f"{name}: output type must be fp32, fp16 or bf16, got {out_dtype}")
-    if x.shape[-1] != K:
-        raise TfmqError(f"{name}: x has {x.shape[-1]} channels, the weight {K}")
-    _same_device(d, weight=w)
-    if not quantised:
-        dt = _dt_code(x, name)
-        M, _, ld = _rows2d(x, name)
+        raise TfmqError(f"linear_fp8: output type must be fp32, fp16 or bf16, got {out_dtype}")
+    if x.shape[-1] != pw.K:
+        raise TfmqError(f"linear_fp8: x has {x.shape[-1]} channels, the weight {pw.K}")
+    _same_device(d, weight=pw.q)
+    if quantised:
+        M, dt, ld = src.shape[0], 0, 0
     else:
-        M = src.shape[0]
-    y = _alloc(tuple(x.shape[:-1]) + (N,), dtype=out_dtype, device=src.device)
+        dt = _dt_code(x, "linear_fp8")
+        M, _, ld = _rows2d(x, "linear_fp8")
+    y = _alloc(tuple(x.shape[:-1]) + (pw.N,), dtype=out_dtype, device=src.device)
     if M == 0:
         return y
     h = handle(d)
-    if not quantised and M <= _FP8_SMALL_M:
-        h.call("linear_fp8_small", _p(x), dt, M, K, ld, _p(w), _p(ws), _p(bias), _p(y), _DT_CODE[out_dtype], N, _stream(d))
-        return y
-    xq = x if quantised else quantize_fp8(x)
-    h.call("gemm_fp8", _p(xq.q), _p(xq.scale), _p(w), _p(ws), ws.shape[1], 1, 0, _p(bias), _p(y), _DT_CODE[out_dtype], M, N, ws.shape[1], _stream(d))
+    nb = 0 if quantised else h.lib.tfmq_linear_fp8_ws_bytes(h.h, M, pw.N, pw.K)
+    ws = _alloc(nb, dtype=torch.uint8, device=src.device) if nb else None
+    h.call("linear_fp8", None if quantised else _p(x), dt, M, pw.K, ld, _p(x.q) if quantised else None, _p(x.scale) if quantised else None, _p(pw.q),
+           _p(pw.scale), pw.scale.shape[1], 1, _p(pw.bias), _p(y), _DT_CODE[out_dtype], pw.N, _p(ws), _stream(d))
     return y
-
-
-def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """y = x W^T + bias on e4m3 operands, one scale per 128 channels of a row of x and per 128 x 128 of W, fp32 sums, rounded once to out_dtype
-    (default: x's).  x: [..., K] fp32 / fp16 / bf16 (quantised here as quantize_fp8 does) or a QuantFp8."""
-    return _fp8_product(x, pw.q, pw.scale, pw.bias, pw.N, pw.K, out_dtype, "linear_fp8")
 
 
 def linear_fp8_bwd(x: torch.Tensor, gy: torch.Tensor, pw: PackedFp8, want_gx: bool = True, want_gw: bool = True):
     """Gradients of linear_fp8 with the same operand form: gx = gy W (gy quantised per row and 128 outputs, the weight's own bytes) in gy's type,
     gw = gy^T x (both quantised down their columns, one scale per 128 tokens) in fp32.  -> (gx [..., K] | None, gw [N, K] | None).  The rounding
-    of the forward's operands is passed straight through; the bias gradient is gy summed over its rows."""
+    of the forward's operands is passed straight through; the bias gradient is gy summed over its rows.  The same bits on every call."""
     d = _dev(gy)
     _same_device(d, x=x, weight=pw.q)
     if x.shape[-1] != pw.K or gy.shape[-1] != pw.N or x.shape[:-1] != gy.shape[:-1]:
         raise TfmqError(f"linear_fp8_bwd: x {tuple(x.shape)} and gy {tuple(gy.shape)} do not fit a weight [{pw.N}, {pw.K}]")
-    _dt_code(x, "linear_fp8_bwd"), _dt_code(gy, "linear_fp8_bwd")
-    gx = _fp8_product(gy, pw.qt, pw.scale_t, None, pw.K, pw.N, None, "linear_fp8_bwd") if want_gx else None
-    gw = None
-    if want_gw:
-        gw = _alloc(pw.N, pw.K, dtype=torch.float32, device=gy.device)
-        if gy.numel() == 0:
+    dx, dg = _dt_code(x, "linear_fp8_bwd"), _dt_code(gy, "linear_fp8_bwd")
+    M, _, ldx = _rows2d(x, "linear_fp8_bwd")
+    _, _, ldg = _rows2d(gy, "linear_fp8_bwd")
+    gx = _alloc(tuple(x.shape), dtype=gy.dtype, device=gy.device) if want_gx else None
+    gw = _alloc(pw.N, pw.K, dtype=torch.float32, device=gy.device) if want_gw else None
+    if M == 0:
+        if want_gw:
             gw.zero_()
-            return gx, gw
-        gq, gs = _quant_cols_fp8(gy, "linear_fp8_bwd")
-        xq, xs = _quant_cols_fp8(x, "linear_fp8_bwd")
-        handle(d).call("gemm_fp8", _p(gq), _p(gs), _p(xq), _p(xs), 0, 0, 1, None, _p(gw), 0, pw.N, pw.K, gs.shape[0], _stream(d))
+        return gx, gw
+    if want_gx or want_gw:
+        h = handle(d)
+        nb = h.lib.tfmq_linear_fp8_bwd_ws_bytes(h.h, M, pw.N, pw.K, int(want_gx), int(want_gw))
+        ws = _alloc(nb, dtype=torch.uint8, device=gy.device) if nb else None
+        h.call("linear_fp8_bwd", _p(x), dx, ldx, _p(gy), dg, ldg, M, pw.N, pw.K, _p(pw.qt), _p(pw.scale), _p(gx), _p(gw), _p(ws), _stream(d))
     return gx, gw
 
 
