@@ -47,6 +47,7 @@ struct XattnP {
   long R;                            // rep * Tq
   float scale;
   int nrb, nsplit;                   // row (or key) blocks, slices of the other axis
+  int rows_per;                      // short states: rows a workgroup walks
 };
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int T) { return lens ? min(max(lens[b], 0), T) : T; }
@@ -64,10 +65,40 @@ __device__ __forceinline__ void drop_keys(v16f (&s)[2], unsigned long long keep,
   }
 }
 
-// ---- a tile of NROW rows x D channels: global -> registers -> LDS (rows of STRIDE bytes).  Rows outside `ok` and channels from d on are zeros, so
-// what a masked place holds (NaN included) never reaches a product.
+// ---- a tile of NROW consecutive keys x D channels: global -> registers -> LDS (rows of STRIDE bytes).  The loads are unconditional (a scalar base,
+// one 32-bit offset per piece for the whole walk; past the last stored key the last one is read again) and asynchronous; keys that are not kept,
+// and channels from d on, become zeros on the way into LDS, so what a dropped place holds (NaN included) never reaches a product.
 template <typename T, int D, int NROW, int STRIDE, int NT = 256>
-struct Tile {
+struct KeyTile {
+  static constexpr int DP = D / 8, N = NROW * DP, PT = (N + NT - 1) / NT;
+  uint4 reg[PT];
+  __device__ __forceinline__ static int row_of(int it) { return min((static_cast<int>(threadIdx.x) + it * NT) / DP, NROW - 1); }
+  __device__ __forceinline__ static int piece_of(int it) { return (static_cast<int>(threadIdx.x) + it * NT) % DP; }
+  // keys [k0, k0 + NROW) of a tensor with Tk stored keys, token stride ts (elements, NROW * ts * 2 < 2^31)
+  __device__ __forceinline__ void load(const T* base, long ts, int k0, int Tk, int d) {
+    const char* p = reinterpret_cast<const char*>(base + k0 * ts);
+    const int last = Tk - 1 - k0;
+#pragma unroll
+    for (int it = 0; it < PT; ++it) {
+      const unsigned off = static_cast<unsigned>(min(row_of(it), last)) * static_cast<unsigned>(ts * 2) + static_cast<unsigned>(min(piece_of(it) * 8, d - 8) * 2);
+      reg[it] = *reinterpret_cast<const uint4*>(p + off);
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* lds, unsigned long long keep, unsigned long long all, int d) {
+    if (keep != all || d != D) {
+#pragma unroll
+      for (int it = 0; it < PT; ++it)
+        if (!((keep >> row_of(it)) & 1) || piece_of(it) * 8 >= d) reg[it] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int it = 0; it < PT; ++it)
+      if (N % NT == 0 || static_cast<int>(threadIdx.x) + it * NT < N) *reinterpret_cast<uint4*>(lds + row_of(it) * STRIDE + piece_of(it) * 16) = reg[it];
+  }
+};
+
+// ---- a tile of NROW rows of the row space, gathered: rows outside are zeros
+template <typename T, int D, int NROW, int STRIDE, int NT = 256>
+struct RowTile {
   static constexpr int DP = D / 8, N = NROW * DP, PT = (N + NT - 1) / NT;
   uint4 reg[PT];
   template <typename RowOff>          // RowOff(row) -> element offset of a row, < 0: zeros

@@ -86,13 +86,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
   const uint8_t* mb = p.mask ? p.mask + b * p.mask_bs : nullptr;
   auto keep_bit = [&](int t) { const int key = t * 64 + lane; return key < klen && (!mb || mb[key] != 0); };
   const int nt = (klen + 63) / 64;
-  Tile<T, D, 64, KS> tk;
-  Tile<T, D, 64, VS> tv;
+  KeyTile<T, D, 64, KS> tk;
+  KeyTile<T, D, 64, VS> tv;
   unsigned long long cur = 0, nxt = 0;
-  auto fetch = [&](int t, unsigned long long m) {
-    auto live = [&](int r) { return (m >> r) & 1; };
-    tk.load(kb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.k.ts : -1L; });
-    tv.load(vb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.v.ts : -1L; });
+  auto fetch = [&](int t) {
+    tk.load(kb, p.k.ts, t * 64, p.Tk, p.d);
+    tv.load(vb, p.v.ts, t * 64, p.Tk, p.d);
   };
   const float c2 = p.scale * LOG2E;
   v16f acc[NRT];
@@ -100,17 +99,17 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
   for (int t = 0; t < NRT; ++t) acc[t] = zero16();
   if (nt > 0) {
     cur = __ballot(keep_bit(0));
-    fetch(0, cur);
+    fetch(0);
   }
   for (int t = 0; t < nt; ++t) {
     __syncthreads();
-    tk.store(sK);
-    tv.store(sV);
+    tk.store(sK, cur, ~0ull, p.d);
+    tv.store(sV, cur, ~0ull, p.d);
     __syncthreads();
     nxt = 0;
     if (t + 1 < nt) {
       nxt = __ballot(keep_bit(t + 1));
-      fetch(t + 1, nxt);
+      fetch(t + 1);
     }
     if (cur != 0) {
       v16f s[2];
@@ -202,7 +201,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
     ff = __builtin_amdgcn_exp2f(static_cast<float>(fe) - PSHIFT);
     unf = __builtin_amdgcn_exp2f(static_cast<float>(-fe));
   }
-  Tile<T, D, NR, S> tq, tg;
+  RowTile<T, D, NR, S> tq, tg;
   float rl = INFINITY, rd = 0.0f;
   auto fetch = [&](int t) {
     const long r0 = static_cast<long>(t) * NR;
@@ -365,6 +364,7 @@ extern "C" int tfmq_xattn_bwd(tfmq_handle h, const tfmq_xattn_desc* a, void* str
   TFMQ_CHECK_ARG(h, a->dtype == 1 || a->dtype == 2, "xattn_bwd: fp16 or bf16");
   TFMQ_CHECK_ARG(h, a->q && a->k && a->v && a->o && a->go && a->lse && a->dq && a->dk && a->dv && a->ws, "xattn_bwd: null tensor");
   TFMQ_CHECK_ARG(h, a->nsplit >= 1, "xattn_bwd: bad slice count");
+  TFMQ_CHECK_ARG(h, a->k_ts < (1 << 23) && a->v_ts < (1 << 23) && a->k_ts >= 0 && a->v_ts >= 0, "xattn_bwd: token strides of k and v must lie in [0, 2^23)");
   XattnP p{};
   p.q = {a->q, a->q_bs, a->q_ts};
   p.k = {a->k, a->k_bs, a->k_ts};

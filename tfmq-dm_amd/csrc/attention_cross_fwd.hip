@@ -7,6 +7,7 @@
 // while the previous tile is multiplied, and stored to LDS row-major; V is read transposed by ds_read_b64_tr_b16.  Scores, statistics and sums are fp32;
 // the probabilities are rounded to the operand type for the second product (they are <= 1, the sum takes them unrounded).
 #include "attention_cross.hpp"
+#include <algorithm>
 
 using namespace xattn;
 
@@ -47,13 +48,12 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
 
   const int nt = (klen + 63) / 64, per = (nt + p.nsplit - 1) / p.nsplit;
   const int t0 = sp * per, t1 = min(nt, t0 + per);
-  Tile<T, D, 64, KS> tk;
-  Tile<T, D, 64, VS> tv;
+  KeyTile<T, D, 64, KS> tk;
+  KeyTile<T, D, 64, VS> tv;
   unsigned long long cur = 0, nxt = 0;
-  auto fetch = [&](int t, unsigned long long m) {
-    auto live = [&](int r) { return (m >> r) & 1; };
-    tk.load(kb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.k.ts : -1L; });
-    tv.load(vb, p.d, [&](int r) { return live(r) ? (static_cast<long>(t) * 64 + r) * p.v.ts : -1L; });
+  auto fetch = [&](int t) {
+    tk.load(kb, p.k.ts, t * 64, p.Tk, p.d);
+    tv.load(vb, p.v.ts, t * 64, p.Tk, p.d);
   };
   const float c2 = p.scale * LOG2E;
   float m = -INFINITY, l = 0.0f;
@@ -63,17 +63,17 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
 
   if (t0 < t1) {
     cur = __ballot(keep_bit(t0));
-    fetch(t0, cur);
+    fetch(t0);
   }
   for (int t = t0; t < t1; ++t) {
     __syncthreads();                   // every wave is through with the previous tile
-    tk.store(sK);
-    tv.store(sV);
+    tk.store(sK, cur, ~0ull, p.d);
+    tv.store(sV, cur, ~0ull, p.d);
     __syncthreads();
     nxt = 0;
     if (t + 1 < t1) {
       nxt = __ballot(keep_bit(t + 1));
-      fetch(t + 1, nxt);
+      fetch(t + 1);
     }
     if (cur != 0) {
       v16f s[2];
@@ -83,35 +83,34 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) s[kt] = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s[kt]);
       }
+      if (cur != ~0ull) drop_keys(s, cur, hh);
       float mx = -INFINITY;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kt][r] *= c2;
-      if (cur != ~0ull) drop_keys(s, cur, hh);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.0f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m - mu);
-      m = mn;
-      float rs = 0.0f;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[kt][r] = __builtin_amdgcn_exp2f(s[kt][r] - mu);
-          rs += s[kt][r];
-        }
-      l = __builtin_fmaf(l, alpha, rs);
-      if (__any(alpha != 1.0f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;          // (scale > 0)
+      // the sums move to a new maximum only where one has risen by more than 2^8 since (or there was none): probabilities up to 256 are as exact as
+      // those up to 1, and past the first tile this is rare
+      if (__any(mx > m + 8.0f)) {
+        const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+        m = mn;
+        l *= alpha;
 #pragma unroll
         for (int t2 = 0; t2 < NRT; ++t2)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[t2][r] *= alpha;
       }
+      const float mu = m == -INFINITY ? 0.0f : m;
+      float rs[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], c2, -mu));
+          rs[r & 1] += s[kt][r];
+        }
+      l += rs[0] + rs[1];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const V8 pf = frag_regs<T>(s[u >> 1], u & 1);
@@ -150,6 +149,124 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
   if (p.lse && hh == 0) p.lse[orow] = ok && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
+// ---- up to 128 states (a text encoder's): K and V of one (item, key head) stay in LDS, the waves walk over rows on their own, without barriers, the next
+// rows' queries under way.  All keys are in the accumulators at once: one maximum, no running rescale.
+// registers of the scores, the sums and two sets of queries; past 160 the kernel would spill at two waves per SIMD
+constexpr int short_regs(int D, int NKT) { return NKT * 16 + nrt(D) * 16 + nks(D) * 8; }
+constexpr bool short_fits(int D, int NKT) { return NKT <= 2 || short_regs(D, NKT) <= 160; }
+
+template <typename T, int D, int NKT>
+__global__ __launch_bounds__(256, short_regs(D, NKT) > 104 ? 2 : 3) void k_xattn_short(XattnP p) {
+  constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_rows(D), VS = stride_cols(D), NK = NKT * 32;
+  using V8 = typename Vec8<T>::type;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* sK = smem;
+  unsigned char* sV = smem + NK * KS;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
+  const int id = xcd_tile_id();
+  const int rb = id % p.nrb, bg = id / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
+  const uint8_t* mb = p.mask ? p.mask + b * p.mask_bs : nullptr;
+  const T* qb = static_cast<const T*>(p.q.p) + b * p.q.bs + static_cast<long>(g) * p.rep * p.d;
+
+  const long r_end = min(p.R, (static_cast<long>(rb) + 1) * p.rows_per);
+  long row = static_cast<long>(rb) * p.rows_per + wid * 32 + j;
+  V8 qf[NKS];
+  bool ok = false;
+  int hi = 0, i = 0;
+  auto load_q = [&](long r) {
+    hi = static_cast<int>(r / p.Tq);
+    i = static_cast<int>(r - static_cast<long>(hi) * p.Tq);
+    ok = r < r_end && i < qlen;
+    const T* qrow = qb + i * p.q.ts + static_cast<long>(hi) * p.d;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = ks * 16 + hh * 8;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (ok && c < p.d) w = *reinterpret_cast<const uint4*>(qrow + c);
+      qf[ks] = __builtin_bit_cast(V8, w);
+    }
+  };
+  load_q(row);
+  unsigned long long keep[2] = {0, 0};
+  {
+#pragma unroll
+    for (int w = 0; w < (NKT + 1) / 2; ++w) {
+      const int key = w * 64 + lane;
+      keep[w] = __ballot(key < klen && (!mb || mb[min(key, p.Tk - 1)] != 0));
+    }
+#pragma unroll
+    for (int t = 0; t < NKT; ++t) {          // 32 keys at a time
+      KeyTile<T, D, 32, KS> tk;
+      KeyTile<T, D, 32, VS> tv;
+      const int k0 = min(t * 32, p.Tk - 1);
+      tk.load(kb, p.k.ts, k0, p.Tk, p.d);
+      tv.load(vb, p.v.ts, k0, p.Tk, p.d);
+      const unsigned long long kk = (keep[t >> 1] >> (32 * (t & 1))) & 0xffffffffull;
+      tk.store(sK + t * 32 * KS, kk, 0xffffffffull, p.d);
+      tv.store(sV + t * 32 * VS, kk, 0xffffffffull, p.d);
+    }
+  }
+  __syncthreads();
+  const bool every = keep[0] == (NKT == 1 ? 0xffffffffull : ~0ull) && (NKT <= 2 || keep[1] == (NKT == 3 ? 0xffffffffull : ~0ull));
+  const float c2 = p.scale * LOG2E;
+  while (row - j < r_end) {
+    const long orow = (static_cast<long>(b) * p.H + g * p.rep + hi) * p.Tq + i;
+    T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(g * p.rep + hi) * p.d;
+    const bool in = row < r_end, cur = ok;
+    v16f s[NKT];
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt) {
+      s[kt] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) s[kt] = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s[kt]);
+    }
+    row += 128;
+    if (row - j < r_end) load_q(row);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt) {
+      if (!every) {
+        const unsigned bits = static_cast<unsigned>(keep[kt >> 1] >> (32 * (kt & 1))) >> (4 * hh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kt][r] = ((bits >> crow(r, 0)) & 1) ? s[kt][r] : -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
+    const float mu = mx == -INFINITY ? 0.0f : mx;
+    float rs[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], c2, -mu));
+        rs[r & 1] += s[kt][r];
+      }
+    float l = rs[0] + rs[1];
+    l += __shfl_xor(l, 32, 64);
+    v16f o[NRT];
+#pragma unroll
+    for (int t = 0; t < NRT; ++t) o[t] = zero16();
+#pragma unroll
+    for (int u = 0; u < 2 * NKT; ++u) {
+      const V8 pf = frag_regs<T>(s[u >> 1], u & 1);
+#pragma unroll
+      for (int t = 0; t < NRT; ++t) o[t] = mfma16(frag_cols<T>(sV, VS, u * 16, t, lane), pf, o[t]);
+    }
+    if (in) {
+      zero_unless(cur, o);
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, o[t], inv);
+      if (p.lse && hh == 0) p.lse[orow] = cur && l != 0.0f ? (mx + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    }
+  }
+}
+
 // joins the slices of a row: 16 lanes a row, four (eight) channels a lane and step
 template <typename T>
 __global__ __launch_bounds__(256) void k_xattn_join(XattnP p) {
@@ -186,10 +303,35 @@ __global__ __launch_bounds__(256) void k_xattn_join(XattnP p) {
   if (p.lse && c16 == 0) p.lse[r] = l != 0.0f ? (M + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
+template <typename T, int D, int NKT>
+int launch_short(tfmq_handle h, XattnP p, hipStream_t st) {
+  if constexpr (short_fits(D, NKT)) {
+  auto kern = &k_xattn_short<T, D, NKT>;
+  constexpr int smem = NKT * 32 * (stride_rows(D) + stride_cols(D));
+  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the states are staged once per workgroup: as many rows each as leave two workgroups per CU
+  const long pairs = static_cast<long>(p.B) * p.G, tiles = (p.R + 127) / 128;
+  const long per = std::min<long>(tiles, std::max<long>(1, pairs * tiles / (2L * h->cu_count)));
+  p.rows_per = static_cast<int>(per) * 128;
+  p.nrb = ceil_div(p.R, p.rows_per);
+  TFMQ_CHECK_ARG(h, pairs * p.nrb < (1L << 31), "xattn_fwd: too many workgroups");
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(pairs * p.nrb)), dim3(256), smem, st, p);
+  TFMQ_LAUNCH_CHECK(h);
+  }
+  return TFMQ_OK;
+}
+
 template <typename T>
 int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
   return for_head_dim(p.d, [&](auto dc) {
     constexpr int D = decltype(dc)::value;
+    const int nkt = (p.Tk + 31) / 32;
+    if (p.nsplit == 1 && nkt <= 4 && short_fits(D, nkt)) {
+      if (nkt == 1) return launch_short<T, D, 1>(h, p, st);
+      if (nkt == 2) return launch_short<T, D, 2>(h, p, st);
+      if (nkt == 3) return launch_short<T, D, 3>(h, p, st);
+      return launch_short<T, D, 4>(h, p, st);
+    }
     auto kern = &k_xattn_fwd<T, D>;
     constexpr int smem = 64 * (stride_rows(D) + stride_cols(D));
     TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -214,6 +356,7 @@ extern "C" int tfmq_xattn_splits(tfmq_handle h, int B, int H, int G, int Tq, int
   const long blocks = static_cast<long>(B) * G * ceil_div(static_cast<long>(H / G) * Tq, 128);
   const long want = 3L * h->cu_count;
   if (blocks * 2 > want) return 1;
+  if (Tk <= 128) return 1;
   const long most = (Tk + 127) / 128;
   const long n = want / blocks;
   return static_cast<int>(n < 1 ? 1 : n < most ? n : most);
@@ -227,6 +370,7 @@ extern "C" int tfmq_xattn_fwd(tfmq_handle h, const tfmq_xattn_desc* a, void* str
   TFMQ_CHECK_ARG(h, a->dtype == 1 || a->dtype == 2, "xattn_fwd: fp16 or bf16");
   TFMQ_CHECK_ARG(h, a->q && (a->Tk == 0 || (a->k && a->v)) && a->o, "xattn_fwd: null tensor");
   TFMQ_CHECK_ARG(h, a->nsplit >= 1 && (a->nsplit == 1 || a->ws), "xattn_fwd: slices need a workspace");
+  TFMQ_CHECK_ARG(h, a->k_ts < (1 << 23) && a->v_ts < (1 << 23) && a->k_ts >= 0 && a->v_ts >= 0, "xattn_fwd: token strides of k and v must lie in [0, 2^23)");
   XattnP p{};
   p.q = {a->q, a->q_bs, a->q_ts};
   p.k = {a->k, a->k_bs, a->k_ts};
