@@ -96,28 +96,71 @@ struct KeyTile {
   }
 };
 
-// ---- a tile of NROW rows of the row space, gathered: rows outside are zeros
+// ---- tiles of NROW rows of the row space, walked in order, of two tensors at once (queries and upstream gradients).  A thread keeps where its rows are
+// and steps NROW rows ahead (no division in the loop); rows past the end, or behind q_lens, are read from the item's first row and become zeros.
 template <typename T, int D, int NROW, int STRIDE, int NT = 256>
-struct RowTile {
+struct RowTile2 {
   static constexpr int DP = D / 8, N = NROW * DP, PT = (N + NT - 1) / NT;
-  uint4 reg[PT];
-  template <typename RowOff>          // RowOff(row) -> element offset of a row, < 0: zeros
-  __device__ __forceinline__ void load(const T* base, int d, RowOff off) {
+  uint4 a[PT], b[PT];
+  long oa[PT], ob[PT];          // element offsets of the rows
+  int i[PT];                    // their query index
+  long left;                    // rows from the tile's first on
+  unsigned live;
+  int di;
+  long da, db, wa, wb;          // a step of NROW rows, and of a wrap to the next head
+  __device__ __forceinline__ static int row_of(int it) { return min((static_cast<int>(threadIdx.x) + it * NT) / DP, NROW - 1); }
+  __device__ __forceinline__ static int piece_of(int it) { return (static_cast<int>(threadIdx.x) + it * NT) % DP; }
+  __device__ __forceinline__ void start(long row0, long R, int Tq, int d, long ats, long bts) {
+    const int dh = NROW / Tq;
+    di = NROW - dh * Tq;
+    da = di * ats + static_cast<long>(dh) * d;
+    db = di * bts + static_cast<long>(dh) * d;
+    wa = d - Tq * ats;
+    wb = d - Tq * bts;
+    left = R - row0;
 #pragma unroll
     for (int it = 0; it < PT; ++it) {
-      const int idx = static_cast<int>(threadIdx.x) + it * NT, row = idx / DP, pc = idx - row * DP;
-      const long o = (N % NT == 0 || idx < N) && pc * 8 < d ? off(row) : -1;
-      reg[it] = o >= 0 ? *reinterpret_cast<const uint4*>(base + o + pc * 8) : make_uint4(0, 0, 0, 0);
+      const long row = row0 + row_of(it), h = row / Tq;
+      i[it] = static_cast<int>(row - h * Tq);
+      oa[it] = i[it] * ats + h * d;
+      ob[it] = i[it] * bts + h * d;
     }
   }
-  __device__ __forceinline__ void store(unsigned char* lds) const {
+  // the tile at hand into registers, and a step ahead
+  __device__ __forceinline__ void load(const T* pa, const T* pb, int Tq, int qlen, int d) {
+    live = 0;
 #pragma unroll
     for (int it = 0; it < PT; ++it) {
-      const int idx = static_cast<int>(threadIdx.x) + it * NT, row = idx / DP, pc = idx - row * DP;
-      if (N % NT == 0 || idx < N) *reinterpret_cast<uint4*>(lds + row * STRIDE + pc * 16) = reg[it];
+      const bool ok = row_of(it) < left && i[it] < qlen;
+      const int c = min(piece_of(it) * 8, d - 8);
+      a[it] = *reinterpret_cast<const uint4*>(pa + (ok ? oa[it] : 0) + c);
+      b[it] = *reinterpret_cast<const uint4*>(pb + (ok ? ob[it] : 0) + c);
+      live |= (ok && piece_of(it) * 8 < d ? 1u : 0u) << it;
+      i[it] += di;
+      const bool wrap = i[it] >= Tq;
+      i[it] -= wrap ? Tq : 0;
+      oa[it] += da + (wrap ? wa : 0);
+      ob[it] += db + (wrap ? wb : 0);
     }
+    left -= NROW;
+  }
+  __device__ __forceinline__ void store(unsigned char* la, unsigned char* lb) {
+    if (__any(live != (1u << PT) - 1)) {
+#pragma unroll
+      for (int it = 0; it < PT; ++it)
+        if (!((live >> it) & 1)) a[it] = b[it] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int it = 0; it < PT; ++it)
+      if (N % NT == 0 || static_cast<int>(threadIdx.x) + it * NT < N) {
+        *reinterpret_cast<uint4*>(la + row_of(it) * STRIDE + piece_of(it) * 16) = a[it];
+        *reinterpret_cast<uint4*>(lb + row_of(it) * STRIDE + piece_of(it) * 16) = b[it];
+      }
   }
 };
+
+// keeps the order of what stands before and behind it: operand reads asked for early stay early
+__device__ __forceinline__ void hold_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // rows [row0, row0 + 32) of a tile as an operand, channels [16 ks, +16): lane j = row, half hh = 8 of the 16 channels
 template <typename T>

@@ -24,7 +24,7 @@ __device__ __forceinline__ int inv_exponent(float a) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
+__global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
   constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_both(D), VS = stride_rows(D);
   using V8 = typename Vec8<T>::type;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -112,27 +112,47 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
       fetch(t + 1);
     }
     if (cur != 0) {
-      v16f s[2];
+      // (operand reads run ahead of the products, as in k_xattn_dkv)
+      V8 kr[NKS], vr[NKS];
+      auto read_rows = [&](int kt) {
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+          kr[ks] = frag_rows<T>(sK, KS, kt * 32 + j, ks, hh);
+          vr[ks] = frag_rows<T>(sV, VS, kt * 32 + j, ks, hh);
+        }
+      };
+      read_rows(0);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        s[kt] = zero16();
+        hold_order();
+        v16f s = zero16(), dp = zero16();
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) s[kt] = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s[kt]);
-      }
-      if (cur != ~0ull) drop_keys(s, cur, hh);
+        for (int ks = 0; ks < NKS; ++ks) {
+          s = mfma16(kr[ks], qf[ks], s);
+          dp = mfma16(vr[ks], gf[ks], dp);
+        }
+        V8 ct[2][NRT];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        v16f dp = zero16();
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) dp = mfma16(frag_rows<T>(sV, VS, kt * 32 + j, ks, hh), gf[ks], dp);
+          for (int t2 = 0; t2 < NRT; ++t2) ct[u][t2] = frag_cols<T>(sK, KS, kt * 32 + u * 16, t2, lane);
+        hold_order();
+        const unsigned bits = static_cast<unsigned>(cur >> (32 * kt)) >> (4 * hh);
+        if (cur != ~0ull) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], c2, -sh)) * (dp[r] - dl);
-      }
+          for (int r = 0; r < 16; ++r) s[r] = ((bits >> crow(r, 0)) & 1) ? s[r] : -INFINITY;
+        }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const V8 df = frag_regs<T>(s[u >> 1], u & 1);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -sh)) * (dp[r] - dl);
+        V8 df[2];
 #pragma unroll
-        for (int t2 = 0; t2 < NRT; ++t2) acc[t2] = mfma16(frag_cols<T>(sK, KS, u * 16, t2, lane), df, acc[t2]);
+        for (int u = 0; u < 2; ++u) df[u] = frag_regs<T>(s, u);
+        hold_order();
+        if (kt == 0) read_rows(1);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int t2 = 0; t2 < NRT; ++t2) acc[t2] = mfma16(ct[u][t2], df[u], acc[t2]);
       }
     }
     cur = nxt;
@@ -145,7 +165,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
   for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, acc[t], f);
 }
 
-template <int D> constexpr int dkv_rows() { return D <= 64 ? 64 : 32; }
+template <int D> constexpr int dkv_rows() { return D <= 128 ? 64 : 32; }
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
@@ -201,50 +221,70 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
     ff = __builtin_amdgcn_exp2f(static_cast<float>(fe) - PSHIFT);
     unf = __builtin_amdgcn_exp2f(static_cast<float>(-fe));
   }
-  RowTile<T, D, NR, S> tq, tg;
+  const T* qb = static_cast<const T*>(p.q.p) + b * p.q.bs + static_cast<long>(g) * p.rep * p.d;
+  const T* gb = static_cast<const T*>(p.go.p) + b * p.go.bs + static_cast<long>(g) * p.rep * p.d;
+  RowTile2<T, D, NR, S> tile;
+  tile.start(static_cast<long>(t0) * NR, p.R, p.Tq, p.d, p.q.ts, p.go.ts);
+  long srow = static_cast<long>(t0) * NR + tid;          // threads below NR: the row whose statistics this one brings
+  int si = static_cast<int>(srow % p.Tq);
   float rl = INFINITY, rd = 0.0f;
-  auto fetch = [&](int t) {
-    const long r0 = static_cast<long>(t) * NR;
-    auto at = [&](int r, const View& v) -> long {
-      const long row = r0 + r;
-      if (row >= p.R) return -1;
-      const int hi = static_cast<int>(row / p.Tq), i = static_cast<int>(row - static_cast<long>(hi) * p.Tq);
-      return i < qlen ? i * v.ts + static_cast<long>(hi) * p.d : -1;
-    };
-    const long hc = b * p.q.bs + static_cast<long>(g) * p.rep * p.d, gc = b * p.go.bs + static_cast<long>(g) * p.rep * p.d;
-    tq.load(static_cast<const T*>(p.q.p) + hc, p.d, [&](int r) { return at(r, p.q); });
-    tg.load(static_cast<const T*>(p.go.p) + gc, p.d, [&](int r) { return at(r, p.go); });
+  auto fetch = [&]() {
+    tile.load(qb, gb, p.Tq, qlen, p.d);
     if (tid < NR) {
-      const long row = r0 + tid;
       rl = INFINITY;
       rd = 0.0f;
-      if (row < p.R && static_cast<int>(row % p.Tq) < qlen) {
-        const float v = p.lse_in[brow0 + row];
+      if (srow < p.R && si < qlen) {
+        const float v = p.lse_in[brow0 + srow];
         rl = v == -INFINITY ? INFINITY : v * LOG2E;
-        rd = p.delta[brow0 + row];
+        rd = p.delta[brow0 + srow];
       }
+      srow += NR;
+      si += tile.di;
+      si -= si >= p.Tq ? p.Tq : 0;
     }
   };
   const float c2 = p.scale * LOG2E;
   v16f ak[NRT], av[NRT];
 #pragma unroll
   for (int t = 0; t < NRT; ++t) ak[t] = zero16(), av[t] = zero16();
-  if (t0 < t1) fetch(t0);
+  if (t0 < t1) fetch();
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
-    tq.store(sQ);
-    tg.store(sG);
+    tile.store(sQ, sG);
     if (tid < NR) sL[tid] = rl - PSHIFT, sD[tid] = rd;
     __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
+    if (t + 1 < t1) fetch();
     if (work) {
+      // operand reads run ahead of the products: the rows of the next half, and the transposed tiles while the exponentials are taken
+      V8 qr[NKS], gr[NKS];
+      auto read_rows = [&](int half) {
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+          qr[ks] = frag_rows<T>(sQ, S, half * 32 + j, ks, hh);
+          gr[ks] = frag_rows<T>(sG, S, half * 32 + j, ks, hh);
+        }
+      };
+      read_rows(0);
 #pragma unroll
       for (int half = 0; half < NR / 32; ++half) {
+        hold_order();
         v16f s = zero16(), dp = zero16();
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) s = mfma16(frag_rows<T>(sQ, S, half * 32 + j, ks, hh), kf[ks], s);
+        for (int ks = 0; ks < NKS; ++ks) {
+          s = mfma16(qr[ks], kf[ks], s);
+          dp = mfma16(gr[ks], vf[ks], dp);
+        }
+        V8 gt[2][NRT], qt[2][NRT];
+        auto read_cols = [&](int u) {
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) dp = mfma16(frag_rows<T>(sG, S, half * 32 + j, ks, hh), vf[ks], dp);
+          for (int t2 = 0; t2 < NRT; ++t2) {
+            gt[u][t2] = frag_cols<T>(sG, S, half * 32 + u * 16, t2, lane);
+            qt[u][t2] = frag_cols<T>(sQ, S, half * 32 + u * 16, t2, lane);
+          }
+        };
+        read_cols(0);
+        if (D <= 128) read_cols(1);          // (at 160 the registers hold one of the two)
+        hold_order();
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float4 L = *reinterpret_cast<const float4*>(sL + half * 32 + 8 * a + 4 * hh);
@@ -255,16 +295,24 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
             const int r = 4 * a + c;
             const float pr = keep ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lv[c])) : 0.0f;
             s[r] = pr;
-            dp[r] = pr * (dp[r] - dv[c]) * ff;
+            dp[r] = is_f16<T>() ? pr * (dp[r] - dv[c]) * ff : pr * (dp[r] - dv[c]);
           }
         }
+        V8 pf[2], df[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) pf[u] = frag_regs<T>(s, u), df[u] = frag_regs<T>(dp, u);
+        hold_order();
+        if (half + 1 < NR / 32) read_rows(half + 1);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const V8 pf = frag_regs<T>(s, u), df = frag_regs<T>(dp, u);
+          if (u == 1 && D > 128) {
+            hold_order();
+            read_cols(1);
+          }
 #pragma unroll
           for (int t2 = 0; t2 < NRT; ++t2) {
-            av[t2] = mfma16(frag_cols<T>(sG, S, half * 32 + u * 16, t2, lane), pf, av[t2]);
-            ak[t2] = mfma16(frag_cols<T>(sQ, S, half * 32 + u * 16, t2, lane), df, ak[t2]);
+            av[t2] = mfma16(gt[u][t2], pf[u], av[t2]);
+            ak[t2] = mfma16(qt[u][t2], df[u], ak[t2]);
           }
         }
       }
