@@ -5,6 +5,7 @@
 // so shared key heads cost nothing extra and a one-token call still fills a fragment with its H / G heads.
 #pragma once
 #include "conv_common.hpp"
+#include <algorithm>
 #include <type_traits>
 
 namespace xattn {
@@ -170,12 +171,12 @@ __device__ __forceinline__ typename Vec8<T>::type frag_rows(const unsigned char*
 
 // The tile transposed: channels [32 t, +32) as the operand's rows, tile rows [r0, +16) as its 16 reduction steps, in the order in which a lane
 // of the other operand holds a product's registers (half hh: rows r0 + 4 hh + (0 .. 3), then r0 + 8 + 4 hh + (0 .. 3)).  ds_read_b64_tr_b16 hands lane
-// i of 16 the i-th of 16 channels of four rows; the channel groups are dealt so that operand row 8 a + 4 h + c is channel 32 t + 16 h + 4 a + c:
-// register r of half hh of the result is channel 32 t + 16 hh + r, 16 consecutive ones a lane.
+// i of 16 the i-th of 16 channels of four rows; the channel groups are dealt so that register r of half hh of the result is channel
+// 32 t + 16 (r >> 3) + 8 hh + (r & 7): eight consecutive ones, and the two halves of a wave side by side, so that a store covers 32 bytes of a row.
 template <typename T>
 __device__ __forceinline__ typename Vec8<T>::type frag_cols(const unsigned char* lds, int stride, int r0, int t, int lane) {
   const int L = lane & 15, gg = (lane >> 4) & 1, hh = lane >> 5, cg = L & 3;
-  const unsigned char* p = lds + (r0 + 4 * hh + (L >> 2)) * stride + (t * 32 + 16 * (cg & 1) + 8 * gg + 4 * (cg >> 1)) * 2;
+  const unsigned char* p = lds + (r0 + 4 * hh + (L >> 2)) * stride + (t * 32 + 16 * gg + 8 * (cg & 1) + 4 * (cg >> 1)) * 2;
   using P = __attribute__((address_space(3))) v4s*;
   const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p));
   const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 8 * stride));
@@ -193,6 +194,92 @@ __device__ __forceinline__ typename Vec8<T>::type frag_regs(const v16f& s, int u
   return f;
 }
 
+// ---- buffers whose reads past the end give zeros and whose writes past it are dropped: rows and channels that are not there need no branches, and
+// without branches around them the compiler can count stores and loads apart (a wait for the next rows does not wait for the last stores)
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+using Rsrc = __amdgpu_buffer_rsrc_t;
+constexpr unsigned NOWHERE = 0xfffffff0u;
+__device__ __forceinline__ Rsrc buffer_of(const void* p, long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform_ptr(static_cast<const char*>(p))), 0, __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), 0x00027000);
+}
+template <typename V8>
+__device__ __forceinline__ V8 load8(Rsrc r, unsigned off) {
+  return __builtin_bit_cast(V8, __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(off), 0, 0));
+}
+// a lane's 16 channels (of 32 from c0 on) of the row at byte `row`
+template <typename T>
+__device__ __forceinline__ void store16(Rsrc r, unsigned row, bool ok, int c0, int hh, int d, const v16f& v, float f) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int c = c0 + 16 * g + 8 * hh;
+    typename Vec8<T>::type w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(v[8 * g + e] * f);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, w), r, static_cast<int>(ok && c < d ? row + 2 * c : NOWHERE), 0, 0);
+  }
+}
+
+// a lane's place in the row space of one (item, key head), 128 rows further each step
+struct RowWalk {
+  long row;
+  int hi, i, dh, di, Tq;
+  __device__ __forceinline__ RowWalk(long r, int tq) : row(r), Tq(tq) {
+    hi = static_cast<int>(r / Tq);
+    i = static_cast<int>(r - static_cast<long>(hi) * Tq);
+    dh = 128 / Tq;
+    di = 128 - dh * Tq;
+  }
+  __device__ __forceinline__ void step() {
+    row += 128;
+    hi += dh;
+    i += di;
+    if (i >= Tq) {
+      i -= Tq;
+      ++hi;
+    }
+  }
+};
+
+// all of up to 128 states into LDS: K and V rows (dropped keys and channels from d on: zeros) and 0 / -inf per key; a barrier behind it
+template <typename T, int D, int NKT, int KS, int VS>
+__device__ __forceinline__ void stage_short(const XattnP& p, int b, int g, int klen, unsigned char* sK, unsigned char* sV, float* sB) {
+  const int lane = threadIdx.x & 63;
+  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
+  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
+  const uint8_t* mb = p.mask ? p.mask + b * p.mask_bs : nullptr;
+  unsigned long long keep[2] = {0, 0};
+#pragma unroll
+  for (int w = 0; w < (NKT + 1) / 2; ++w) {
+    const int key = w * 64 + lane;
+    const bool kept = key < klen && (!mb || mb[min(key, p.Tk - 1)] != 0);
+    keep[w] = __ballot(kept);
+    if (threadIdx.x < 64 && key < NKT * 32) sB[key] = kept ? 0.0f : -INFINITY;
+  }
+#pragma unroll
+  for (int t = 0; t < NKT; ++t) {
+    KeyTile<T, D, 32, KS> tk;
+    KeyTile<T, D, 32, VS> tv;
+    const int k0 = min(t * 32, p.Tk - 1);
+    tk.load(kb, p.k.ts, k0, p.Tk, p.d);
+    tv.load(vb, p.v.ts, k0, p.Tk, p.d);
+    const unsigned long long kk = (keep[t >> 1] >> (32 * (t & 1))) & 0xffffffffull;
+    tk.store(sK + t * 32 * KS, kk, 0xffffffffull, p.d);
+    tv.store(sV + t * 32 * VS, kk, 0xffffffffull, p.d);
+  }
+  __syncthreads();
+}
+
+// scores start from 0 for kept keys and from -inf for dropped ones (whose rows of K are zeros): a mask costs no arithmetic
+__device__ __forceinline__ v16f start_scores(const float* bias, int hh) {
+  v16f s;
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const float4 b = *reinterpret_cast<const float4*>(bias + 8 * a + 4 * hh);
+    s[4 * a] = b.x; s[4 * a + 1] = b.y; s[4 * a + 2] = b.z; s[4 * a + 3] = b.w;
+  }
+  return s;
+}
+
 // what a row that is not there (or has no query) leaves: zeros, whatever its lanes computed
 template <int N>
 __device__ __forceinline__ void zero_unless(bool ok, v16f (&a)[N]) {
@@ -202,16 +289,24 @@ __device__ __forceinline__ void zero_unless(bool ok, v16f (&a)[N]) {
   }
 }
 
-// 16 consecutive channels of one row (those below d; d % 8 == 0)
+// a lane's 16 channels (of 32 from c0 on) of one row; those below d, d % 8 == 0
 template <typename T>
-__device__ __forceinline__ void store16(T* row, int c0, int d, const v16f& v, float f) {
+__device__ __forceinline__ void store16(T* row, int c0, int hh, int d, const v16f& v, float f) {
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    if (c0 + 8 * g >= d) continue;
+    const int c = c0 + 16 * g + 8 * hh;
+    if (c >= d) continue;
     typename Vec8<T>::type w;
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(v[8 * g + e] * f);
-    *reinterpret_cast<typename Vec8<T>::type*>(row + c0 + 8 * g) = w;
+    *reinterpret_cast<typename Vec8<T>::type*>(row + c) = w;
+  }
+}
+__device__ __forceinline__ void store16_f32(float* row, int c0, int hh, int d, const v16f& v, float f) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int c = c0 + 16 * (q >> 1) + 8 * hh + 4 * (q & 1);
+    if (c < d) *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * q] * f, v[4 * q + 1] * f, v[4 * q + 2] * f, v[4 * q + 3] * f);
   }
 }
 
@@ -227,6 +322,18 @@ constexpr int stride_both(int D) {
     const int m = (s / 4) % 64;
     if ((s / 16) % 2 == 1 && s >= nrt(D) * 64 && (m == 12 || m == 20 || m == 44 || m == 52)) return s;
   }
+}
+
+// short states are staged once per workgroup: as many rows each (of pairs x R) as leave `per_cu` workgroups per CU
+inline int short_rows(tfmq_handle h, long pairs, long R, int per_cu) {
+  const long tiles = (R + 127) / 128;
+  return static_cast<int>(std::min<long>(tiles, std::max<long>(1, pairs * tiles / (static_cast<long>(per_cu) * h->cu_count)))) * 128;
+}
+
+// the row walks address an item's rows with 32 bits (2 GiB a tensor and item); longer ones take the tiled kernels
+inline bool rows_fit(const XattnP& p) {
+  const long m = 1L << 30, C = static_cast<long>(p.H) * p.d;
+  return p.Tq * C < m && p.q.ts >= 0 && p.q.ts * p.Tq + C < m && (!p.go.p || (p.go.ts >= 0 && p.go.ts * p.Tq + C < m && p.o.ts >= 0 && p.o.ts * p.Tq + C < m));
 }
 
 // head dims run in the smallest of these that holds them

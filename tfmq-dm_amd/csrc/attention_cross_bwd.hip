@@ -162,7 +162,101 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
   const float f = p.scale * __builtin_amdgcn_exp2f(static_cast<float>(-fe));
   T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
 #pragma unroll
-  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, acc[t], f);
+  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, acc[t], f);
+}
+
+// ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form)
+constexpr int dq_short_waves(int D, int NKT) { return D <= 64 ? 4 : D <= 96 ? 3 : 2; }
+template <typename T, int D, int NKT>
+__global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(XattnP p) {
+  constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_both(D), VS = stride_rows(D), NK = NKT * 32;
+  using V8 = typename Vec8<T>::type;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* sK = smem;
+  unsigned char* sV = smem + NK * KS;
+  float* sB = reinterpret_cast<float*>(smem + NK * (KS + VS));
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
+  const int id = xcd_tile_id();
+  const int rb = id % p.nrb, bg = id / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
+  const long hc = static_cast<long>(g) * p.rep * p.d, C = static_cast<long>(p.H) * p.d, rd = static_cast<long>(p.rep) * p.d;
+  const long brow0 = (static_cast<long>(b) * p.H + g * p.rep) * p.Tq, rows = static_cast<long>(p.B) * p.H * p.Tq;
+  const Rsrc rq = buffer_of(static_cast<const T*>(p.q.p) + b * p.q.bs + hc, ((p.Tq - 1) * p.q.ts + rd) * 2);
+  const Rsrc rg = buffer_of(static_cast<const T*>(p.go.p) + b * p.go.bs + hc, ((p.Tq - 1) * p.go.ts + rd) * 2);
+  const Rsrc ro = buffer_of(static_cast<const T*>(p.o.p) + b * p.o.bs + hc, ((p.Tq - 1) * p.o.ts + rd) * 2);
+  const Rsrc ry = buffer_of(static_cast<T*>(p.y) + b * p.Tq * C + hc, (p.Tq * C - hc) * 2);
+  const Rsrc rl = buffer_of(p.lse_in + brow0, p.R * 4), rdl = buffer_of(p.delta + brow0, p.R * 4), rgm = buffer_of(p.delta + rows + brow0, p.R * 4);
+  const unsigned qts = static_cast<unsigned>(p.q.ts) * 2, gts = static_cast<unsigned>(p.go.ts) * 2, ots = static_cast<unsigned>(p.o.ts) * 2;
+  const unsigned yts = static_cast<unsigned>(C) * 2, hs = static_cast<unsigned>(p.d) * 2;
+
+  const long r_end = min(p.R, (static_cast<long>(rb) + 1) * p.rows_per);
+  RowWalk w(static_cast<long>(rb) * p.rows_per + wid * 32 + j, p.Tq);
+  V8 qf[NKS], gf[NKS], of[NKS];
+  float lse = 0.0f;
+  auto load_rows = [&]() {
+    const bool ok = w.row < r_end && w.i < qlen;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = ks * 16 + hh * 8;
+      const bool there = ok && c < p.d;
+      const unsigned col = w.hi * hs + c * 2;
+      qf[ks] = load8<V8>(rq, there ? w.i * qts + col : NOWHERE);
+      gf[ks] = load8<V8>(rg, there ? w.i * gts + col : NOWHERE);
+      of[ks] = load8<V8>(ro, there ? w.i * ots + col : NOWHERE);
+    }
+    lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, static_cast<int>(ok ? static_cast<unsigned>(w.row) * 4 : NOWHERE), 0, 0));
+  };
+  load_rows();
+  stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);
+  const float c2 = p.scale * LOG2E;
+  while (w.row - j < r_end) {
+    const bool in = w.row < r_end, ok = in && w.i < qlen;
+    const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
+    float dl = 0.0f, gm = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = static_cast<float>(gf[ks][e]);
+        dl = __builtin_fmaf(static_cast<float>(of[ks][e]), x, dl);
+        if (is_f16<T>()) gm = fmaxf(gm, fabsf(x));
+      }
+    dl += __shfl_xor(dl, 32, 64);
+    gm = fmaxf(gm, __shfl_xor(gm, 32, 64));
+    const int fe = is_f16<T>() ? inv_exponent(gm) : 0;
+    const float sh = (ok && lse != -INFINITY ? lse * LOG2E : INFINITY) - static_cast<float>(fe);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), rdl, static_cast<int>(loff), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(gm), rgm, static_cast<int>(loff), 0, 0);
+    V8 df[2 * NKT];
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt) {
+      hold_order();                      // (one key tile's scores at a time: all of them at once would spill)
+      v16f s = start_scores(sB + kt * 32, hh), dp = zero16();
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        s = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s);
+        dp = mfma16(frag_rows<T>(sV, VS, kt * 32 + j, ks, hh), gf[ks], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -sh)) * (dp[r] - dl);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) df[2 * kt + u] = frag_regs<T>(s, u);
+    }
+    hold_order();
+    w.step();
+    load_rows();
+    v16f acc[NRT];
+#pragma unroll
+    for (int t = 0; t < NRT; ++t) acc[t] = zero16();
+#pragma unroll
+    for (int u = 0; u < 2 * NKT; ++u)
+#pragma unroll
+      for (int t = 0; t < NRT; ++t) acc[t] = mfma16(frag_cols<T>(sK, KS, u * 16, t, lane), df[u], acc[t]);
+    zero_unless(ok, acc);
+    const float f = p.scale * __builtin_amdgcn_exp2f(static_cast<float>(-fe));
+#pragma unroll
+    for (int t = 0; t < NRT; ++t) store16<T>(ry, yoff, in, t * 32, hh, p.d, acc[t], f);
+  }
 }
 
 template <int D> constexpr int dkv_rows() { return D <= 128 ? 64 : 32; }
@@ -325,20 +419,16 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
     const long n = static_cast<long>(p.B) * p.Tk * p.G * p.d;
     float* pk = p.part + 2 * sp * n + krow * p.d;
 #pragma unroll
-    for (int t = 0; t < NRT; ++t)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int c = t * 32 + 16 * hh + 4 * q4;
-        if (c >= p.d) continue;
-        *reinterpret_cast<float4*>(pk + c) = make_float4(ak[t][4 * q4] * fk, ak[t][4 * q4 + 1] * fk, ak[t][4 * q4 + 2] * fk, ak[t][4 * q4 + 3] * fk);
-        *reinterpret_cast<float4*>(pk + n + c) = make_float4(av[t][4 * q4] * fv, av[t][4 * q4 + 1] * fv, av[t][4 * q4 + 2] * fv, av[t][4 * q4 + 3] * fv);
-      }
+    for (int t = 0; t < NRT; ++t) {
+      store16_f32(pk, t * 32, hh, p.d, ak[t], fk);
+      store16_f32(pk + n, t * 32, hh, p.d, av[t], fv);
+    }
     return;
   }
 #pragma unroll
   for (int t = 0; t < NRT; ++t) {
-    store16<T>(static_cast<T*>(p.dk) + krow * p.d, t * 32 + 16 * hh, p.d, ak[t], fk);
-    store16<T>(static_cast<T*>(p.dv) + krow * p.d, t * 32 + 16 * hh, p.d, av[t], fv);
+    store16<T>(static_cast<T*>(p.dk) + krow * p.d, t * 32, hh, p.d, ak[t], fk);
+    store16<T>(static_cast<T*>(p.dv) + krow * p.d, t * 32, hh, p.d, av[t], fv);
   }
 }
 
@@ -362,24 +452,50 @@ __global__ __launch_bounds__(256) void k_xattn_sum(XattnP p, long n) {
   *reinterpret_cast<typename Vec8<T>::type*>(out) = w;
 }
 
+template <typename T, int D, int NKT>
+int launch_dq_short(tfmq_handle h, XattnP p, hipStream_t st) {
+  auto kern = &k_xattn_dq_short<T, D, NKT>;
+  constexpr int smem = NKT * 32 * (stride_both(D) + stride_rows(D) + 4);
+  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const long pairs = static_cast<long>(p.B) * p.G;
+  p.rows_per = short_rows(h, pairs, p.R, dq_short_waves(D, NKT));
+  p.nrb = ceil_div(p.R, p.rows_per);
+  TFMQ_CHECK_ARG(h, pairs * p.nrb < (1L << 31), "xattn_bwd: too many workgroups");
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(pairs * p.nrb)), dim3(256), smem, st, p);
+  TFMQ_LAUNCH_CHECK(h);
+  return TFMQ_OK;
+}
+template <typename T, int D>
+int launch_dq(tfmq_handle h, XattnP p, hipStream_t st) {
+  const int nkt = rows_fit(p) ? (p.Tk + 31) / 32 : 5;
+  if (nkt == 1) return launch_dq_short<T, D, 1>(h, p, st);
+  if (nkt == 2) return launch_dq_short<T, D, 2>(h, p, st);
+  if (nkt == 3) return launch_dq_short<T, D, 3>(h, p, st);
+  if (nkt == 4) return launch_dq_short<T, D, 4>(h, p, st);
+  auto kern = &k_xattn_dq<T, D>;
+  constexpr int smem = 64 * (stride_both(D) + stride_rows(D));
+  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  p.nrb = ceil_div(p.R, 128);
+  const long n = static_cast<long>(p.B) * p.G * p.nrb;
+  TFMQ_CHECK_ARG(h, n < (1L << 31), "xattn_bwd: too many workgroups");
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(n)), dim3(256), smem, st, p);
+  TFMQ_LAUNCH_CHECK(h);
+  return TFMQ_OK;
+}
+
 template <typename T>
 int launch_bwd(tfmq_handle h, XattnP p, hipStream_t st) {
   return for_head_dim(p.d, [&](auto dc) {
     constexpr int D = decltype(dc)::value;
-    auto kq = &k_xattn_dq<T, D>;
     auto kk = &k_xattn_dkv<T, D>;
-    constexpr int sq = 64 * (stride_both(D) + stride_rows(D)), sk = 2 * dkv_rows<D>() * (stride_both(D) + 4) + 16;
-    TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kq), hipFuncAttributeMaxDynamicSharedMemorySize, sq));
+    constexpr int sk = 2 * dkv_rows<D>() * (stride_both(D) + 4) + 16;
     TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kk), hipFuncAttributeMaxDynamicSharedMemorySize, sk));
-    XattnP a = p;
-    a.nrb = ceil_div(p.R, 128);
-    const long nq = static_cast<long>(p.B) * p.G * a.nrb;
+    const int rc = launch_dq<T, D>(h, p, st);
+    if (rc != TFMQ_OK) return rc;
     XattnP c = p;
     c.nrb = ceil_div(p.Tk, 128);
     const long nk = static_cast<long>(p.B) * p.G * c.nrb * p.nsplit;
-    TFMQ_CHECK_ARG(h, nq < (1L << 31) && nk < (1L << 31), "xattn_bwd: too many workgroups");
-    hipLaunchKernelGGL(kq, dim3(static_cast<unsigned>(nq)), dim3(256), sq, st, a);
-    TFMQ_LAUNCH_CHECK(h);
+    TFMQ_CHECK_ARG(h, nk < (1L << 31), "xattn_bwd: too many workgroups");
     hipLaunchKernelGGL(kk, dim3(static_cast<unsigned>(nk)), dim3(256), sk, st, c);
     TFMQ_LAUNCH_CHECK(h);
     if (p.nsplit > 1) {

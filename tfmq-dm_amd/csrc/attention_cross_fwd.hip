@@ -7,7 +7,6 @@
 // while the previous tile is multiplied, and stored to LDS row-major; V is read transposed by ds_read_b64_tr_b16.  Scores, statistics and sums are fp32;
 // the probabilities are rounded to the operand type for the second product (they are <= 1, the sum takes them unrounded).
 #include "attention_cross.hpp"
-#include <algorithm>
 
 using namespace xattn;
 
@@ -128,13 +127,7 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
     // slice sp's sums against its own maximum: [slice][row][d] and {m, l} behind them
     float* po = p.part + (static_cast<long>(sp) * p.B * p.H * p.Tq + orow) * p.d;
 #pragma unroll
-    for (int t = 0; t < NRT; ++t) {
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int c = t * 32 + 16 * hh + 4 * q4;
-        if (c < p.d) *reinterpret_cast<float4*>(po + c) = make_float4(o[t][4 * q4], o[t][4 * q4 + 1], o[t][4 * q4 + 2], o[t][4 * q4 + 3]);
-      }
-    }
+    for (int t = 0; t < NRT; ++t) store16_f32(po, t * 32, hh, p.d, o[t], 1.0f);
     if (hh == 0) {
       float* ml = p.part + static_cast<long>(p.nsplit) * p.B * p.H * p.Tq * p.d + (static_cast<long>(sp) * p.B * p.H * p.Tq + orow) * 2;
       ml[0] = ok ? m : -INFINITY;
@@ -145,97 +138,65 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
   const float inv = ok && l != 0.0f ? 1.0f / l : 0.0f;
   T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
 #pragma unroll
-  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, o[t], inv);
+  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, o[t], inv);
   if (p.lse && hh == 0) p.lse[orow] = ok && l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 // ---- up to 128 states (a text encoder's): K and V of one (item, key head) stay in LDS, the waves walk over rows on their own, without barriers, the next
 // rows' queries under way.  All keys are in the accumulators at once: one maximum, no running rescale.
-// registers of the scores, the sums and two sets of queries; past 160 the kernel would spill at two waves per SIMD
-constexpr int short_regs(int D, int NKT) { return NKT * 16 + nrt(D) * 16 + nks(D) * 8; }
-constexpr bool short_fits(int D, int NKT) { return NKT <= 2 || short_regs(D, NKT) <= 160; }
+// waves per SIMD that the registers allow without spilling (the walk waits for memory: 4 against 2 took the 128 x 1024 x 77 call from 114 to FWDSHORT us)
+constexpr int short_waves(int D, int NKT) { return D <= 64 || (D <= 96 && NKT <= 3) ? 4 : D <= 128 || NKT <= 2 ? 3 : 2; }
 
 template <typename T, int D, int NKT>
-__global__ __launch_bounds__(256, short_regs(D, NKT) > 104 ? 2 : 3) void k_xattn_short(XattnP p) {
+__global__ __launch_bounds__(256, short_waves(D, NKT)) void k_xattn_short(XattnP p) {
   constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_rows(D), VS = stride_cols(D), NK = NKT * 32;
   using V8 = typename Vec8<T>::type;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   unsigned char* sK = smem;
   unsigned char* sV = smem + NK * KS;
+  float* sB = reinterpret_cast<float*>(smem + NK * (KS + VS));
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
   const int id = xcd_tile_id();
   const int rb = id % p.nrb, bg = id / p.nrb, b = bg / p.G, g = bg - b * p.G;
   const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
-  const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
-  const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
-  const uint8_t* mb = p.mask ? p.mask + b * p.mask_bs : nullptr;
-  const T* qb = static_cast<const T*>(p.q.p) + b * p.q.bs + static_cast<long>(g) * p.rep * p.d;
+  const long hc = static_cast<long>(g) * p.rep * p.d, C = static_cast<long>(p.H) * p.d;
+  const Rsrc rq = buffer_of(static_cast<const T*>(p.q.p) + b * p.q.bs + hc, ((p.Tq - 1) * p.q.ts + static_cast<long>(p.rep) * p.d) * 2);
+  const Rsrc ry = buffer_of(static_cast<T*>(p.y) + b * p.Tq * C + hc, (p.Tq * C - hc) * 2);
+  const Rsrc rl = buffer_of(p.lse ? p.lse + (static_cast<long>(b) * p.H + g * p.rep) * p.Tq : nullptr, p.lse ? p.R * 4 : 0);
+  const unsigned qts = static_cast<unsigned>(p.q.ts) * 2, yts = static_cast<unsigned>(C) * 2, hs = static_cast<unsigned>(p.d) * 2;
 
   const long r_end = min(p.R, (static_cast<long>(rb) + 1) * p.rows_per);
-  long row = static_cast<long>(rb) * p.rows_per + wid * 32 + j;
+  RowWalk w(static_cast<long>(rb) * p.rows_per + wid * 32 + j, p.Tq);
   V8 qf[NKS];
-  bool ok = false;
-  int hi = 0, i = 0;
-  auto load_q = [&](long r) {
-    hi = static_cast<int>(r / p.Tq);
-    i = static_cast<int>(r - static_cast<long>(hi) * p.Tq);
-    ok = r < r_end && i < qlen;
-    const T* qrow = qb + i * p.q.ts + static_cast<long>(hi) * p.d;
+  auto load_q = [&]() {
+    const unsigned off = w.row < r_end && w.i < qlen ? w.i * qts + w.hi * hs : NOWHERE;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) {
       const int c = ks * 16 + hh * 8;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (ok && c < p.d) w = *reinterpret_cast<const uint4*>(qrow + c);
-      qf[ks] = __builtin_bit_cast(V8, w);
+      qf[ks] = load8<V8>(rq, off != NOWHERE && c < p.d ? off + c * 2 : NOWHERE);
     }
   };
-  load_q(row);
-  unsigned long long keep[2] = {0, 0};
-  {
-#pragma unroll
-    for (int w = 0; w < (NKT + 1) / 2; ++w) {
-      const int key = w * 64 + lane;
-      keep[w] = __ballot(key < klen && (!mb || mb[min(key, p.Tk - 1)] != 0));
-    }
-#pragma unroll
-    for (int t = 0; t < NKT; ++t) {          // 32 keys at a time
-      KeyTile<T, D, 32, KS> tk;
-      KeyTile<T, D, 32, VS> tv;
-      const int k0 = min(t * 32, p.Tk - 1);
-      tk.load(kb, p.k.ts, k0, p.Tk, p.d);
-      tv.load(vb, p.v.ts, k0, p.Tk, p.d);
-      const unsigned long long kk = (keep[t >> 1] >> (32 * (t & 1))) & 0xffffffffull;
-      tk.store(sK + t * 32 * KS, kk, 0xffffffffull, p.d);
-      tv.store(sV + t * 32 * VS, kk, 0xffffffffull, p.d);
-    }
-  }
-  __syncthreads();
-  const bool every = keep[0] == (NKT == 1 ? 0xffffffffull : ~0ull) && (NKT <= 2 || keep[1] == (NKT == 3 ? 0xffffffffull : ~0ull));
+  load_q();
+  stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);
   const float c2 = p.scale * LOG2E;
-  while (row - j < r_end) {
-    const long orow = (static_cast<long>(b) * p.H + g * p.rep + hi) * p.Tq + i;
-    T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(g * p.rep + hi) * p.d;
-    const bool in = row < r_end, cur = ok;
+  while (w.row - j < r_end) {
+    const bool in = w.row < r_end, ok = in && w.i < qlen;
+    const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
     v16f s[NKT];
 #pragma unroll
     for (int kt = 0; kt < NKT; ++kt) {
-      s[kt] = zero16();
+      s[kt] = start_scores(sB + kt * 32, hh);
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) s[kt] = mfma16(frag_rows<T>(sK, KS, kt * 32 + j, ks, hh), qf[ks], s[kt]);
     }
-    row += 128;
-    if (row - j < r_end) load_q(row);
+    hold_order();
+    w.step();
+    load_q();
     float mx = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < NKT; ++kt) {
-      if (!every) {
-        const unsigned bits = static_cast<unsigned>(keep[kt >> 1] >> (32 * (kt & 1))) >> (4 * hh);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kt][r] = ((bits >> crow(r, 0)) & 1) ? s[kt][r] : -INFINITY;
-      }
+    for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
-    }
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
     const float mu = mx == -INFINITY ? 0.0f : mx;
     float rs[2] = {0.0f, 0.0f};
@@ -248,22 +209,23 @@ __global__ __launch_bounds__(256, short_regs(D, NKT) > 104 ? 2 : 3) void k_xattn
       }
     float l = rs[0] + rs[1];
     l += __shfl_xor(l, 32, 64);
+    V8 pf[2 * NKT];
+#pragma unroll
+    for (int u = 0; u < 2 * NKT; ++u) pf[u] = frag_regs<T>(s[u >> 1], u & 1);
+    hold_order();                        // (the scores' registers are free from here on)
     v16f o[NRT];
 #pragma unroll
     for (int t = 0; t < NRT; ++t) o[t] = zero16();
 #pragma unroll
-    for (int u = 0; u < 2 * NKT; ++u) {
-      const V8 pf = frag_regs<T>(s[u >> 1], u & 1);
+    for (int u = 0; u < 2 * NKT; ++u)
 #pragma unroll
-      for (int t = 0; t < NRT; ++t) o[t] = mfma16(frag_cols<T>(sV, VS, u * 16, t, lane), pf, o[t]);
-    }
-    if (in) {
-      zero_unless(cur, o);
-      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      for (int t = 0; t < NRT; ++t) o[t] = mfma16(frag_cols<T>(sV, VS, u * 16, t, lane), pf[u], o[t]);
+    zero_unless(ok, o);
+    const float inv = ok && l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-      for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32 + 16 * hh, p.d, o[t], inv);
-      if (p.lse && hh == 0) p.lse[orow] = cur && l != 0.0f ? (mx + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
-    }
+    for (int t = 0; t < NRT; ++t) store16<T>(ry, yoff, in, t * 32, hh, p.d, o[t], inv);
+    const float lse = ok && l != 0.0f ? (mx + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse), rl, static_cast<int>(loff), 0, 0);
   }
 }
 
@@ -305,19 +267,15 @@ __global__ __launch_bounds__(256) void k_xattn_join(XattnP p) {
 
 template <typename T, int D, int NKT>
 int launch_short(tfmq_handle h, XattnP p, hipStream_t st) {
-  if constexpr (short_fits(D, NKT)) {
   auto kern = &k_xattn_short<T, D, NKT>;
-  constexpr int smem = NKT * 32 * (stride_rows(D) + stride_cols(D));
+  constexpr int smem = NKT * 32 * (stride_rows(D) + stride_cols(D) + 4);
   TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
-  // the states are staged once per workgroup: as many rows each as leave two workgroups per CU
-  const long pairs = static_cast<long>(p.B) * p.G, tiles = (p.R + 127) / 128;
-  const long per = std::min<long>(tiles, std::max<long>(1, pairs * tiles / (2L * h->cu_count)));
-  p.rows_per = static_cast<int>(per) * 128;
+  const long pairs = static_cast<long>(p.B) * p.G;
+  p.rows_per = short_rows(h, pairs, p.R, short_waves(D, NKT));
   p.nrb = ceil_div(p.R, p.rows_per);
   TFMQ_CHECK_ARG(h, pairs * p.nrb < (1L << 31), "xattn_fwd: too many workgroups");
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(pairs * p.nrb)), dim3(256), smem, st, p);
   TFMQ_LAUNCH_CHECK(h);
-  }
   return TFMQ_OK;
 }
 
@@ -326,7 +284,7 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
   return for_head_dim(p.d, [&](auto dc) {
     constexpr int D = decltype(dc)::value;
     const int nkt = (p.Tk + 31) / 32;
-    if (p.nsplit == 1 && nkt <= 4 && short_fits(D, nkt)) {
+    if (p.nsplit == 1 && nkt <= 4 && rows_fit(p)) {
       if (nkt == 1) return launch_short<T, D, 1>(h, p, st);
       if (nkt == 2) return launch_short<T, D, 2>(h, p, st);
       if (nkt == 3) return launch_short<T, D, 3>(h, p, st);
