@@ -45,6 +45,7 @@ BASE = dict(q=(2, 5, 64), k=(2, 7, 64), v=(2, 7, 64), heads=2, scale=1.0)
     (dict(q=_z(2, 64, 5).transpose(1, 2)), "unit channel stride"),
     (dict(k=_z(2, 7, 65)[..., 1:]), "aligned"),
     (dict(v=_z(2, 7, 68)[..., :64]), "aligned"),
+    (dict(k=torch.empty_strided((2, 2, 64), (1 << 24, 1 << 23, 1), dtype=F16, device="meta"), v=_z(2, 2, 64)), "token strides"),
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(kv_lens=torch.zeros(2, dtype=torch.int64)), "kv_lens"),
     (dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"),
@@ -92,5 +93,12 @@ def test_descriptor_layout_matches_the_header(tmp_path):
     src.write_text('#include <stdio.h>\n#include "tfmq_hip.h"\nint main(void){printf("%zu",sizeof(tfmq_xattn_desc));' +
                    "".join(f'printf(" %zu",offsetof(tfmq_xattn_desc,{n}));' for n in names) + "return 0;}\n")
     subprocess.run([cc, "-I", inc, str(src), "-o", str(tmp_path / "l")], check=True)
+    import tfmq_dm_amd.ops as ops
+    # the packed form that the calls send: the same places (it ends at the last field)
+    last = names[-1]
+    assert ops._XATTN.size == getattr(L.XattnDesc, last).offset + getattr(L.XattnDesc, last).size
+    raw = ops._XATTN.pack(*range(1, 8), 8.0, *range(9, 9 + len(names) - 8))
+    back = L.XattnDesc.from_buffer_copy(raw + bytes(C.sizeof(L.XattnDesc) - len(raw)))
+    assert [getattr(back, n) for n in names] == list(range(1, len(names) + 1))
     got = [int(x) for x in subprocess.run([str(tmp_path / "l")], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [C.sizeof(L.XattnDesc)] + [getattr(L.XattnDesc, n).offset for n in names]

@@ -456,7 +456,8 @@ template <typename T, int D, int NKT>
 int launch_dq_short(tfmq_handle h, XattnP p, hipStream_t st) {
   auto kern = &k_xattn_dq_short<T, D, NKT>;
   constexpr int smem = NKT * 32 * (stride_both(D) + stride_rows(D) + 4);
-  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static LdsRoom room_kern;
+  TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
   const long pairs = static_cast<long>(p.B) * p.G;
   p.rows_per = short_rows(h, pairs, p.R, dq_short_waves(D, NKT));
   p.nrb = ceil_div(p.R, p.rows_per);
@@ -474,7 +475,8 @@ int launch_dq(tfmq_handle h, XattnP p, hipStream_t st) {
   if (nkt == 4) return launch_dq_short<T, D, 4>(h, p, st);
   auto kern = &k_xattn_dq<T, D>;
   constexpr int smem = 64 * (stride_both(D) + stride_rows(D));
-  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static LdsRoom room_kern;
+  TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
   p.nrb = ceil_div(p.R, 128);
   const long n = static_cast<long>(p.B) * p.G * p.nrb;
   TFMQ_CHECK_ARG(h, n < (1L << 31), "xattn_bwd: too many workgroups");
@@ -489,7 +491,8 @@ int launch_bwd(tfmq_handle h, XattnP p, hipStream_t st) {
     constexpr int D = decltype(dc)::value;
     auto kk = &k_xattn_dkv<T, D>;
     constexpr int sk = 2 * dkv_rows<D>() * (stride_both(D) + 4) + 16;
-    TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kk), hipFuncAttributeMaxDynamicSharedMemorySize, sk));
+    static LdsRoom room_kk;
+  TFMQ_HIP(h, room_kk.ask(h, reinterpret_cast<const void*>(kk), sk));
     const int rc = launch_dq<T, D>(h, p, st);
     if (rc != TFMQ_OK) return rc;
     XattnP c = p;

@@ -269,7 +269,8 @@ template <typename T, int D, int NKT>
 int launch_short(tfmq_handle h, XattnP p, hipStream_t st) {
   auto kern = &k_xattn_short<T, D, NKT>;
   constexpr int smem = NKT * 32 * (stride_rows(D) + stride_cols(D) + 4);
-  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static LdsRoom room_kern;
+  TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
   const long pairs = static_cast<long>(p.B) * p.G;
   p.rows_per = short_rows(h, pairs, p.R, short_waves(D, NKT));
   p.nrb = ceil_div(p.R, p.rows_per);
@@ -292,7 +293,8 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
     }
     auto kern = &k_xattn_fwd<T, D>;
     constexpr int smem = 64 * (stride_rows(D) + stride_cols(D));
-    TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static LdsRoom room_kern;
+  TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
     p.nrb = ceil_div(p.R, 128);
     const long nb = static_cast<long>(p.B) * p.G * p.nrb * p.nsplit;
     TFMQ_CHECK_ARG(h, nb < (1L << 31), "xattn_fwd: too many workgroups");

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -101,6 +102,18 @@ struct DeviceGuard {
   }
   ~DeviceGuard() {
     if (switched) (void)hipSetDevice(prev);
+  }
+};
+
+// Dynamic LDS beyond 64 KB has to be asked for once per kernel and device (one static object per kernel; asking twice is harmless).
+struct LdsRoom {
+  std::atomic<unsigned long long> done{0};
+  hipError_t ask(tfmq_handle h, const void* kernel, int bytes) {
+    const unsigned long long bit = 1ull << (h->device & 63);
+    if (h->device < 64 && (done.load(std::memory_order_acquire) & bit)) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
   }
 };
 

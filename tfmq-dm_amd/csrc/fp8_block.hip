@@ -520,7 +520,8 @@ template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
 int launch_gemm(tfmq_handle h, GemmF8P p, hipStream_t st) {
   constexpr int NW = (BM / WM) * (BN / WN), smem = 2 * (BM + BN) * 128 + (SBROW ? NW * WN * 4 : 0);
   auto kern = &k_gemm_f8<BM, BN, WM, WN, YDT, SBROW, WPS>;
-  TFMQ_HIP(h, hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static LdsRoom room_kern;
+  TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
   p.tm = ceil_div(p.M, BM);
   p.tn = ceil_div(p.N, BN);
   const long nt = static_cast<long>(p.tm) * p.tn;

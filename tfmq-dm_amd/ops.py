@@ -9,11 +9,12 @@ from __future__ import annotations
 import ctypes as C
 import contextvars
 import os
+import struct
 from typing import Optional, Tuple
 
 import torch
 
-from ._lib import ChainDesc, ConvDesc, FfDesc, GnDesc, QSel, TfmqError, XattnDesc
+from ._lib import ChainDesc, ConvDesc, FfDesc, GnDesc, QSel, TfmqError
 from ._lib import handle as _lib_handle
 
 NULL = None
@@ -147,8 +148,12 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+# the current stream's handle without building a Stream object (1 us of every call's host time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _stream(dev: int):
-    return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    return C.c_void_p(_raw_stream(dev))
 
 
 def _chk(t: torch.Tensor, dtype, name: str):
@@ -1755,9 +1760,10 @@ def _rows2d(x: torch.Tensor, name: str):
     tensor included); unit column stride."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise TfmqError(f"{name}: expected [..., K] with K >= 1, got {tuple(x.shape)}")
-    K, M = x.shape[-1], x.numel() // x.shape[-1]
-    if M == 0:
-        return 0, K, K
+    K = x.shape[-1]
+    M = x.numel() // K
+    if M == 0 or x.is_contiguous():
+        return M, K, K
     if K > 1 and x.stride(-1) != 1:
         raise TfmqError(f"{name}: the last dimension must have unit stride")
     ld, span = None, None
@@ -1776,10 +1782,10 @@ def _rows2d(x: torch.Tensor, name: str):
     return M, K, ld
 
 
-def _same_device(d: int, **tensors):
-    for n, t in tensors.items():
+def _same_device(d: int, *tensors):
+    for t in tensors:
         if t is not None and _dev(t) != d:
-            raise TfmqError(f"{n}: on cuda:{_dev(t)}, the call is on cuda:{d}")
+            raise TfmqError(f"operands on cuda:{_dev(t)} and cuda:{d} in one call")
 
 
 class QuantFp8:
@@ -1797,6 +1803,9 @@ class PackedFp8:
 
     def __init__(self, q, qt, scale, bias, N, K):
         self.q, self.qt, self.scale, self.bias, self.N, self.K = q, qt, scale, bias, N, K
+        self.Kb = scale.shape[1]
+        # addresses of this object's own tensors, which never change
+        self._q, self._qt, self._scale, self._bias = q.data_ptr(), qt.data_ptr(), scale.data_ptr(), None if bias is None else bias.data_ptr()
 
 
 def quantize_fp8(x: torch.Tensor) -> QuantFp8:
@@ -1830,7 +1839,7 @@ def _bias_f32(bias, N: int, d: int, name: str):
         return None
     if tuple(bias.shape) != (N,):
         raise TfmqError(f"{name}: bias must be [{N}], got {tuple(bias.shape)}")
-    _same_device(d, bias=bias)
+    _same_device(d, bias)
     return bias.detach().float().contiguous()
 
 
@@ -1860,7 +1869,7 @@ def load_w_fp8(q: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor
     Nb, Kb = (N + 127) // 128, (K + 127) // 128
     if scale.dtype != torch.float32 or tuple(scale.shape) != (Nb, Kb):
         raise TfmqError(f"load_w_fp8: scale must be fp32 [{Nb}, {Kb}], got {scale.dtype} {tuple(scale.shape)}")
-    _same_device(d, scale=scale)
+    _same_device(d, scale)
     b = q.contiguous().view(torch.uint8)
     q8 = torch.zeros(N, Kb * 128, dtype=torch.uint8, device=q.device)
     qt = torch.zeros(K, Nb * 128, dtype=torch.uint8, device=q.device)
@@ -1880,7 +1889,7 @@ def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> tor
         raise TfmqError(f"linear_fp8: output type must be fp32, fp16 or bf16, got {out_dtype}")
     if x.shape[-1] != pw.K:
         raise TfmqError(f"linear_fp8: x has {x.shape[-1]} channels, the weight {pw.K}")
-    _same_device(d, weight=pw.q)
+    _same_device(d, pw.q)
     if quantised:
         M, dt, ld = src.shape[0], 0, 0
     else:
@@ -1892,8 +1901,9 @@ def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> tor
     h = handle(d)
     nb = 0 if quantised else h.lib.tfmq_linear_fp8_ws_bytes(h.h, M, pw.N, pw.K)
     ws = _alloc(nb, dtype=torch.uint8, device=src.device) if nb else None
-    h.call("linear_fp8", None if quantised else _p(x), dt, M, pw.K, ld, _p(x.q) if quantised else None, _p(x.scale) if quantised else None, _p(pw.q),
-           _p(pw.scale), pw.scale.shape[1], 1, _p(pw.bias), _p(y), _DT_CODE[out_dtype], pw.N, _p(ws), _stream(d))
+    xp, qp, sp = (None, src.data_ptr(), x.scale.data_ptr()) if quantised else (x.data_ptr(), None, None)
+    h.call("linear_fp8", xp, dt, M, pw.K, ld, qp, sp, pw._q, pw._scale, pw.Kb, 1, pw._bias, y.data_ptr(), _DT_CODE[out_dtype], pw.N,
+           None if ws is None else ws.data_ptr(), _stream(d))
     return y
 
 
@@ -1902,7 +1912,7 @@ def linear_fp8_bwd(x: torch.Tensor, gy: torch.Tensor, pw: PackedFp8, want_gx: bo
     gw = gy^T x (both quantised down their columns, one scale per 128 tokens) in fp32.  -> (gx [..., K] | None, gw [N, K] | None).  The rounding
     of the forward's operands is passed straight through; the bias gradient is gy summed over its rows.  The same bits on every call."""
     d = _dev(gy)
-    _same_device(d, x=x, weight=pw.q)
+    _same_device(d, x, pw.q)
     if x.shape[-1] != pw.K or gy.shape[-1] != pw.N or x.shape[:-1] != gy.shape[:-1]:
         raise TfmqError(f"linear_fp8_bwd: x {tuple(x.shape)} and gy {tuple(gy.shape)} do not fit a weight [{pw.N}, {pw.K}]")
     dx, dg = _dt_code(x, "linear_fp8_bwd"), _dt_code(gy, "linear_fp8_bwd")
@@ -1918,57 +1928,78 @@ def linear_fp8_bwd(x: torch.Tensor, gy: torch.Tensor, pw: PackedFp8, want_gx: bo
         h = handle(d)
         nb = h.lib.tfmq_linear_fp8_bwd_ws_bytes(h.h, M, pw.N, pw.K, int(want_gx), int(want_gw))
         ws = _alloc(nb, dtype=torch.uint8, device=gy.device) if nb else None
-        h.call("linear_fp8_bwd", _p(x), dx, ldx, _p(gy), dg, ldg, M, pw.N, pw.K, _p(pw.qt), _p(pw.scale), _p(gx), _p(gw), _p(ws), _stream(d))
+        h.call("linear_fp8_bwd", x.data_ptr(), dx, ldx, gy.data_ptr(), dg, ldg, M, pw.N, pw.K, pw._qt, pw._scale, None if gx is None else gx.data_ptr(),
+               None if gw is None else gw.data_ptr(), None if ws is None else ws.data_ptr(), _stream(d))
     return gx, gw
 
 
 # ------------------------------------------------------------------------------ K18: cross attention to an encoder's states
-def _xattn_view(t: torch.Tensor, T: int, C_: int, B: int, dtype, name: str):
+# tfmq_xattn_desc as the C compiler lays it out (_lib.XattnDesc; packing it in one go is a third of the host time of assigning its fields)
+_XATTN = struct.Struct("@7i f 3P 6q 3P q P 2q 2P 2q 4P i")
+
+
+def _xattn_view(t: torch.Tensor, T: int, C_: int, B: int, dtype, name: str, what: str):
     """(pointer, batch stride, token stride) of a [B, T, C] operand: unit channel stride, rows 16-byte aligned."""
-    if tuple(t.shape) != (B, T, C_):
-        raise TfmqError(f"{name}: expected [{B}, {T}, {C_}], got {tuple(t.shape)}")
+    if t.shape != (B, T, C_):
+        raise TfmqError(f"{name} {what}: expected [{B}, {T}, {C_}], got {tuple(t.shape)}")
     if t.dtype != dtype:
-        raise TfmqError(f"{name}: expected {dtype}, got {t.dtype}")
-    bs = t.stride(0) if B > 1 else 0
-    ts = t.stride(1) if T > 1 else 0
-    if t.numel() and (t.stride(2) != 1 or bs % 8 or ts % 8 or t.data_ptr() % 16):
-        raise TfmqError(f"{name}: needs unit channel stride and 16-byte aligned rows (strides {tuple(t.stride())}, address % 16 = {t.data_ptr() % 16})")
-    return t.data_ptr(), bs, ts
+        raise TfmqError(f"{name} {what}: expected {dtype}, got {t.dtype}")
+    p = t.data_ptr()
+    bs, ts, cs = t.stride()
+    bs, ts = bs if B > 1 else 0, ts if T > 1 else 0
+    if (cs != 1 or bs % 8 or ts % 8 or p % 16) and t.numel():
+        raise TfmqError(f"{name} {what}: needs unit channel stride and 16-byte aligned rows (strides {t.stride()}, address % 16 = {p % 16})")
+    return p, bs, ts
 
 
-def _xattn_desc(q, k, v, heads: int, scale: float, kv_heads, q_lens, kv_lens, mask, name: str):
-    d_ = _dev(q)
-    _same_device(d_, k=k, v=v, q_lens=q_lens, kv_lens=kv_lens, mask=mask)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TfmqError(f"{name}: fp16 or bf16 operands (fp32: attention_f32_fwd), got {q.dtype}")
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
-        raise TfmqError(f"{name}: q, k, v must be [B, T, heads * d]")
-    B, Tq, Cq = q.shape
-    Tk = k.shape[1]
-    G = heads if kv_heads is None else int(kv_heads)
-    if heads < 1 or G < 1 or Cq % heads or heads % G:
-        raise TfmqError(f"{name}: {Cq} channels do not split into {heads} heads over {G} key heads")
-    d = Cq // heads
-    if d % 8 or not 0 < d <= 160:
-        raise TfmqError(f"{name}: head dim {d} (a multiple of 8, at most 160)")
-    scale = float(scale)
-    if not (0.0 < scale < float("inf")):
-        raise TfmqError(f"{name}: scale must be positive and finite, got {scale}")
-    a = XattnDesc()
-    a.dtype, a.B, a.H, a.G, a.Tq, a.Tk, a.d, a.scale = _DT_CODE[q.dtype], B, heads, G, Tq, Tk, d, scale
-    a.q, a.q_bs, a.q_ts = _xattn_view(q, Tq, Cq, B, q.dtype, name + " q")
-    a.k, a.k_bs, a.k_ts = _xattn_view(k, Tk, G * d, B, q.dtype, name + " k")
-    a.v, a.v_bs, a.v_ts = _xattn_view(v, Tk, G * d, B, q.dtype, name + " v")
-    for n, t in (("q_lens", q_lens), ("kv_lens", kv_lens)):
-        if t is not None:
-            if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
-                raise TfmqError(f"{name}: {n} must be contiguous int32 [{B}], got {t.dtype} {tuple(t.shape)}")
-            setattr(a, n, t.data_ptr())
-    if mask is not None:
-        if mask.dtype != torch.bool or tuple(mask.shape) != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
-            raise TfmqError(f"{name}: mask must be bool [{B}, {Tk}] (True: attend) with unit key stride, got {mask.dtype} {tuple(mask.shape)}")
-        a.mask, a.mask_bs = mask.data_ptr(), mask.stride(0)
-    return d_, a
+class _Xattn:
+    """A checked call: sizes, and the packed descriptor's fields."""
+    __slots__ = ("d_", "dt", "B", "H", "G", "Tq", "Tk", "d", "scale", "q", "k", "v", "ql", "kl", "mask", "mask_bs")
+
+    def __init__(self, q, k, v, heads: int, scale: float, kv_heads, q_lens, kv_lens, mask, name: str):
+        self.d_ = d_ = _dev(q)
+        _same_device(d_, k, v, q_lens, kv_lens, mask)
+        dt = q.dtype
+        if dt is not torch.float16 and dt is not torch.bfloat16:
+            raise TfmqError(f"{name}: fp16 or bf16 operands (fp32: attention_f32_fwd), got {dt}")
+        if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+            raise TfmqError(f"{name}: q, k, v must be [B, T, heads * d]")
+        B, Tq, Cq = q.shape
+        Tk = k.shape[1]
+        G = heads if kv_heads is None else int(kv_heads)
+        if heads < 1 or G < 1 or Cq % heads or heads % G:
+            raise TfmqError(f"{name}: {Cq} channels do not split into {heads} heads over {G} key heads")
+        d = Cq // heads
+        if d % 8 or not 0 < d <= 160:
+            raise TfmqError(f"{name}: head dim {d} (a multiple of 8, at most 160)")
+        scale = float(scale)
+        if not (0.0 < scale < float("inf")):
+            raise TfmqError(f"{name}: scale must be positive and finite, got {scale}")
+        self.dt, self.B, self.H, self.G, self.Tq, self.Tk, self.d, self.scale = _DT_CODE[dt], B, heads, G, Tq, Tk, d, scale
+        self.q = _xattn_view(q, Tq, Cq, B, dt, name, "q")
+        self.k = _xattn_view(k, Tk, G * d, B, dt, name, "k")
+        self.v = _xattn_view(v, Tk, G * d, B, dt, name, "v")
+        if max(self.k[2], self.v[2]) >= 1 << 23 or min(self.k[2], self.v[2]) < 0:
+            raise TfmqError(f"{name}: token strides of k and v must lie in [0, 2^23) elements, got {self.k[2]} and {self.v[2]}")
+        self.ql = self.kl = self.mask = self.mask_bs = 0
+        if q_lens is not None:
+            self.ql = self._lens(q_lens, "q_lens", name)
+        if kv_lens is not None:
+            self.kl = self._lens(kv_lens, "kv_lens", name)
+        if mask is not None:
+            if mask.dtype != torch.bool or mask.shape != (B, Tk) or (Tk > 1 and mask.stride(1) != 1):
+                raise TfmqError(f"{name}: mask must be bool [{B}, {Tk}] (True: attend) with unit key stride, got {mask.dtype} {tuple(mask.shape)}")
+            self.mask, self.mask_bs = mask.data_ptr(), mask.stride(0)
+
+    def _lens(self, t, n: str, name: str) -> int:
+        if t.dtype != torch.int32 or t.shape != (self.B,) or not t.is_contiguous():
+            raise TfmqError(f"{name}: {n} must be contiguous int32 [{self.B}], got {t.dtype} {tuple(t.shape)}")
+        return t.data_ptr()
+
+    def pack(self, o, lse: int, ws: int, nsplit: int, go=(0, 0, 0), dq: int = 0, dk: int = 0, dv: int = 0) -> bytes:
+        q, k, v = self.q, self.k, self.v
+        return _XATTN.pack(self.dt, self.B, self.H, self.G, self.Tq, self.Tk, self.d, self.scale, q[0], k[0], v[0], q[1], q[2], k[1], k[2], v[1], v[2],
+                           self.ql, self.kl, self.mask, self.mask_bs, o[0], o[1], o[2], lse, go[0], go[1], go[2], dq, dk, dv, ws, nsplit)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, scale: float, kv_heads: Optional[int] = None,
@@ -1985,19 +2016,18 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: in
     and infinities included, reaches a result.  Lengths and mask are read by the kernels on the current stream.
 
     -> o [B, Tq, heads * d], or (o, lse fp32 [B, heads, Tq]) with lse = log sum exp(scale q k^T) over the kept keys, -inf where there is none."""
-    d_, a = _xattn_desc(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, "cross_attention")
-    o = _alloc(tuple(q.shape), dtype=q.dtype, device=q.device)
+    a = _Xattn(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, "cross_attention")
+    o = _alloc(a.B, a.Tq, a.H * a.d, dtype=q.dtype, device=q.device)
     lse = _alloc(a.B, a.H, a.Tq, dtype=torch.float32, device=q.device) if want_lse else None
-    if q.numel() == 0 or a.Tk == 0:
+    if a.B == 0 or a.Tq == 0 or a.Tk == 0:
         o.zero_()
         if want_lse:
             lse.fill_(float("-inf"))
         return (o, lse) if want_lse else o
-    h = handle(d_)
-    a.nsplit = h.lib.tfmq_xattn_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk)
-    ws = _alloc(a.nsplit * a.B * a.H * a.Tq * (a.d + 2), dtype=torch.float32, device=q.device) if a.nsplit > 1 else None
-    a.o, a.lse, a.ws = o.data_ptr(), (lse.data_ptr() if want_lse else None), (ws.data_ptr() if ws is not None else None)
-    h.call("xattn_fwd", C.byref(a), _stream(d_))
+    h = handle(a.d_)
+    n = h.lib.tfmq_xattn_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk) if a.Tk > 128 else 1          # (never sliced below)
+    ws = _alloc(n * a.B * a.H * a.Tq * (a.d + 2), dtype=torch.float32, device=q.device) if n > 1 else None
+    h.call("xattn_fwd", a.pack((o.data_ptr(), 0, 0), lse.data_ptr() if want_lse else 0, 0 if ws is None else ws.data_ptr(), n), _stream(a.d_))
     return (o, lse) if want_lse else o
 
 
@@ -2007,23 +2037,23 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
     """-> (dq, dk, dv) of cross_attention for the upstream gradient g_o [B, Tq, heads * d], given its o and lse; contiguous, in the operands'
     type.  dk / dv of shared key heads are summed over their query heads; dropped keys and rows have zeros; a k or v that was expanded over the
     batch gets its gradient per item.  The same bits on every call."""
-    d_, a = _xattn_desc(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, "cross_attention_bwd")
-    _same_device(d_, o=o, lse=lse, g_o=g_o)
-    a.o, a.o_bs, a.o_ts = _xattn_view(o, a.Tq, a.H * a.d, a.B, q.dtype, "cross_attention_bwd o")
-    a.go, a.go_bs, a.go_ts = _xattn_view(g_o, a.Tq, a.H * a.d, a.B, q.dtype, "cross_attention_bwd g_o")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Tq) or not lse.is_contiguous():
-        raise TfmqError(f"cross_attention_bwd: lse must be contiguous fp32 [{a.B}, {a.H}, {a.Tq}], got {lse.dtype} {tuple(lse.shape)}")
-    dq = _alloc(tuple(q.shape), dtype=q.dtype, device=q.device)
-    dk = _alloc(tuple(k.shape), dtype=q.dtype, device=q.device)
-    dv = _alloc(tuple(v.shape), dtype=q.dtype, device=q.device)
-    if q.numel() == 0 or a.Tk == 0:
+    name = "cross_attention_bwd"
+    a = _Xattn(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, name)
+    _same_device(a.d_, o, lse, g_o)
+    ov = _xattn_view(o, a.Tq, a.H * a.d, a.B, q.dtype, name, "o")
+    gv = _xattn_view(g_o, a.Tq, a.H * a.d, a.B, q.dtype, name, "g_o")
+    if lse.dtype != torch.float32 or lse.shape != (a.B, a.H, a.Tq) or not lse.is_contiguous():
+        raise TfmqError(f"{name}: lse must be contiguous fp32 [{a.B}, {a.H}, {a.Tq}], got {lse.dtype} {tuple(lse.shape)}")
+    dq = _alloc(a.B, a.Tq, a.H * a.d, dtype=q.dtype, device=q.device)
+    dk = _alloc(a.B, a.Tk, a.G * a.d, dtype=q.dtype, device=q.device)
+    dv = _alloc(a.B, a.Tk, a.G * a.d, dtype=q.dtype, device=q.device)
+    if a.B == 0 or a.Tq == 0 or a.Tk == 0:
         for t in (dq, dk, dv):
             t.zero_()
         return dq, dk, dv
-    h = handle(d_)
-    a.nsplit = h.lib.tfmq_xattn_bwd_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk, a.d)
+    h = handle(a.d_)
+    n = h.lib.tfmq_xattn_bwd_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk, a.d)
     rows = (2 * a.B * a.H * a.Tq + 3) // 4 * 4
-    ws = _alloc(rows + (2 * a.nsplit * dk.numel() if a.nsplit > 1 else 0), dtype=torch.float32, device=q.device)
-    a.lse, a.dq, a.dk, a.dv, a.ws = lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr()
-    h.call("xattn_bwd", C.byref(a), _stream(d_))
+    ws = _alloc(rows + (2 * n * a.B * a.Tk * a.G * a.d if n > 1 else 0), dtype=torch.float32, device=q.device)
+    h.call("xattn_bwd", a.pack(ov, lse.data_ptr(), ws.data_ptr(), n, gv, dq.data_ptr(), dk.data_ptr(), dv.data_ptr()), _stream(a.d_))
     return dq, dk, dv
