@@ -53,6 +53,22 @@ struct XattnP {
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int T) { return lens ? min(max(lens[b], 0), T) : T; }
 
+// (pair = item and key head, block of it) of this workgroup, `nb` blocks a pair: a pair's blocks stay on one XCD (they read the same K and V), and
+// neighbouring pairs go to different ones, so that items of different lengths load the XCDs evenly.  (Placement is a matter of speed only.)
+__device__ __forceinline__ void pair_block(int npair, int nb, int& pair, int& blk) {
+  int q = blockIdx.x;
+  const int whole = npair / 8 * 8;
+  if (q < whole * nb) {
+    const int t = q >> 3;
+    pair = t / nb * 8 + (q & 7);
+    blk = t % nb;
+  } else {
+    q -= whole * nb;
+    pair = whole + q / nb;
+    blk = q % nb;
+  }
+}
+
 // a fragment register r of half hh holds row 8 (r >> 2) + 4 hh + (r & 3) of a 32-row product
 __device__ __forceinline__ constexpr int crow(int r, int hh) { return 8 * (r >> 2) + 4 * hh + (r & 3); }
 
@@ -162,6 +178,15 @@ struct RowTile2 {
 
 // keeps the order of what stands before and behind it: operand reads asked for early stay early
 __device__ __forceinline__ void hold_order() { __builtin_amdgcn_sched_barrier(0); }
+// N matrix instructions with R LDS reads behind each: the LDS counter holds 15 reads, a burst of more would stall the wave behind them
+template <int N, int R>
+__device__ __forceinline__ void deal_reads() {
+  if constexpr (N > 0) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    deal_reads<N - 1, R>();
+  }
+}
 
 // rows [row0, row0 + 32) of a tile as an operand, channels [16 ks, +16): lane j = row, half hh = 8 of the 16 channels
 template <typename T>

@@ -31,8 +31,9 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
   unsigned char* sK = smem;
   unsigned char* sV = smem + 64 * KS;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
-  const int id = xcd_tile_id();
-  const int rb = id % p.nrb, bg = id / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  int bg, rb;
+  pair_block(p.B * p.G, p.nrb, bg, rb);
+  const int b = bg / p.G, g = bg - b * p.G;
   const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
   const long row = static_cast<long>(rb) * 128 + wid * 32 + j;
   const int hi = static_cast<int>(row / p.Tq), i = static_cast<int>(row - static_cast<long>(hi) * p.Tq);
@@ -136,6 +137,7 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int t2 = 0; t2 < NRT; ++t2) ct[u][t2] = frag_cols<T>(sK, KS, kt * 32 + u * 16, t2, lane);
+        deal_reads<2 * NKS, 1>();
         hold_order();
         const unsigned bits = static_cast<unsigned>(cur >> (32 * kt)) >> (4 * hh);
         if (cur != ~0ull) {
@@ -153,6 +155,7 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int t2 = 0; t2 < NRT; ++t2) acc[t2] = mfma16(ct[u][t2], df[u], acc[t2]);
+        if (kt == 0) deal_reads<2 * NRT, 2>();
       }
     }
     cur = nxt;
@@ -272,9 +275,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
   float* sD = sL + NR;
   float* sM = sD + NR;                                              // 4 floats: the waves' maxima
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
-  const int id = xcd_tile_id();
-  const int sp = id % p.nsplit, kbk = (id / p.nsplit) % p.nrb;
-  const int bg = id / p.nsplit / p.nrb, b = bg / p.G, g = bg - b * p.G;
+  int bg, blk;
+  pair_block(p.B * p.G, p.nrb * p.nsplit, bg, blk);
+  const int sp = blk % p.nsplit, kbk = blk / p.nsplit, b = bg / p.G, g = bg - b * p.G;
   const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
   const int key = kbk * 128 + wid * 32 + j;
   const bool keep = key < klen && (!p.mask || p.mask[b * p.mask_bs + key] != 0);
@@ -378,6 +381,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
         };
         read_cols(0);
         if (D <= 128) read_cols(1);          // (at 160 the registers hold one of the two)
+        deal_reads<2 * NKS, 2>();
         hold_order();
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
@@ -409,6 +413,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
             ak[t2] = mfma16(qt[u][t2], df[u], ak[t2]);
           }
         }
+        if (half + 1 < NR / 32) deal_reads<4 * NRT, 1>();
       }
     }
   }
