@@ -24,7 +24,9 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
          "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("TFMQ_EXTRA_HIPCC_FLAGS", "").split()
 # Per-file additions.  VGPR-form MFMA: the softmax works on the score accumulators with VALU instructions, and with
 # the accumulators in AGPRs every key tile paid 64 v_accvgpr_read/write (a quarter of the kernel's VALU time).
-FILE_FLAGS = {"attention_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# The gradient kernels of the cross attention carry more accumulators than there are VGPRs beside their operands: in AGPR form every accumulator was
+# copied to AGPRs and back around each tile's products.
+FILE_FLAGS = {"attention_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "attention_cross_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _hipcc():

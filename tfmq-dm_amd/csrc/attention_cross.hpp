@@ -53,20 +53,14 @@ struct XattnP {
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int T) { return lens ? min(max(lens[b], 0), T) : T; }
 
-// (pair = item and key head, block of it) of this workgroup, `nb` blocks a pair: a pair's blocks stay on one XCD (they read the same K and V), and
-// neighbouring pairs go to different ones, so that items of different lengths load the XCDs evenly.  (Placement is a matter of speed only.)
-__device__ __forceinline__ void pair_block(int npair, int nb, int& pair, int& blk) {
-  int q = blockIdx.x;
-  const int whole = npair / 8 * 8;
-  if (q < whole * nb) {
-    const int t = q >> 3;
-    pair = t / nb * 8 + (q & 7);
-    blk = t % nb;
-  } else {
-    q -= whole * nb;
-    pair = whole + q / nb;
-    blk = q % nb;
-  }
+// (item, key head, block of the pair) of this workgroup, `nb` blocks a pair.  Workgroups go to the 8 XCDs in turn: with the heads running fastest a
+// head's blocks, which read the same K and V, share an XCD (or few), and an item's blocks spread over all of them, so that items of different
+// lengths load the XCDs evenly.  (Placement is a matter of speed only.)
+__device__ __forceinline__ void pair_block(int G, int nb, int& b, int& g, int& blk) {
+  const int q = blockIdx.x, r = q / G;
+  g = q - r * G;
+  b = r / nb;
+  blk = r - b * nb;
 }
 
 // a fragment register r of half hh holds row 8 (r >> 2) + 4 hh + (r & 3) of a 32-row product

@@ -31,9 +31,8 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
   unsigned char* sK = smem;
   unsigned char* sV = smem + 64 * KS;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
-  int bg, rb;
-  pair_block(p.B * p.G, p.nrb, bg, rb);
-  const int b = bg / p.G, g = bg - b * p.G;
+  int b, g, rb;
+  pair_block(p.G, p.nrb, b, g, rb);
   const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
   const long row = static_cast<long>(rb) * 128 + wid * 32 + j;
   const int hi = static_cast<int>(row / p.Tq), i = static_cast<int>(row - static_cast<long>(hi) * p.Tq);
@@ -271,13 +270,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   unsigned char* sQ = smem;
   unsigned char* sG = smem + NR * S;
-  float* sL = reinterpret_cast<float*>(smem + 2 * NR * S);          // lse (base 2) of the tile's rows, +inf: not a row
+  float* sL = reinterpret_cast<float*>(smem + 2 * NR * S);          // lse (base 2) of the tile's rows, +inf: not a row; -D of them
   float* sD = sL + NR;
   float* sM = sD + NR;                                              // 4 floats: the waves' maxima
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
-  int bg, blk;
-  pair_block(p.B * p.G, p.nrb * p.nsplit, bg, blk);
-  const int sp = blk % p.nsplit, kbk = blk / p.nsplit, b = bg / p.G, g = bg - b * p.G;
+  int b, g, blk;
+  pair_block(p.G, p.nrb * p.nsplit, b, g, blk);
+  const int sp = blk % p.nsplit, kbk = blk / p.nsplit;
   const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
   const int key = kbk * 128 + wid * 32 + j;
   const bool keep = key < klen && (!p.mask || p.mask[b * p.mask_bs + key] != 0);
@@ -341,6 +340,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
     }
   };
   const float c2 = p.scale * LOG2E;
+  v16f bias;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) bias[r] = keep ? 0.0f : -INFINITY;
   v16f ak[NRT], av[NRT];
 #pragma unroll
   for (int t = 0; t < NRT; ++t) ak[t] = zero16(), av[t] = zero16();
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
     tile.store(sQ, sG);
-    if (tid < NR) sL[tid] = rl - PSHIFT, sD[tid] = rd;
+    if (tid < NR) sL[tid] = rl - PSHIFT, sD[tid] = -rd;
     __syncthreads();
     if (t + 1 < t1) fetch();
     if (work) {
@@ -365,7 +367,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
 #pragma unroll
       for (int half = 0; half < NR / 32; ++half) {
         hold_order();
-        v16f s = zero16(), dp = zero16();
+        v16f s = bias, dp = start_scores(sD + half * 32, hh);          // (-inf for a dropped key; dp - D)
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
           s = mfma16(qr[ks], kf[ks], s);
@@ -386,14 +388,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
           const float4 L = *reinterpret_cast<const float4*>(sL + half * 32 + 8 * a + 4 * hh);
-          const float4 dd = *reinterpret_cast<const float4*>(sD + half * 32 + 8 * a + 4 * hh);
-          const float lv[4] = {L.x, L.y, L.z, L.w}, dv[4] = {dd.x, dd.y, dd.z, dd.w};
+          const float lv[4] = {L.x, L.y, L.z, L.w};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int r = 4 * a + c;
-            const float pr = keep ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lv[c])) : 0.0f;
+            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lv[c]));
             s[r] = pr;
-            dp[r] = is_f16<T>() ? pr * (dp[r] - dv[c]) * ff : pr * (dp[r] - dv[c]);
+            dp[r] = is_f16<T>() ? pr * dp[r] * ff : pr * dp[r];
           }
         }
         V8 pf[2], df[2];

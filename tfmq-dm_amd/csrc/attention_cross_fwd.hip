@@ -20,9 +20,9 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
   unsigned char* sK = smem;
   unsigned char* sV = smem + 64 * KS;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, j = lane & 31, hh = lane >> 5;
-  int bg, blk;
-  pair_block(p.B * p.G, p.nrb * p.nsplit, bg, blk);
-  const int sp = blk % p.nsplit, rb = blk / p.nsplit, b = bg / p.G, g = bg - b * p.G;
+  int b, g, blk;
+  pair_block(p.G, p.nrb * p.nsplit, b, g, blk);
+  const int sp = blk % p.nsplit, rb = blk / p.nsplit;
   const int qlen = clamp_len(p.q_lens, b, p.Tq), klen = clamp_len(p.kv_lens, b, p.Tk);
 
   const long row = static_cast<long>(rb) * 128 + wid * 32 + j;
