@@ -288,6 +288,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
   const int t0 = sp * per;
   int t1 = min(nt, t0 + per);
   if (kbk * 128 >= klen || qlen == 0) t1 = t0;          // nothing to sum: zeros are written below
+  if (p.nsplit > 1 && kbk * 128 >= klen) return;          // (k_xattn_sum knows)
 
   V8 kf[NKS], vf[NKS];
   {
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
       }
     }
   }
-  if (key >= p.Tk) return;
+  if (key >= (p.nsplit > 1 ? klen : p.Tk)) return;
   const float fk = p.scale * unf, fv = is_f16<T>() ? 1.0f / 4096.0f : 1.0f;
   const long krow = (static_cast<long>(b) * p.Tk + key) * p.G + g;
   if (p.nsplit > 1) {
@@ -446,7 +447,10 @@ __global__ __launch_bounds__(256) void k_xattn_sum(XattnP p, long n) {
   float a[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) a[e] = 0.0f;
-  for (int s = 0; s < p.nsplit; ++s) {
+  const long key = (i < n ? i : i - n) / (static_cast<long>(p.G) * p.d);          // of [B][Tk]
+  const int b = static_cast<int>(key / p.Tk);
+  const int slices = key - static_cast<long>(b) * p.Tk < clamp_len(p.kv_lens, b, p.Tk) ? p.nsplit : 0;          // (nothing was written behind the length)
+  for (int s = 0; s < slices; ++s) {
     const float4* q = reinterpret_cast<const float4*>(p.part + 2 * s * n + i);
     const float4 x = q[0], y = q[1];
     a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w; a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;

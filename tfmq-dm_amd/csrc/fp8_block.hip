@@ -43,29 +43,51 @@ __device__ __forceinline__ unsigned pack4_f8(float a, float b, float c, float d)
   return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
 
-// 8 consecutive elements of a row from column c (zeros from column K on)
+// 8 consecutive elements of a row from column c (zeros from column K on).  Inside the row they are one 16-byte load (fp32: two) at any alignment of
+// the elements; VEC: rows are 16-byte aligned and K % 8 == 0, so that a group is inside or outside as a whole.
+struct Raw8 {
+  uint4 a, b;          // 16-bit types: a
+};
+template <int ES, bool VEC>
+__device__ __forceinline__ Raw8 raw8(const char* row, int c, int K) {
+  Raw8 r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  const char* p = row + static_cast<long>(c) * ES;
+  if (VEC ? c < K : c + 8 <= K) {
+    __builtin_memcpy(&r.a, p, 16);
+    if (ES == 4) __builtin_memcpy(&r.b, p + 16, 16);
+  } else if (!VEC && c < K) {
+    unsigned w[8] = {};
+    unsigned short h[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < K) {
+        if (ES == 4) __builtin_memcpy(&w[i], p + i * 4, 4);
+        else __builtin_memcpy(&h[i], p + i * 2, 2);
+      }
+    if (ES == 4) {
+      r.a = make_uint4(w[0], w[1], w[2], w[3]);
+      r.b = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+      r.a = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
+  }
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void widen8(const Raw8& r, float (&v)[8]) {
+  if constexpr (DT == DT_F32) {
+    v[0] = __uint_as_float(r.a.x); v[1] = __uint_as_float(r.a.y); v[2] = __uint_as_float(r.a.z); v[3] = __uint_as_float(r.a.w);
+    v[4] = __uint_as_float(r.b.x); v[5] = __uint_as_float(r.b.y); v[6] = __uint_as_float(r.b.z); v[7] = __uint_as_float(r.b.w);
+  } else {
+    typedef typename Elem<DT>::type v8t __attribute__((ext_vector_type(8)));
+    const v8t t = __builtin_bit_cast(v8t, r.a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(t[i]);
+  }
+}
 template <int DT, bool VEC>
 __device__ __forceinline__ void load8(const typename Elem<DT>::type* row, int c, int K, float (&v)[8]) {
-  using T = typename Elem<DT>::type;
-  if (VEC) {          // row 16-byte aligned, K % 8 == 0
-    if (c < K) {
-      if constexpr (DT == DT_F32) {
-        const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      } else {
-        typedef T v8t __attribute__((ext_vector_type(8)));
-        const v8t a = *reinterpret_cast<const v8t*>(row + c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(a[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? static_cast<float>(row[c + i]) : 0.0f;
-  }
+  widen8<DT>(raw8<DT == DT_F32 ? 4 : 2, VEC>(reinterpret_cast<const char*>(row), c, K), v);
 }
 
 // ---- rows: q [M][Kp], s [Kb][M].  16 lanes hold one block of one row (8 values each); a workgroup takes 16 rows of one block column, so the
@@ -106,40 +128,37 @@ struct QuantTileP {
   uint8_t *q, *qc;
   float *s, *sc;               // q, s null: columns only
 };
-__device__ __forceinline__ void load8_any(const QuantTileP& p, long row, int c, float (&v)[8]) {
-  if (p.dt == DT_F32) {
-    const float* x = static_cast<const float*>(p.x) + row;
-    p.vec ? load8<DT_F32, true>(x, c, p.K, v) : load8<DT_F32, false>(x, c, p.K, v);
-  } else if (p.dt == DT_F16) {
-    const _Float16* x = static_cast<const _Float16*>(p.x) + row;
-    p.vec ? load8<DT_F16, true>(x, c, p.K, v) : load8<DT_F16, false>(x, c, p.K, v);
-  } else {
-    const __bf16* x = static_cast<const __bf16*>(p.x) + row;
-    p.vec ? load8<DT_BF16, true>(x, c, p.K, v) : load8<DT_BF16, false>(x, c, p.K, v);
+// the thread's 8 rows of 8: all loads before the first conversion
+template <int ES, bool VEC>
+__device__ __forceinline__ void tile_raw(const QuantTileP& p, long m0, int k, Raw8 (&r)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r[i] = Raw8{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (m0 + i < p.M) r[i] = raw8<ES, VEC>(static_cast<const char*>(p.x) + (m0 + i) * p.ld * ES, k, p.K);
   }
 }
-__device__ __forceinline__ void quant_tile(const QuantTileP& p, int t) {
-  __shared__ unsigned amax[16][128];
-  __shared__ __attribute__((aligned(16))) unsigned bytes[128][33];
+template <int DT>
+__device__ __forceinline__ void quant_tile_of(const QuantTileP& p, int t) {
+  constexpr int ES = DT == DT_F32 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) unsigned amax[16][128];
+  __shared__ __attribute__((aligned(16))) unsigned bytes[128][36];
   const long mb = t / p.Kb, Mp = (p.M + 127) / 128 * 128;
   const int kb = t % p.Kb;
   const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, k = kb * 128 + cg * 8;
   const long m0 = mb * 128 + rg * 8;
+  Raw8 raw[8];
+  if (p.vec) tile_raw<ES, true>(p, m0, k, raw);
+  else tile_raw<ES, false>(p, m0, k, raw);
   float v[8][8];
   unsigned cm[8] = {};
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    if (m0 + r < p.M) {
-      load8_any(p, (m0 + r) * p.ld, k, v[r]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[r][e] = 0.0f;
-    }
+    widen8<DT>(raw[r], v[r]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) cm[e] = max(cm[e], mag_bits(v[r][e]));
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) amax[rg][cg * 8 + e] = cm[e];
+  *reinterpret_cast<uint4*>(&amax[rg][cg * 8]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+  *reinterpret_cast<uint4*>(&amax[rg][cg * 8 + 4]) = make_uint4(cm[4], cm[5], cm[6], cm[7]);
   if (p.q) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
@@ -160,21 +179,29 @@ __device__ __forceinline__ void quant_tile(const QuantTileP& p, int t) {
   }
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    unsigned a = 0;
+  for (int g = 0; g < 16; ++g) {
+    const uint4 x = *reinterpret_cast<const uint4*>(&amax[g][cg * 8]), y = *reinterpret_cast<const uint4*>(&amax[g][cg * 8 + 4]);
+    cm[0] = max(cm[0], x.x); cm[1] = max(cm[1], x.y); cm[2] = max(cm[2], x.z); cm[3] = max(cm[3], x.w);
+    cm[4] = max(cm[4], y.x); cm[5] = max(cm[5], y.y); cm[6] = max(cm[6], y.z); cm[7] = max(cm[7], y.w);
+  }
 #pragma unroll
-    for (int g = 0; g < 16; ++g) a = max(a, amax[g][cg * 8 + e]);
-    const float2 sc = block_scale(a);
+  for (int e = 0; e < 8; ++e) {
+    const float2 sc = block_scale(cm[e]);
     if (rg == 0 && k + e < p.K) p.sc[mb * p.K + k + e] = sc.y;
     bytes[cg * 8 + e][rg * 2] = pack4_f8(v[0][e] * sc.x, v[1][e] * sc.x, v[2][e] * sc.x, v[3][e] * sc.x);
     bytes[cg * 8 + e][rg * 2 + 1] = pack4_f8(v[4][e] * sc.x, v[5][e] * sc.x, v[6][e] * sc.x, v[7][e] * sc.x);
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int idx = threadIdx.x + i * 256, row = idx >> 5, w = idx & 31;
-    if (kb * 128 + row < p.K) *reinterpret_cast<unsigned*>(p.qc + static_cast<long>(kb * 128 + row) * Mp + mb * 128 + w * 4) = bytes[row][w];
+  for (int i = 0; i < 4; ++i) {
+    const int idx = threadIdx.x + i * 256, row = idx >> 3, w = (idx & 7) * 4;
+    if (kb * 128 + row < p.K) *reinterpret_cast<uint4*>(p.qc + static_cast<long>(kb * 128 + row) * Mp + mb * 128 + w * 4) = *reinterpret_cast<const uint4*>(&bytes[row][w]);
   }
+}
+__device__ __forceinline__ void quant_tile(const QuantTileP& p, int t) {
+  if (p.dt == DT_F32) quant_tile_of<DT_F32>(p, t);
+  else if (p.dt == DT_F16) quant_tile_of<DT_F16>(p, t);
+  else quant_tile_of<DT_BF16>(p, t);
 }
 // one launch for up to two tensors (n0 tiles of the first)
 __global__ __launch_bounds__(256) void k_quant_cols(QuantTileP a, QuantTileP b, int n0) {
@@ -289,10 +316,9 @@ __device__ __forceinline__ void store_run(typename Elem<YDT>::type* p, const flo
 // Operand tiles of one block (128 bytes a row) travel by LDS-DMA into two stages, the next one in flight while this one is multiplied.  A workgroup
 // walks over its tiles (or, sliced, one K range of a tile) as one sequence of blocks: the next tile's first stage is under way while the results of
 // this one are rounded and stored.
-template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), WPS) void k_gemm_f8(GemmF8P p) {
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW>
+__device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, int bid, int nblocks, int first) {
   constexpr int NWM = BM / WM, NWN = BN / WN, NW = NWM * NWN, TM = WM / 32, TN = WN / 32;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int STAGE = (BM + BN) * 128;
   using YT = typename Elem<YDT>::type;
   using F = Frag<YDT == DT_F32>;
@@ -335,10 +361,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), WPS) void k_gemm_f8(Gem
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff[i]), "s"(base), "s"(dst + i * 1024) : "memory", "m0");
   };
   // this workgroup's slice of the blocks, and its tiles
-  const int sl = p.nslice > 1 ? static_cast<int>(blockIdx.x) % p.nslice : 0;
+  const int sl = p.nslice > 1 ? bid % p.nslice : 0;
   const int per = (p.Kb + p.nslice - 1) / p.nslice, k_lo = sl * per, k_hi = min(p.Kb, k_lo + per);
-  int tile = p.nslice > 1 ? static_cast<int>(blockIdx.x) / p.nslice : xcd_tile_id();
-  const int stride = p.nslice > 1 ? ntile : static_cast<int>(gridDim.x);
+  int tile = p.nslice > 1 ? bid / p.nslice : first;
+  const int stride = p.nslice > 1 ? ntile : nblocks;
   if (tile >= ntile) return;
   const int nb_last = (p.N - 1) >> 7;
   static_assert(!SBROW || WN == 64, "a lane per column");
@@ -494,6 +520,20 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), WPS) void k_gemm_f8(Gem
     }
     stores = full;
   }
+}
+
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), WPS) void k_gemm_f8(GemmF8P p) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  gemm_f8<BM, BN, WM, WN, YDT, SBROW>(p, smem, blockIdx.x, gridDim.x, xcd_tile_id());
+}
+// a weight gradient's slices (the longer workgroups, first) and the other gradient's tiles in one launch: either alone leaves CUs idle
+template <int YDT>
+__global__ __launch_bounds__(256, 2) void k_gemm_f8_grads(GemmF8P gw, GemmF8P gx, int nw) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int q = blockIdx.x;
+  if (q < nw) gemm_f8<128, 128, 64, 64, DT_F32, true>(gw, smem, q, nw, q);
+  else gemm_f8<128, 128, 64, 64, YDT, false>(gx, smem, q - nw, gridDim.x - nw, q - nw);
 }
 
 // slices of the K axis, added in order; four outputs a thread
@@ -668,6 +708,21 @@ int launch_small(tfmq_handle h, const SmallF8P& p, int dtype, int y_dtype, hipSt
   });
 }
 
+template <int YDT>
+int launch_grads(tfmq_handle h, GemmF8P gw, GemmF8P gx, hipStream_t st) {
+  constexpr int smem = 2 * 256 * 128 + 4 * 64 * 4;
+  auto kern = &k_gemm_f8_grads<YDT>;
+  static LdsRoom room;
+  TFMQ_HIP(h, room.ask(h, reinterpret_cast<const void*>(kern), smem));
+  gw.tm = ceil_div(gw.M, 128), gw.tn = ceil_div(gw.N, 128);
+  gx.tm = ceil_div(gx.M, 128), gx.tn = ceil_div(gx.N, 128);
+  const long nw = static_cast<long>(gw.tm) * gw.tn * gw.nslice, nx = static_cast<long>(gx.tm) * gx.tn;
+  TFMQ_CHECK_ARG(h, (nw + nx) * 8 < (1L << 31), "linear_fp8_bwd: too many tiles");
+  hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nw + nx)), dim3(256), smem, st, gw, gx, static_cast<int>(nw));
+  TFMQ_LAUNCH_CHECK(h);
+  return TFMQ_OK;
+}
+
 // ---- which kernel multiplies.  Tiles of 256 x 256 where they fill the card in whole rounds (at least three quarters of the last one), else 128 x 128.
 bool big_tiles(tfmq_handle h, long M, int N) {
   const long nt = static_cast<long>(ceil_div(M, 256)) * ceil_div(N, 256), cu = h->cu_count;
@@ -806,15 +861,21 @@ extern "C" int tfmq_linear_fp8_bwd(tfmq_handle h, const void* x, int x_dtype, lo
     rc = launch_quant_rows(h, gy, gy_dtype, M, N, gy_ld, b.gq, b.gs, st);
   }
   if (rc != TFMQ_OK) return rc;
-  if (gx) {          // the weight's blocks seen from its columns: scale (n block, k block) at ws[n block][k block]
-    rc = b.gq ? launch_product(h, GemmF8P{b.gq, wt, b.gs, ws, 1, Kb, nullptr, gx, M, K, Nb, 0, 0, 1}, gy_dtype, st)
-              : launch_small(h, SmallF8P{gy, gy_ld, static_cast<int>(M), N, wt, ws, 1, Kb, nullptr, gx, K, Nb}, gy_dtype, gy_dtype, st);
-    if (rc != TFMQ_OK) return rc;
+  // the weight's blocks seen from its columns: scale (n block, k block) at ws[n block][k block]
+  const GemmF8P px{b.gq, wt, b.gs, ws, 1, Kb, nullptr, gx, M, K, Nb, 0, 0, 1};
+  const int Mb = static_cast<int>((M + 127) / 128);
+  const GemmF8P pw{b.gc, b.xc, b.gcs, b.xcs, 0, 0, nullptr, gw ? (b.part ? b.part : gw) : nullptr, N, K, Mb, 0, 0, gw ? b.slices : 1};
+  if (gx && gw && !big_tiles(h, M, K)) {
+    if (gy_dtype == DT_F32) rc = launch_grads<DT_F32>(h, pw, px, st);
+    else rc = gy_dtype == DT_F16 ? launch_grads<DT_F16>(h, pw, px, st) : launch_grads<DT_BF16>(h, pw, px, st);
+  } else {
+    if (gx)
+      rc = b.gq ? launch_product(h, px, gy_dtype, st)
+                : launch_small(h, SmallF8P{gy, gy_ld, static_cast<int>(M), N, wt, ws, 1, Kb, nullptr, gx, K, Nb}, gy_dtype, gy_dtype, st);
+    if (rc == TFMQ_OK && gw) rc = launch_gemm<128, 128, 64, 64, DT_F32, true, 2>(h, pw, st);
   }
-  if (gw) {
-    const int Mb = static_cast<int>((M + 127) / 128);
-    rc = launch_gemm<128, 128, 64, 64, DT_F32, true, 2>(h, GemmF8P{b.gc, b.xc, b.gcs, b.xcs, 0, 0, nullptr, b.part ? b.part : gw, N, K, Mb, 0, 0, b.slices}, st);
-    if (rc != TFMQ_OK || !b.part) return rc;
+  if (rc != TFMQ_OK) return rc;
+  if (gw && b.part) {
     const long n = static_cast<long>(N) * K;
     hipLaunchKernelGGL(k_sum_slices, dim3(static_cast<unsigned>((n + 1023) / 1024)), dim3(256), 0, st, b.part, gw, n, b.slices);
     TFMQ_LAUNCH_CHECK(h);
