@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void k_quant_rows(const typename Elem<DT>::typ
 
 // ---- columns: x [M][K] -> qc [K][Mp] with one scale per column and block of 128 rows, sc [Mb][K]; the row form (q, s as above) from the same
 // values where it is wanted too, so that an upstream gradient, which both products read, is read once.  A workgroup takes 128 rows x 128 columns, a
-// thread 8 x 8 of them; the columns' maxima meet in LDS, the bytes are transposed through LDS and leave as 128-byte rows.  HBM-bound.
+// thread 4 x 8 of them; the columns' maxima meet in LDS, the bytes are transposed through LDS and leave as 128-byte rows.  HBM-bound.
 struct QuantTileP {
   const void* x;
   int dt, vec;                 // type code; rows 16-byte aligned and K % 8 == 0
@@ -128,40 +128,50 @@ struct QuantTileP {
   uint8_t *q, *qc;
   float *s, *sc;               // q, s null: columns only
 };
-// the thread's 8 rows of 8: all loads before the first conversion
+// the thread's 4 rows of 8: all loads before the first conversion
 template <int ES, bool VEC>
-__device__ __forceinline__ void tile_raw(const QuantTileP& p, long m0, int k, Raw8 (&r)[8]) {
+__device__ __forceinline__ void tile_raw(const QuantTileP& p, long m0, int k, Raw8 (&r)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     r[i] = Raw8{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     if (m0 + i < p.M) r[i] = raw8<ES, VEC>(static_cast<const char*>(p.x) + (m0 + i) * p.ld * ES, k, p.K);
   }
 }
+struct QuantLds {
+  unsigned amax[8][128];          // per wave and column
+  float scale[128];               // reciprocals
+  unsigned bytes[128][36];        // 16-byte pieces of a column's 128 bytes at piece ^ (column >> 4): the writes, four bytes of 16 columns 8 apart, spread over the banks
+};
 template <int DT>
-__device__ __forceinline__ void quant_tile_of(const QuantTileP& p, int t) {
+__device__ __forceinline__ void quant_tile_of(const QuantTileP& p, int t, QuantLds& L) {
   constexpr int ES = DT == DT_F32 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) unsigned amax[16][128];
-  __shared__ __attribute__((aligned(16))) unsigned bytes[128][36];
   const long mb = t / p.Kb, Mp = (p.M + 127) / 128 * 128;
   const int kb = t % p.Kb;
   const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, k = kb * 128 + cg * 8;
-  const long m0 = mb * 128 + rg * 8;
-  Raw8 raw[8];
+  const long m0 = mb * 128 + rg * 4;
+  Raw8 raw[4];
   if (p.vec) tile_raw<ES, true>(p, m0, k, raw);
   else tile_raw<ES, false>(p, m0, k, raw);
-  float v[8][8];
+  float v[4][8];
   unsigned cm[8] = {};
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
+  for (int r = 0; r < 4; ++r) {
     widen8<DT>(raw[r], v[r]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) cm[e] = max(cm[e], mag_bits(v[r][e]));
   }
-  *reinterpret_cast<uint4*>(&amax[rg][cg * 8]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
-  *reinterpret_cast<uint4*>(&amax[rg][cg * 8 + 4]) = make_uint4(cm[4], cm[5], cm[6], cm[7]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cm[e] = max(cm[e], static_cast<unsigned>(__shfl_xor(static_cast<int>(cm[e]), 16, 64)));
+    cm[e] = max(cm[e], static_cast<unsigned>(__shfl_xor(static_cast<int>(cm[e]), 32, 64)));
+  }
+  if ((threadIdx.x & 63) < 16) {
+    *reinterpret_cast<uint4*>(&L.amax[threadIdx.x >> 6][cg * 8]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+    *reinterpret_cast<uint4*>(&L.amax[threadIdx.x >> 6][cg * 8 + 4]) = make_uint4(cm[4], cm[5], cm[6], cm[7]);
+  }
   if (p.q) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < 4; ++r) {
       unsigned a = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) a = max(a, mag_bits(v[r][e]));
@@ -178,35 +188,38 @@ __device__ __forceinline__ void quant_tile_of(const QuantTileP& p, int t) {
     }
   }
   __syncthreads();
+  if (threadIdx.x < 128) {
+    unsigned a = 0;
 #pragma unroll
-  for (int g = 0; g < 16; ++g) {
-    const uint4 x = *reinterpret_cast<const uint4*>(&amax[g][cg * 8]), y = *reinterpret_cast<const uint4*>(&amax[g][cg * 8 + 4]);
-    cm[0] = max(cm[0], x.x); cm[1] = max(cm[1], x.y); cm[2] = max(cm[2], x.z); cm[3] = max(cm[3], x.w);
-    cm[4] = max(cm[4], y.x); cm[5] = max(cm[5], y.y); cm[6] = max(cm[6], y.z); cm[7] = max(cm[7], y.w);
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float2 sc = block_scale(cm[e]);
-    if (rg == 0 && k + e < p.K) p.sc[mb * p.K + k + e] = sc.y;
-    bytes[cg * 8 + e][rg * 2] = pack4_f8(v[0][e] * sc.x, v[1][e] * sc.x, v[2][e] * sc.x, v[3][e] * sc.x);
-    bytes[cg * 8 + e][rg * 2 + 1] = pack4_f8(v[4][e] * sc.x, v[5][e] * sc.x, v[6][e] * sc.x, v[7][e] * sc.x);
+    for (int w = 0; w < 8; ++w) a = max(a, L.amax[w][threadIdx.x]);
+    const float2 sc = block_scale(a);
+    L.scale[threadIdx.x] = sc.x;
+    if (kb * 128 + static_cast<int>(threadIdx.x) < p.K) p.sc[mb * p.K + kb * 128 + threadIdx.x] = sc.y;
   }
   __syncthreads();
+  const float4 s0 = *reinterpret_cast<const float4*>(&L.scale[cg * 8]), s1 = *reinterpret_cast<const float4*>(&L.scale[cg * 8 + 4]);
+  const float sr[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int idx = threadIdx.x + i * 256, row = idx >> 3, w = (idx & 7) * 4;
-    if (kb * 128 + row < p.K) *reinterpret_cast<uint4*>(p.qc + static_cast<long>(kb * 128 + row) * Mp + mb * 128 + w * 4) = *reinterpret_cast<const uint4*>(&bytes[row][w]);
+  for (int e = 0; e < 8; ++e) L.bytes[cg * 8 + e][rg ^ ((cg >> 1) << 2)] = pack4_f8(v[0][e] * sr[e], v[1][e] * sr[e], v[2][e] * sr[e], v[3][e] * sr[e]);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int idx = threadIdx.x + i * 512, row = idx >> 3, pc = idx & 7;
+    if (kb * 128 + row < p.K)
+      *reinterpret_cast<uint4*>(p.qc + static_cast<long>(kb * 128 + row) * Mp + mb * 128 + pc * 16) = *reinterpret_cast<const uint4*>(&L.bytes[row][(pc ^ (row >> 4)) * 4]);
   }
 }
-__device__ __forceinline__ void quant_tile(const QuantTileP& p, int t) {
-  if (p.dt == DT_F32) quant_tile_of<DT_F32>(p, t);
-  else if (p.dt == DT_F16) quant_tile_of<DT_F16>(p, t);
-  else quant_tile_of<DT_BF16>(p, t);
-}
 // one launch for up to two tensors (n0 tiles of the first)
-__global__ __launch_bounds__(256) void k_quant_cols(QuantTileP a, QuantTileP b, int n0) {
-  const int t = blockIdx.x;
-  quant_tile(t < n0 ? a : b, t < n0 ? t : t - n0);
+struct QuantPairP {
+  QuantTileP t[2];
+};
+__global__ __launch_bounds__(512) void k_quant_cols(QuantPairP pr, int n0) {
+  __shared__ __attribute__((aligned(16))) QuantLds L;
+  const int second = static_cast<int>(blockIdx.x) >= n0, t = blockIdx.x - (second ? n0 : 0);
+  const QuantTileP& p = pr.t[second];
+  if (p.dt == DT_F32) quant_tile_of<DT_F32>(p, t, L);
+  else if (p.dt == DT_F16) quant_tile_of<DT_F16>(p, t, L);
+  else quant_tile_of<DT_BF16>(p, t, L);
 }
 
 // ---- weights: w fp32 [N][K] -> q [N][Kp] and its transpose qt [K][Np], s [Nb][Kb]; one workgroup per 128 x 128 block, run once per layer
@@ -592,7 +605,7 @@ int launch_quant_cols(tfmq_handle h, const QuantTileP& a, const QuantTileP* b, h
   auto tiles = [](const QuantTileP& p) { return (p.M + 127) / 128 * p.Kb; };
   const long na = tiles(a), n = na + (b ? tiles(*b) : 0);
   TFMQ_CHECK_ARG(h, n < (1L << 31), "quantize_fp8: too many blocks");
-  hipLaunchKernelGGL(k_quant_cols, dim3(static_cast<unsigned>(n)), dim3(256), 0, st, a, b ? *b : a, static_cast<int>(na));
+  hipLaunchKernelGGL(k_quant_cols, dim3(static_cast<unsigned>(n)), dim3(512), 0, st, QuantPairP{{a, b ? *b : a}}, static_cast<int>(na));
   TFMQ_LAUNCH_CHECK(h);
   return TFMQ_OK;
 }
