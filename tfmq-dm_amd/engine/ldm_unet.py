@@ -260,7 +260,16 @@ class LdmUNetEngine(DdimUNetEngine):
         d = Cc // heads
         Bc, Lp, Dc = cpad.shape
         fkv = self.fused_kv.get(p)
-        if fkv is not None and fkv.kind == "w4a8" and Cc % 128 == 0 and os.environ.get("TFMQ_FUSED_KV", "1") != "0":
+        fused = fkv is not None and fkv.kind == "w4a8" and Cc % 128 == 0 and os.environ.get("TFMQ_FUSED_KV", "1") != "0"
+        if self._ctx_mask is not None:      # the masked attention reads k and v as token rows
+            def rows(l):
+                return ops.conv2d_w4a8(ops.quantize_act(cpad, l.aq).reshape(Bc, Lp, 1, Dc), l.p, l.aq, out_f16=True).reshape(Bc, Lp, -1)
+            if fused:
+                kv = rows(fkv)
+                k16, v16 = kv[..., :Cc], kv[..., Cc:]
+            else:
+                k16, v16 = rows(lk), rows(lv)
+        elif fused:
             # to_k and to_v quantise the same context with quantizers that agree at every step (prepare()): one quantise pass and
             # one GEMM write k as fp16 rows and v as its fp16 transpose (the transposed region starts at a multiple of 128 channels)
             kv, vt = ops.conv2d_w4a8(ops.quantize_act(cpad, fkv.aq).reshape(Bc, Lp, 1, Dc), fkv.p, fkv.aq, out_f16=True, t_col0=Cc)
@@ -269,7 +278,10 @@ class LdmUNetEngine(DdimUNetEngine):
             k16 = ops.conv2d_w4a8(ops.quantize_act(cpad, lk.aq).reshape(Bc, Lp, 1, Dc), lk.p, lk.aq, out_f16=True).reshape(Bc, Lp, Cc)
             _, vt = ops.conv2d_w4a8(ops.quantize_act(cpad, lv.aq).reshape(Bc, Lp, 1, Dc), lv.p, lv.aq, out_f16=True, t_col0=0)
         aq = to_out.aq if to_out.kind == "w4a8" else None
-        if aq is not None:
+        if self._ctx_mask is not None:
+            o = ops.cross_attention(q16, k16[:, :n_ctx], v16[:, :n_ctx], heads, float(d ** -0.5), mask=self._ctx_mask)
+            o = ops.quantize_act(o, aq) if aq is not None else o.float()
+        elif aq is not None:
             _, o = ops.attention_f16(q16, k16, vt, heads, float(d ** -0.5), aq, want_f32=False, n_keys=n_ctx)
         else:
             o, _ = ops.attention_f16(q16, k16, vt, heads, float(d ** -0.5), n_keys=n_ctx)
@@ -279,6 +291,9 @@ class LdmUNetEngine(DdimUNetEngine):
 
     def _attention_rest(self, p, xq_src, ctx, x_res, self_attn: bool):
         """_attention's generic forms (fp32 operands, calibration observation, exact / quantised attention)."""
+        if not self_attn and self._ctx_mask is not None:
+            raise TfmqError(f"LdmUNetEngine: {p} cannot take context_mask: it needs 4-bit to_q / to_k / to_v with 8-bit activations on the fp16-operand "
+                            "attention (no calibration, exact-fp mode or live attention quantizers)")
         L = self.layers
         heads = self.cfg["num_heads"]
         to_out = L[p + ".to_out.0"]
@@ -373,7 +388,7 @@ class LdmUNetEngine(DdimUNetEngine):
         _, o = ops.attention_f16(y16[..., :Cc], y16[..., Cc:2 * Cc], vt, heads, float((Cc // heads) ** -0.5), to_out.aq, want_f32=False)
         pend = self._pair_half
         lq = L[p + ".attn2.to_q"]
-        single = ctx is not None and ctx.shape[1] == 1 and os.environ.get("TFMQ_SINGLE_CTX_TOKEN", "1") != "0"
+        single = ctx is not None and ctx.shape[1] == 1 and self._ctx_mask is None and os.environ.get("TFMQ_SINGLE_CTX_TOKEN", "1") != "0"
         if (not single) and self._cross_ok(p + ".attn2") and lq.p.cout == Cc:
             mid = ops.row_chain(o.reshape(B * T, Cc), T, [dict(pw=to_out.p, aq=to_out.aq, residual=h.reshape(B * T, Cc), ln=True), dict(pw=lq.p, aq=lq.aq)],
                                 ln=(self.sd[p + ".norm2.weight"], self.sd[p + ".norm2.bias"], 1e-5))
@@ -420,7 +435,7 @@ class LdmUNetEngine(DdimUNetEngine):
         # pair_prefix: everything up to here saw only (x, t) -- identical for the two members of a guidance pair -- and ran once per
         # pair; the first cross attention is where the members part (norm2 / to_q's quantizer still see the shared tensor)
         pend = self._pair_half
-        if (ctx is not None and ctx.shape[1] == 1 and self.calib is None and x.shape[-1] % 8 == 0 and not self.exact_fp and (p + ".attn2") not in self.attn_q
+        if (ctx is not None and ctx.shape[1] == 1 and self._ctx_mask is None and self.calib is None and x.shape[-1] % 8 == 0 and not self.exact_fp and (p + ".attn2") not in self.attn_q
                 and os.environ.get("TFMQ_SINGLE_CTX_TOKEN", "1") != "0"):
             if pend:
                 x, self._pair_half = self._dup(x), False
@@ -637,8 +652,12 @@ class LdmUNetEngine(DdimUNetEngine):
             return None
 
     def _forward(self, x: torch.Tensor, t: Optional[torch.Tensor] = None, context: Optional[torch.Tensor] = None,
-                taps: Optional[dict] = None, pair_prefix: bool = False) -> torch.Tensor:
+                taps: Optional[dict] = None, pair_prefix: bool = False, context_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x: fp32 NHWC latents [B,H,W,C]; t: [B] timesteps (or None -> per-step TIB table); context: fp32 [B,L,D].
+
+        context_mask: bool, one row per context row and one column per token, True: attend (CrossAttention.forward's `mask`,
+        ldm/modules/attention.py:168-194) -- prompts of different lengths in one batch.  An item that attends to nothing gets zeros from its
+        cross attentions (the reference's masked_fill with the lowest value would average all tokens).
 
         pair_prefix (classifier-free guidance, ldm/models/diffusion/ddim.py:180-186: x_in = cat([x] * 2), t_in = cat([t] * 2),
         c_in = cat([uc, c])): `x` holds the B latents ONCE, `context` the 2B rows cat(uc, c); returns eps of the 2B-item batch.
@@ -676,6 +695,13 @@ class LdmUNetEngine(DdimUNetEngine):
                             rowadd_step_stride=self.tib_table.shape[1])
         ctx = None if context is None else context.contiguous()
         self._ctx_pad = None
+        self._ctx_mask = None
+        if context_mask is not None:
+            if ctx is None or context_mask.dtype != torch.bool or tuple(context_mask.shape) != tuple(ctx.shape[:2]) or context_mask.device != ctx.device:
+                raise TfmqError("LdmUNetEngine: context_mask must be bool, one row per context row and one column per token, on the context's device")
+            if self.calib is not None or taps is not None or self.exact_fp:
+                raise TfmqError("LdmUNetEngine: context_mask is not available in calibration, with taps or in the exact-fp mode")
+            self._ctx_mask = context_mask.contiguous()
         if ctx is not None and self.calib is None:
             Bc, Lc, Dc = ctx.shape
             Lp = (Lc + 7) // 8 * 8
