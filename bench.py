@@ -26,6 +26,7 @@ The JSON line also carries
 import argparse
 import json
 import os
+import subprocess
 import sys
 import time
 
@@ -856,7 +857,7 @@ def main():
     if not torch.cuda.is_available():
         raise SystemExit("bench.py needs an MI355X: the TFMQ hot path has no CPU fallback")
     if args.gpus > 1 and "WORLD_SIZE" not in os.environ:
-        # `python bench.py --gpus N` on its own: become N ranks (one process per GPU) under torch.distributed.run,
+        # `python bench.py --gpus N` on its own: start N ranks (one process per GPU) under torch.distributed.run,
         # exactly the command the driver uses
         if torch.cuda.device_count() < args.gpus and not ONE_DEVICE:
             raise SystemExit(f"bench.py --gpus {args.gpus}: this node has {torch.cuda.device_count()} GPU(s)")
@@ -864,8 +865,9 @@ def main():
         with socket.socket() as sk:
             sk.bind(("127.0.0.1", 0))
             port = sk.getsockname()[1]
-        os.execv(sys.executable, [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={args.gpus}",
-                                  "--master-addr", "127.0.0.1", "--master-port", str(port), os.path.abspath(__file__)] + sys.argv[1:])
+        # (a child process: this one has opened the GPU above and must not be replaced by another program)
+        raise SystemExit(subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={args.gpus}",
+                                         "--master-addr", "127.0.0.1", "--master-port", str(port), os.path.abspath(__file__)] + sys.argv[1:]).returncode)
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))
