@@ -70,6 +70,7 @@ class LdmUNetEngine(DdimUNetEngine):
         super().__init__(sd2, dict(cfg), device)
         self.res_names = ldm_resblock_paths(self.sd)
         self._ctx_pad = None
+        self._ctx_mask = None       # context_mask of the forward that runs
         self._pair_half = False
         self.fuse_q8 = os.environ.get("TFMQ_NO_Q8") is None
 
@@ -725,4 +726,5 @@ class LdmUNetEngine(DdimUNetEngine):
         for i in range(_n_children(self.sd, "output_blocks")):
             h = self._seq(f"output_blocks.{i}", h, hs.pop(), ctx, rowadd, taps)
         h, _ = self._gn("out.0", h, None, True, None, eps=1e-5, half=self._fp_conv_half_ok(L["out.2"]))
+        self._ctx_mask = None       # (a block run on its own takes none)
         return L["out.2"].run(h, pad=(1, 1, 1, 1), want_stats=False)
