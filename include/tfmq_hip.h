@@ -620,7 +620,8 @@ int tfmq_quantize_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, lo
 int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint8_t* q, uint8_t* qt, float* s, void* stream);
 /* y[m][n] = sum_kb sx[kb][m] sw(n / 128, kb) (sum_{k in kb} qx[m][k] qw[n][k]) + bias[n], y [M][N] contiguous of y_dtype (16-byte aligned), fp32 sums.
  * x [M][K] of dtype, row stride ld, is quantised here; or x = NULL and xq / xs as tfmq_quantize_fp8 leaves them.  w as tfmq_pack_w_fp8 leaves it; the
- * scale of (column block nb, k block kb) at ws[nb * ws_n + kb * ws_k].  work: tfmq_linear_fp8_ws_bytes (0 for up to 32 rows: one launch). */
+ * scale of (column block nb, k block kb) at ws[nb * ws_n + kb * ws_k].  work: tfmq_linear_fp8_ws_bytes (0 where one launch
+ * does it: up to 32 rows, or few outputs). */
 size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K);
 int tfmq_linear_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* xq, const float* xs, const uint8_t* w,
                     const float* ws, long ws_n, long ws_k, const float* bias, void* y, int y_dtype, int N, void* work, void* stream);

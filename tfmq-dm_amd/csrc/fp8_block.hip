@@ -299,40 +299,22 @@ struct GemmF8P {
 __device__ __forceinline__ int key_x(int r) { return r & 7; }
 __device__ __forceinline__ int key_w(int r) { return (r & 3) | ((r >> 2) & 4); }
 
-template <int YDT>
-__device__ __forceinline__ void store_run(typename Elem<YDT>::type* p, const float* v, int n, bool vec) {
-  // up to 16 consecutive outputs of one row
-  using T = typename Elem<YDT>::type;
-  if (vec && n == 16) {
-    if constexpr (YDT == DT_F32) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-      typedef T v8t __attribute__((ext_vector_type(8)));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        v8t o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(v[8 * i + e]);
-        reinterpret_cast<v8t*>(p)[i] = o;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < n) p[i] = static_cast<T>(v[i]);
-  }
-}
-
 // The product.  The MFMA computes W_tile X_tile^T, so a lane owns ONE row m of the output (its scale is one register) and its 16 accumulators are
 // columns n; the rows of W enter the fragment in the order n = 16 h + 4 a + c for fragment row 8 a + 4 h + c, so those 16 columns are consecutive.
-// Operand tiles of one block (128 bytes a row) travel by LDS-DMA into two stages, the next one in flight while this one is multiplied.  A workgroup
-// walks over its tiles (or, sliced, one K range of a tile) as one sequence of blocks: the next tile's first stage is under way while the results of
-// this one are rounded and stored.
-template <int BM, int BN, int WM, int WN, int YDT, bool SBROW>
+// Operand tiles of one block (128 bytes a row) and its scales travel by LDS-DMA into S stages, S - 1 of them in flight while one is multiplied.
+// Everything that a block needs comes this way: a compiler-counted load would wait for all LDS-DMA behind it.  A workgroup walks over its tiles (or,
+// sliced, one K range of a tile) as one sequence of blocks: the next tile's first stages are under way while the results of this one are rounded and
+// stored.
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int S>
+struct GemmF8 {
+  static constexpr int NWM = BM / WM, NWN = BN / WN, NW = NWM * NWN;
+  static constexpr int STAGE = (BM + BN) * 128, NSC = BM / 64 + (SBROW ? BN / 64 : 1), SCALES = NSC * 256;
+  static constexpr int LDS = S * (STAGE + SCALES);
+};
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int S>
 __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, int bid, int nblocks, int first) {
-  constexpr int NWM = BM / WM, NWN = BN / WN, NW = NWM * NWN, TM = WM / 32, TN = WN / 32;
-  constexpr int STAGE = (BM + BN) * 128;
+  using G = GemmF8<BM, BN, WM, WN, YDT, SBROW, S>;
+  constexpr int NWM = G::NWM, NW = G::NW, TM = WM / 32, TN = WN / 32, STAGE = G::STAGE;
   using YT = typename Elem<YDT>::type;
   using F = Frag<YDT == DT_F32>;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -340,24 +322,33 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
   const int wm = wid % NWM, wn = wid / NWM;
   const long Kp = static_cast<long>(p.Kb) * 128;
   const int ntile = p.tm * p.tn;
-  float* sS = reinterpret_cast<float*>(smem + 2 * STAGE) + wid * WN;          // SBROW: this wave's column scales of a block
 
-  // ---- LDS-DMA plan: instruction i of a wave moves 8 rows x 128 bytes; rows [0, BN) of a stage are W, [BN, BN + BM) X; a wave moves one of them
-  constexpr int NI = (BM + BN) / 8 / NW;
+  // ---- LDS-DMA plan: instruction i of a wave moves 8 rows x 128 bytes; rows [0, BN) of a stage are W, [BN, BN + BM) X; a wave moves one of them.
+  // One more instruction a wave moves 64 scales: rows of X first, then (SBROW) columns or the column blocks' (surplus waves repeat a piece).
+  constexpr int NI = (BM + BN) / 8 / NW, PER = NI + 1;
   static_assert((BM + BN) % (8 * NW) == 0 && BN % (8 * NI) == 0, "whole rows per wave instruction, one operand per wave");
-  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem)) + wid * NI * 1024;
+  static_assert(G::NSC <= NW && BN % 128 == 0 && 128 % WN == 0, "a wave per 64 scales; a wave's columns share a block");
+  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)smem));
   const bool is_w = wid * NI * 8 < BN;
-  unsigned voff[NI];
-  const uint8_t* src = nullptr;
-  long m0 = 0;
-  int n0 = 0;
-  auto place = [&](int tile) {
-    // neighbouring workgroups of an XCD share rows and columns: groups of 8 row tiles walk the columns
+  const int sc = wid % G::NSC;
+  const bool sc_x = sc < BM / 64;
+  const int nb_last = (p.N - 1) >> 7;
+  // neighbouring workgroups of an XCD share rows and columns: groups of 8 row tiles walk the columns
+  auto origin = [&](int tile, long& m, int& n) {
     const int gsz = 8 * p.tn, grp = tile / gsz, first = grp * 8, rows = min(p.tm - first, 8), in = tile - grp * gsz;
-    m0 = static_cast<long>(first + in % rows) * BM;
-    n0 = (in / rows) * BN;
+    m = static_cast<long>(first + in % rows) * BM;
+    n = (in / rows) * BN;
+  };
+  unsigned voff[NI], soff = 0;
+  const uint8_t* src = nullptr;
+  const float* ssrc = nullptr;
+  auto place = [&](int tile) {
+    long m0;
+    int n0;
+    origin(tile, m0, n0);
     src = uniform_ptr(is_w ? p.b + n0 * Kp : p.a + m0 * Kp);
-    const unsigned last = __builtin_amdgcn_readfirstlane(static_cast<int>(is_w ? p.N - 1 - n0 : min(static_cast<long>(BM), p.M - m0) - 1));
+    const int last_m = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<long>(BM), p.M - m0) - 1)), last_n = p.N - 1 - n0;
+    const unsigned last = is_w ? last_n : last_m;
     const int r0 = (is_w ? wid : wid - BN / (8 * NI)) * NI * 8 + (lane >> 3);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -365,13 +356,29 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
       voff[i] = min(static_cast<unsigned>(r), last) * static_cast<unsigned>(Kp) + (((lane & 7) ^ (is_w ? key_w(r) : key_x(r))) << 4);
       asm volatile("" : "+v"(voff[i]));          // kept, not recomputed for every block
     }
+    if (sc_x) {
+      ssrc = p.sa + m0;
+      soff = 4 * min(sc * 64 + lane, last_m);
+    } else if (SBROW) {
+      ssrc = p.sb + n0;
+      soff = 4 * min((sc - BM / 64) * 64 + lane, last_n);
+    } else {
+      ssrc = p.sb + static_cast<long>(n0 >> 7) * p.sbn;
+      soff = 4 * static_cast<unsigned>(min(min(lane, BN / 128 - 1), nb_last - (n0 >> 7))) * static_cast<unsigned>(p.sbn);
+    }
+    ssrc = uniform_ptr(ssrc);
+    asm volatile("" : "+v"(soff));
   };
+  const long sstep = sc_x ? p.M : SBROW ? p.N : p.sbk;
   auto fetch = [&](int kb, int st) {
     const uint8_t* base = uniform_ptr(src + static_cast<long>(kb) * 128);
-    const unsigned dst = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE);
+    const unsigned dst = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE + wid * NI * 1024);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff[i]), "s"(base), "s"(dst + i * 1024) : "memory", "m0");
+    const float* sbase = uniform_ptr(ssrc + kb * sstep);
+    const unsigned sdst = __builtin_amdgcn_readfirstlane(lds0 + S * STAGE + st * G::SCALES + sc * 256);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(soff), "s"(sbase), "s"(sdst) : "memory", "m0");
   };
   // this workgroup's slice of the blocks, and its tiles
   const int sl = p.nslice > 1 ? bid % p.nslice : 0;
@@ -379,20 +386,7 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
   int tile = p.nslice > 1 ? bid / p.nslice : first;
   const int stride = p.nslice > 1 ? ntile : nblocks;
   if (tile >= ntile) return;
-  const int nb_last = (p.N - 1) >> 7;
-  static_assert(!SBROW || WN == 64, "a lane per column");
-  static_assert(128 % WN == 0 && BN % 128 == 0, "a wave's columns share a scale");
 
-  float sx[TM], sxn[TM] = {}, sbn = 0.0f;          // row scales (times the column block's) of this block; what has been asked for of the next
-  auto scales = [&](int kb) {
-    const float* row = p.sa + static_cast<long>(kb) * p.M;
-#pragma unroll
-    for (int t = 0; t < TM; ++t) sxn[t] = row[min(m0 + wm * WM + t * 32 + j, p.M - 1)];
-    // (a wave's columns lie in one block of 128.  The scales travel a block ahead and are first touched behind the wait for the stage: a use, or a
-    // load, between the LDS-DMA and that wait would wait for the LDS-DMA)
-    sbn = SBROW ? p.sb[static_cast<long>(kb) * p.N + min(n0 + wn * WN + lane, p.N - 1)]
-                : p.sb[static_cast<long>(min((n0 + wn * WN) >> 7, nb_last)) * p.sbn + kb * p.sbk];
-  };
   // fragment addresses inside a stage: four 16-byte pieces of a row (the sub-tiles are immediates)
   const int rw = wn * WN + 16 * ((j >> 2) & 1) + 4 * (j >> 3) + (j & 3), rx = wm * WM + j;          // fragment row j of W holds row rw
   unsigned pw[4], px[4];
@@ -405,14 +399,23 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
   v16f acc[TN][TM];
   // one block of a stage: products into acc
   auto block = [&](int st) {
-    const unsigned char* S = smem + st * STAGE;
+    const unsigned char* D = smem + st * STAGE;
+    const float* sS = reinterpret_cast<const float*>(smem + S * STAGE + st * G::SCALES);
+    float sx[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) sx[t] = sS[rx + t * 32];
+    if constexpr (!SBROW) {
+      const float sb = sS[BM + ((wn * WN) >> 7)];
+#pragma unroll
+      for (int t = 0; t < TM; ++t) sx[t] *= sb;
+    }
     F wf[TN][2];
     float swr[SBROW ? TN : 1][16];
 #pragma unroll
     for (int u = 0; u < TN; ++u) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint4 w = *reinterpret_cast<const uint4*>(S + pw[q] + u * 32 * 128);
+        const uint4 w = *reinterpret_cast<const uint4*>(D + pw[q] + u * 32 * 128);
         F& f = wf[u][q >> 1];
         f.set(4 * (q & 1), w.x); f.set(4 * (q & 1) + 1, w.y); f.set(4 * (q & 1) + 2, w.z); f.set(4 * (q & 1) + 3, w.w);
       }
@@ -421,7 +424,7 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
       if constexpr (SBROW) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 v = *reinterpret_cast<const float4*>(sS + u * 32 + 16 * hh + 4 * q4);
+          const float4 v = *reinterpret_cast<const float4*>(sS + BM + wn * WN + u * 32 + 16 * hh + 4 * q4);
           swr[u][4 * q4] = v.x; swr[u][4 * q4 + 1] = v.y; swr[u][4 * q4 + 2] = v.z; swr[u][4 * q4 + 3] = v.w;
         }
       }
@@ -431,7 +434,7 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
       F xf[2];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint4 w = *reinterpret_cast<const uint4*>(S + px[q] + t * 32 * 128);
+        const uint4 w = *reinterpret_cast<const uint4*>(D + px[q] + t * 32 * 128);
         F& f = xf[q >> 1];
         f.set(4 * (q & 1), w.x); f.set(4 * (q & 1) + 1, w.y); f.set(4 * (q & 1) + 2, w.z); f.set(4 * (q & 1) + 3, w.w);
       }
@@ -452,11 +455,38 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
     }
   };
 
-  place(tile);
-  scales(min(k_lo, p.Kb - 1));
-  if (k_lo < k_hi) fetch(k_lo, 0);
-  int st = 0;
-  bool stores = false;          // the last tile's stores (at least TM TN 2 instructions a wave) may still be under way
+  // the fetches run S - 1 blocks ahead of the products, over the tiles' ends: (ft, fk) is the next one, `ahead` stages are under way or have arrived
+  int ft = k_lo < k_hi ? tile : ntile, fk = k_lo, ahead = 0;
+  auto fetch_next = [&](int st) {
+    if (ft >= ntile) return;
+    if (fk == k_lo) place(ft);
+    fetch(fk, st);
+    ++ahead;
+    if (++fk == k_hi) {
+      fk = k_lo;
+      ft += stride;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) fetch_next(s);
+  // waits for the oldest stage: what was issued behind it may be under way -- `ahead` - 1 stages and, for S - 1 blocks behind a tile whose stores are
+  // known (every lane, whole lines), those
+  constexpr int NST = TM * TN * (YDT == DT_F32 ? 4 : 2);
+  static_assert((S - 2) * PER + NST < 64, "the counter's range");
+  auto arrive = [&](bool stores) {
+    if (stores) {
+      if (S >= 4 && ahead == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER + NST) : "memory");
+      else if (S >= 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER + NST) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NST) : "memory");
+    } else {
+      if (S >= 4 && ahead == 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+      else if (S >= 3 && ahead == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    --ahead;
+  };
+  static_assert(S >= 2 && S <= 4, "the waits above");
+  int st = 0, stores = 0;
   for (; tile < ntile; tile += stride) {
 #pragma unroll
     for (int u = 0; u < TN; ++u)
@@ -464,39 +494,28 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
       for (int t = 0; t < TM; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[u][t][r] = 0.0f;
-    const long mt = m0;
-    const int nbase = n0 + wn * WN;
-    const bool full = (p.N * sizeof(YT)) % 16 == 0 && m0 + BM <= p.M && n0 + BN <= p.N;
     for (int kb = k_lo; kb < k_hi; ++kb) {
-      if (stores) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TM * TN * (YDT == DT_F32 ? 4 : 2)) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      stores = false;
-#pragma unroll
-      for (int t = 0; t < TM; ++t) {
-        sx[t] = SBROW ? sxn[t] : sxn[t] * sbn;
-        asm volatile("" : "+v"(sx[t]));          // here, not behind the next LDS-DMA
-      }
-      if constexpr (SBROW) sS[lane] = sbn;
-      LDS_BARRIER();                   // this stage has arrived for every wave, and every wave is through with the other one
-      if (kb + 1 < k_hi) {
-        scales(kb + 1);
-        fetch(kb + 1, st ^ 1);
-      } else if (tile + stride < ntile) {
-        place(tile + stride);
-        scales(k_lo);
-        fetch(k_lo, st ^ 1);
-      }
+      arrive(stores > 0);
+      --stores;
+      LDS_BARRIER();                   // this stage has arrived for every wave, and every wave is through with the one before it
+      const int before = st == 0 ? S - 1 : st - 1;
+      fetch_next(before);
       block(st);
-      st ^= 1;
+      st = st == S - 1 ? 0 : st + 1;
     }
     // ---- lane (row m, half hh) holds columns u * 32 + 16 hh + (0 .. 15): out through LDS (this wave's part of the stage just multiplied), 32 rows x
-    // 128 bytes at a time, so that the stores are whole lines
+    // 128 bytes at a time, so that the stores are whole lines; 16-byte piece c of row r at c ^ (r & 7)
+    long mt;
+    int n0;
+    origin(tile, mt, n0);
+    const int nbase = n0 + wn * WN;
+    const bool full = (p.N * sizeof(YT)) % 16 == 0 && mt + BM <= p.M && n0 + BN <= p.N;
     YT* out = reinterpret_cast<YT*>(p.y) + (p.nslice > 1 ? static_cast<long>(sl) * p.M * p.N : 0);
-    constexpr int CW = 128 / static_cast<int>(sizeof(YT)), UC = CW / 32, SR = 144, PE = 16 / static_cast<int>(sizeof(YT));
-    static_assert(NW * 32 * SR <= STAGE, "the waves' store buffers fit a stage");
+    constexpr int CW = 128 / static_cast<int>(sizeof(YT)), UC = CW / 32, PE = 16 / static_cast<int>(sizeof(YT));
+    static_assert(NW * 32 * 128 <= STAGE && WN % CW == 0, "the waves' store buffers fit a stage");
     const bool vec = (p.N * sizeof(YT)) % 16 == 0;
     LDS_BARRIER();                     // every wave is through with that stage
-    unsigned char* sO = smem + (st ^ 1) * STAGE + wid * 32 * SR;
+    unsigned char* sO = smem + (st == 0 ? S - 1 : st - 1) * STAGE + wid * 32 * 128;
 #pragma unroll
     for (int c = 0; c < WN / CW; ++c) {
       const int nc = nbase + c * CW;
@@ -512,41 +531,48 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
 #pragma unroll
             for (int r = 0; r < 16; ++r) v[r] += p.bias[min(nl + r, p.N - 1)];
           }
-          store_run<YDT>(reinterpret_cast<YT*>(sO + j * SR) + u * 32 + 16 * hh, v, 16, true);
+          typedef YT vt __attribute__((ext_vector_type(PE)));
+#pragma unroll
+          for (int i = 0; i < 16 / PE; ++i) {
+            vt o;
+#pragma unroll
+            for (int e = 0; e < PE; ++e) o[e] = static_cast<YT>(v[i * PE + e]);
+            *reinterpret_cast<vt*>(sO + j * 128 + ((((u * 32 + 16 * hh) / PE + i) ^ (j & 7)) << 4)) = o;
+          }
         }
         const long mb = mt + wm * WM + t * 32;
         if (vec) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = i * 8 + (lane >> 3), pc = lane & 7;
-            const uint4 w = *reinterpret_cast<const uint4*>(sO + r * SR + pc * 16);
+            const uint4 w = *reinterpret_cast<const uint4*>(sO + r * 128 + ((pc ^ (r & 7)) << 4));
             if (full || (mb + r < p.M && nc + pc * PE < p.N)) *reinterpret_cast<uint4*>(out + (mb + r) * p.N + nc + pc * PE) = w;
           }
         } else {
 #pragma unroll 1
           for (int e = lane; e < 32 * CW; e += 64) {
             const int r = e / CW, n = e % CW;
-            if (mb + r < p.M && nc + n < p.N) out[(mb + r) * p.N + nc + n] = reinterpret_cast<const YT*>(sO + r * SR)[n];
+            if (mb + r < p.M && nc + n < p.N) out[(mb + r) * p.N + nc + n] = reinterpret_cast<const YT*>(sO + r * 128 + (((n / PE) ^ (r & 7)) << 4))[n % PE];
           }
         }
       }
     }
-    stores = full;
+    stores = full ? S - 1 : 0;
   }
 }
 
-template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), WPS) void k_gemm_f8(GemmF8P p) {
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int S>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_gemm_f8(GemmF8P p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  gemm_f8<BM, BN, WM, WN, YDT, SBROW>(p, smem, blockIdx.x, gridDim.x, xcd_tile_id());
+  gemm_f8<BM, BN, WM, WN, YDT, SBROW, S>(p, smem, blockIdx.x, gridDim.x, xcd_tile_id());
 }
 // a weight gradient's slices (the longer workgroups, first) and the other gradient's tiles in one launch: either alone leaves CUs idle
 template <int YDT>
 __global__ __launch_bounds__(256, 2) void k_gemm_f8_grads(GemmF8P gw, GemmF8P gx, int nw) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int q = blockIdx.x;
-  if (q < nw) gemm_f8<128, 128, 64, 64, DT_F32, true>(gw, smem, q, nw, q);
-  else gemm_f8<128, 128, 64, 64, YDT, false>(gx, smem, q - nw, gridDim.x - nw, q - nw);
+  if (q < nw) gemm_f8<128, 128, 64, 64, DT_F32, true, 2>(gw, smem, q, nw, q);
+  else gemm_f8<128, 128, 64, 64, YDT, false, 2>(gx, smem, q - nw, gridDim.x - nw, q - nw);
 }
 
 // slices of the K axis, added in order; four outputs a thread
@@ -569,21 +595,32 @@ __global__ __launch_bounds__(256) void k_sum_slices(const float* __restrict__ pa
   }
 }
 
-template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int WPS>
+template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int S>
 int launch_gemm(tfmq_handle h, GemmF8P p, hipStream_t st) {
-  constexpr int NW = (BM / WM) * (BN / WN), smem = 2 * (BM + BN) * 128 + (SBROW ? NW * WN * 4 : 0);
-  auto kern = &k_gemm_f8<BM, BN, WM, WN, YDT, SBROW, WPS>;
+  using G = GemmF8<BM, BN, WM, WN, YDT, SBROW, S>;
+  constexpr int NW = G::NW, smem = G::LDS;
+  auto kern = &k_gemm_f8<BM, BN, WM, WN, YDT, SBROW, S>;
   static LdsRoom room_kern;
   TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
   p.tm = ceil_div(p.M, BM);
   p.tn = ceil_div(p.N, BN);
   const long nt = static_cast<long>(p.tm) * p.tn;
   TFMQ_CHECK_ARG(h, nt * 8 < (1L << 31), "gemm_fp8: too many tiles");
-  const long room = static_cast<long>(h->cu_count) * (4 * WPS / NW);          // resident workgroups
+  const long room = static_cast<long>(h->cu_count) * (8 / NW);          // resident workgroups
   const long nb = p.nslice > 1 ? nt * p.nslice : (nt < room ? nt : room);
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nb)), dim3(64 * NW), smem, st, p);
   TFMQ_LAUNCH_CHECK(h);
   return TFMQ_OK;
+}
+
+// 128 x 128 tiles: with at most one a CU, eight waves of 32 x 64 and four stages; else two workgroups a CU, four waves of 64 x 64 and two stages.  us,
+// the latter against the former, quantiser included: 1024 x 5120 x 1280 46.7 / 41.6, 512 x 1280 x 1280 15.3 / 14.1, 2048 x 768 x 1280 13.4 / 12.7.
+// Eight waves at two workgroups a CU (126 registers, four waves a SIMD) gain nothing on full cards: 8192 x 320 x 2560 25.5 / 24.6,
+// 16384 x 5120 x 1280 146 / 152.
+template <int YDT, bool SBROW>
+int launch_128(tfmq_handle h, const GemmF8P& p, hipStream_t st) {
+  const long nb = static_cast<long>(ceil_div(p.M, 128)) * ceil_div(p.N, 128) * p.nslice;
+  return nb <= h->cu_count ? launch_gemm<128, 128, 32, 64, YDT, SBROW, 4>(h, p, st) : launch_gemm<128, 128, 64, 64, YDT, SBROW, 2>(h, p, st);
 }
 
 bool rows_aligned(const void* x, int dtype, int K, long ld) {
@@ -723,7 +760,7 @@ int launch_small(tfmq_handle h, const SmallF8P& p, int dtype, int y_dtype, hipSt
 
 template <int YDT>
 int launch_grads(tfmq_handle h, GemmF8P gw, GemmF8P gx, hipStream_t st) {
-  constexpr int smem = 2 * 256 * 128 + 4 * 64 * 4;
+  constexpr int smem = GemmF8<128, 128, 64, 64, DT_F32, true, 2>::LDS;
   auto kern = &k_gemm_f8_grads<YDT>;
   static LdsRoom room;
   TFMQ_HIP(h, room.ask(h, reinterpret_cast<const void*>(kern), smem));
@@ -736,16 +773,25 @@ int launch_grads(tfmq_handle h, GemmF8P gw, GemmF8P gx, hipStream_t st) {
   return TFMQ_OK;
 }
 
-// ---- which kernel multiplies.  Tiles of 256 x 256 where they fill the card in whole rounds (at least three quarters of the last one), else 128 x 128.
+// ---- which kernel multiplies.  Tiles of 256 x 256 where they fill the card in whole rounds (at least three quarters of all), else 128 x 128.  us, 128^2
+// against 256^2: 16384 x 1280 x 10240 (10 rounds, full) 338 / 288; 6144 x 1280 x 3840 (360 tiles, 70 %) 48.9 / 50.1; 8192 x 320 x 2560 (320 tiles, 62 %)
+// 21.9 / 25.4; 4096 x 1280 x 1280 (80 tiles, 31 %) 16.8 / 24.5.
 bool big_tiles(tfmq_handle h, long M, int N) {
   const long nt = static_cast<long>(ceil_div(M, 256)) * ceil_div(N, 256), cu = h->cu_count;
   return nt >= cu && nt * 4 >= (nt + cu - 1) / cu * cu * 3;
 }
+// One launch that quantises on the way in (tiles of 32 x 32, eight ways along K) instead of two: for few rows, and while its workgroups are at most two
+// per CU -- from there the 128 x 128 tiles' reuse counts for more than their idle CUs.  us, one launch against two: 154 x 1280 x 1280 6.2 / 14.5,
+// 256 x 1280 x 1280 9.9 / 14.6, 256 x 5120 x 1280 31 / 42, 512 x 1280 x 1280 (2.5 per CU) 13.6 / 15.3, 512 x 5120 x 1280 45.6 / 44.5,
+// 1024 x 1280 x 1280 21 / 16.5, 154 x 1280 x 10240 (6 per CU) 26.7 / 15.4.
+bool one_launch(tfmq_handle h, long M, int N) {
+  return M <= 32 || static_cast<long>(ceil_div(M, 32)) * ceil_div(N, 32) <= 2L * h->cu_count;
+}
 int launch_product(tfmq_handle h, const GemmF8P& p, int y_dtype, hipStream_t st) {
-  if (y_dtype == DT_F32) return launch_gemm<128, 128, 64, 64, DT_F32, false, 2>(h, p, st);
+  if (y_dtype == DT_F32) return launch_128<DT_F32, false>(h, p, st);
   if (big_tiles(h, p.M, p.N))
     return y_dtype == DT_F16 ? launch_gemm<256, 256, 128, 64, DT_F16, false, 2>(h, p, st) : launch_gemm<256, 256, 128, 64, DT_BF16, false, 2>(h, p, st);
-  return y_dtype == DT_F16 ? launch_gemm<128, 128, 64, 64, DT_F16, false, 2>(h, p, st) : launch_gemm<128, 128, 64, 64, DT_BF16, false, 2>(h, p, st);
+  return y_dtype == DT_F16 ? launch_128<DT_F16, false>(h, p, st) : launch_128<DT_BF16, false>(h, p, st);
 }
 // slices of the token axis of a weight gradient [N][K]: its tiles alone leave CUs idle, every slice costs a write and a read of the result in fp32
 int grad_slices(tfmq_handle h, long M, int N, int K) {
@@ -754,7 +800,6 @@ int grad_slices(tfmq_handle h, long M, int N, int K) {
   return static_cast<int>(n < 1 ? 1 : n < Mb ? n : Mb);
 }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-constexpr long SMALL_M = 32;          // rows up to which one launch that quantises on the way in beats two
 
 // the buffers of a call inside its workspace; sizes in bytes
 struct Carve {
@@ -782,7 +827,7 @@ struct BwdWs {
   int slices;
   BwdWs(Carve& c, tfmq_handle h, long M, int N, int K, bool gx, bool gw) {
     const long Mb = (M + 127) / 128, Nb = (N + 127) / 128;
-    if (gx && (gw || M > SMALL_M)) {
+    if (gx && !one_launch(h, M, K)) {
       gq = c.take<uint8_t>(static_cast<size_t>(M) * Nb * 128);
       gs = c.take<float>(static_cast<size_t>(M) * Nb);
     }
@@ -821,7 +866,7 @@ extern "C" int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint
 }
 
 extern "C" size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K) {
-  if (!h || !shape_ok(M, N, K) || M <= SMALL_M) return 0;
+  if (!h || !shape_ok(M, N, K) || one_launch(h, M, N)) return 0;
   Carve c{nullptr};
   LinWs w(c, M, K);
   return c.at;
@@ -835,9 +880,9 @@ extern "C" int tfmq_linear_fp8(tfmq_handle h, const void* x, int dtype, long M, 
   TFMQ_CHECK_ARG(h, aligned16(w) && aligned16(xq) && aligned16(y) && aligned16(work), "linear_fp8: operands, output and workspace must be 16-byte aligned");
   hipStream_t st = as_stream(stream);
   const int Kb = (K + 127) / 128;
-  if (x && M <= SMALL_M) return launch_small(h, SmallF8P{x, ld, static_cast<int>(M), K, w, ws, ws_n, ws_k, bias, y, N, Kb}, dtype, y_dtype, st);
+  if (x && one_launch(h, M, N)) return launch_small(h, SmallF8P{x, ld, static_cast<int>(M), K, w, ws, ws_n, ws_k, bias, y, N, Kb}, dtype, y_dtype, st);
   if (x) {
-    TFMQ_CHECK_ARG(h, work, "linear_fp8: more than 32 rows need a workspace");
+    TFMQ_CHECK_ARG(h, work, "linear_fp8: null workspace");
     Carve c{static_cast<char*>(work)};
     const LinWs b(c, M, K);
     const int rc = launch_quant_rows(h, x, dtype, M, K, ld, b.q, b.s, st);
@@ -878,14 +923,14 @@ extern "C" int tfmq_linear_fp8_bwd(tfmq_handle h, const void* x, int x_dtype, lo
   const GemmF8P px{b.gq, wt, b.gs, ws, 1, Kb, nullptr, gx, M, K, Nb, 0, 0, 1};
   const int Mb = static_cast<int>((M + 127) / 128);
   const GemmF8P pw{b.gc, b.xc, b.gcs, b.xcs, 0, 0, nullptr, gw ? (b.part ? b.part : gw) : nullptr, N, K, Mb, 0, 0, gw ? b.slices : 1};
-  if (gx && gw && !big_tiles(h, M, K)) {
+  if (b.gq && gw && !big_tiles(h, M, K)) {
     if (gy_dtype == DT_F32) rc = launch_grads<DT_F32>(h, pw, px, st);
     else rc = gy_dtype == DT_F16 ? launch_grads<DT_F16>(h, pw, px, st) : launch_grads<DT_BF16>(h, pw, px, st);
   } else {
     if (gx)
       rc = b.gq ? launch_product(h, px, gy_dtype, st)
                 : launch_small(h, SmallF8P{gy, gy_ld, static_cast<int>(M), N, wt, ws, 1, Kb, nullptr, gx, K, Nb}, gy_dtype, gy_dtype, st);
-    if (rc == TFMQ_OK && gw) rc = launch_gemm<128, 128, 64, 64, DT_F32, true, 2>(h, pw, st);
+    if (rc == TFMQ_OK && gw) rc = launch_128<DT_F32, true>(h, pw, st);
   }
   if (rc != TFMQ_OK) return rc;
   if (gw && b.part) {
