@@ -660,7 +660,7 @@ int tfmq_xattn_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk);
 int tfmq_xattn_fwd(tfmq_handle h, const tfmq_xattn_desc* a, void* stream);
 /* dq, dk, dv from q, k, v, o, lse, go.  nsplit: slices of the rows in the dk / dv sums; ws: (2 B H Tq rounded up to 4) floats, and
  * nsplit * 2 * B * Tk * G * d more when nsplit > 1.  Deterministic. */
-int tfmq_xattn_bwd_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk, int d);
+int tfmq_xattn_bwd_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk);
 int tfmq_xattn_bwd(tfmq_handle h, const tfmq_xattn_desc* a, void* stream);
 
 /* ---- K16: the exchange step of the sharded calibration: RCCL over xGMI, one rank per GPU.

@@ -209,7 +209,7 @@ _SIGS = {
                                     c_void_p, c_void_p, c_void_p]),
     "tfmq_xattn_splits": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int]),
     "tfmq_xattn_fwd": (c_int, [c_void_p, c_void_p, c_void_p]),
-    "tfmq_xattn_bwd_splits": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "tfmq_xattn_bwd_splits": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int]),
     "tfmq_xattn_bwd": (c_int, [c_void_p, c_void_p, c_void_p]),
     "tfmq_graph_begin": (c_int, [c_void_p, c_void_p]),
     "tfmq_graph_end": (c_int, [c_void_p, c_void_p, C.POINTER(c_int)]),

@@ -144,7 +144,8 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
 
 // ---- up to 128 states (a text encoder's): K and V of one (item, key head) stay in LDS, the waves walk over rows on their own, without barriers, the next
 // rows' queries under way.  All keys are in the accumulators at once: one maximum, no running rescale.
-// waves per SIMD that the registers allow without spilling (the walk waits for memory: 4 against 2 took the 128 x 1024 x 77 call from 114 to FWDSHORT us)
+// waves per SIMD that the registers allow without spilling (the walk waits for memory: 4 against 2 took the 128 x 1024 x 77 call, 8 heads of 80, from 114 to
+// 112 us; reading and writing rows through buffer descriptors then to 105, 3.4 TB/s)
 constexpr int short_waves(int D, int NKT) { return D <= 64 || (D <= 96 && NKT <= 3) ? 4 : D <= 128 || NKT <= 2 ? 3 : 2; }
 
 template <typename T, int D, int NKT>
@@ -229,28 +230,34 @@ __global__ __launch_bounds__(256, short_waves(D, NKT)) void k_xattn_short(XattnP
   }
 }
 
-// joins the slices of a row: 16 lanes a row, four (eight) channels a lane and step
+// joins the slices of a row: a wave a row, 16 lanes of 8 channels for each of four slices at a time (a longer walk per lane waits for memory at every
+// step: 512 slices of one row took 250 us with one lane per 8 channels).  The four partial sums meet in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_xattn_join(XattnP p) {
   const long rows = static_cast<long>(p.B) * p.H * p.Tq;
-  const long r = static_cast<long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int c16 = threadIdx.x & 15;
+  const long r = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c16 = lane & 15, s4 = lane >> 4;
   if (r >= rows) return;
   const float* ml = p.part + static_cast<long>(p.nsplit) * rows * p.d;
   float M = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, ml[(s * rows + r) * 2]);
+  for (int s = lane; s < p.nsplit; s += 64) M = fmaxf(M, ml[(s * rows + r) * 2]);
+  M = wave_reduce_max(M);
   const float mu = M == -INFINITY ? 0.0f : M;
   float l = 0.0f;
-  for (int s = 0; s < p.nsplit; ++s) l = __builtin_fmaf(ml[(s * rows + r) * 2 + 1], __builtin_amdgcn_exp2f(ml[(s * rows + r) * 2] - mu), l);
+  for (int s = lane; s < p.nsplit; s += 64) l = __builtin_fmaf(ml[(s * rows + r) * 2 + 1], __builtin_amdgcn_exp2f(ml[(s * rows + r) * 2] - mu), l);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const long bh = r / p.Tq;
   const int i = static_cast<int>(r - bh * p.Tq), b = static_cast<int>(bh / p.H), head = static_cast<int>(bh - static_cast<long>(b) * p.H);
   T* y = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
-  for (int c = c16 * 8; c < p.d; c += 128) {
+  for (int c0 = 0; c0 < p.d; c0 += 128) {
+    const int c = min(c0 + c16 * 8, p.d - 8);          // (lanes past the head read its last channels)
     float a[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) a[e] = 0.0f;
-    for (int s = 0; s < p.nsplit; ++s) {
+#pragma unroll 4
+    for (int s = s4; s < p.nsplit; s += 4) {
       const float w = __builtin_amdgcn_exp2f(ml[(s * rows + r) * 2] - mu);
       const float4* po = reinterpret_cast<const float4*>(p.part + (s * rows + r) * p.d + c);
       const float4 x = po[0], z = po[1];
@@ -259,10 +266,14 @@ __global__ __launch_bounds__(256) void k_xattn_join(XattnP p) {
     }
     typename Vec8<T>::type w8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w8[e] = static_cast<T>(a[e] * inv);
-    *reinterpret_cast<typename Vec8<T>::type*>(y + c) = w8;
+    for (int e = 0; e < 8; ++e) {
+      a[e] += __shfl_xor(a[e], 16, 64);
+      a[e] += __shfl_xor(a[e], 32, 64);
+      w8[e] = static_cast<T>(a[e] * inv);
+    }
+    if (s4 == 0 && c0 + c16 * 8 < p.d) *reinterpret_cast<typename Vec8<T>::type*>(y + c) = w8;
   }
-  if (p.lse && c16 == 0) p.lse[r] = l != 0.0f ? (M + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+  if (p.lse && lane == 0) p.lse[r] = l != 0.0f ? (M + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
 }
 
 template <typename T, int D, int NKT>
@@ -301,7 +312,7 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nb)), dim3(256), smem, st, p);
     TFMQ_LAUNCH_CHECK(h);
     if (p.nsplit > 1) {
-      hipLaunchKernelGGL((k_xattn_join<T>), dim3(static_cast<unsigned>((static_cast<long>(p.B) * p.H * p.Tq + 15) / 16)), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((k_xattn_join<T>), dim3(static_cast<unsigned>((static_cast<long>(p.B) * p.H * p.Tq + 3) / 4)), dim3(256), 0, st, p);
       TFMQ_LAUNCH_CHECK(h);
     }
     return TFMQ_OK;
@@ -310,15 +321,17 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
 
 }  // namespace
 
-// Slices of the key axis of a forward call: only where the rows alone leave CUs idle; at least two tiles of 64 keys a slice.
+// Slices of the key axis of a forward call, where the rows alone leave CUs idle.  Few rows (at most a wave's 32 of a workgroup's 128: single tokens with
+// shared key heads): four workgroups a CU, so that items of different lengths even out; us at 16 x 1 x 4095, 32 heads on 8 of 128, for 1 / 4 / 6 / 8 / 16
+// slices: lengths drawn 92 / 39 / 32 / 31 / 33, all full 91 / 47 / 55 / 50 / 52.  Full tiles write and join as much as they read: two a CU and none from one
+// a CU on; 2 x 512 x 4096, 16 heads of 64 (128 workgroups), 1 / 2 / 4 / 8 slices 62 / 45 / 34 / 37; 2 x 1000 x 1500, 16 heads on 4 of 128 (256 workgroups)
+// 1 / 2 slices 16 / 35.  A slice has four tiles of 64 keys (1 x 64 x 4096, 16 heads: 16 / 32 slices 13.9 / 16.2; 65536 keys of one head: 256 / 512 slices
+// 36 / 57), two where that leaves fewer than four slices (8 x 16 x 500, 8 heads of 40: 2 / 4 slices 11.6 / 9.3).
 extern "C" int tfmq_xattn_splits(tfmq_handle h, int B, int H, int G, int Tq, int Tk) {
-  if (!h || B <= 0 || H <= 0 || G <= 0 || H % G || Tq <= 0 || Tk <= 0) return 1;
-  const long blocks = static_cast<long>(B) * G * ceil_div(static_cast<long>(H / G) * Tq, 128);
-  const long want = 3L * h->cu_count;
-  if (blocks * 2 > want) return 1;
-  if (Tk <= 128) return 1;
-  const long most = (Tk + 127) / 128;
-  const long n = want / blocks;
+  if (!h || B <= 0 || H <= 0 || G <= 0 || H % G || Tq <= 0 || Tk <= 128) return 1;
+  const long R = static_cast<long>(H / G) * Tq, blocks = static_cast<long>(B) * G * ceil_div(R, 128);
+  if (R > 32 && blocks >= h->cu_count) return 1;
+  const long n = (R > 32 ? 2L : 4L) * h->cu_count / blocks, most = std::max<long>(ceil_div(Tk, 256), std::min<long>(4, ceil_div(Tk, 128)));
   return static_cast<int>(n < 1 ? 1 : n < most ? n : most);
 }
 

@@ -2052,7 +2052,7 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
             t.zero_()
         return dq, dk, dv
     h = handle(a.d_)
-    n = h.lib.tfmq_xattn_bwd_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk, a.d)
+    n = h.lib.tfmq_xattn_bwd_splits(h.h, a.B, a.H, a.G, a.Tq, a.Tk)
     rows = (2 * a.B * a.H * a.Tq + 3) // 4 * 4
     ws = _alloc(rows + (2 * n * a.B * a.Tk * a.G * a.d if n > 1 else 0), dtype=torch.float32, device=q.device)
     h.call("xattn_bwd", a.pack(ov, lse.data_ptr(), ws.data_ptr(), n, gv, dq.data_ptr(), dk.data_ptr(), dv.data_ptr()), _stream(a.d_))
