@@ -231,3 +231,16 @@ def test_captured_and_replayed_on_a_side_stream(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[i])), i
         _ = step(xs[0])                                   # eager work between the replays
+
+
+def test_a_copied_weight_is_its_own(ops):
+    """copy.deepcopy of a model copies the tensors of a packed weight: the copy reads its own bytes, scales and bias."""
+    import copy
+    x = _x(40, 300, torch.float16).to(DEV)
+    pw = ops.pack_w_fp8(_x(200, 300, torch.float32, 1).to(DEV), torch.randn(200).to(DEV))
+    y, g = ops.linear_fp8(x, pw), ops.linear_fp8_bwd(x, _x(40, 200, torch.float16, 3).to(DEV), pw)
+    other = copy.deepcopy(pw)
+    for t in (pw.q, pw.qt, pw.scale, pw.bias):
+        t.zero_()
+    assert torch.equal(ops.linear_fp8(x, other), y) and not ops.linear_fp8(x, pw).any()
+    assert torch.equal(ops.linear_fp8_bwd(x, _x(40, 200, torch.float16, 3).to(DEV), other)[0], g[0])

@@ -91,7 +91,7 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::type* row, int c,
 }
 
 // ---- rows: q [M][Kp], s [Kb][M].  16 lanes hold one block of one row (8 values each); a workgroup takes 16 rows of one block column, so the
-// scales leave as 64 contiguous bytes.  HBM-bound: 2 (4) bytes read and 1 written per element.
+// scales leave as 64 contiguous bytes.  HBM-bound: 2 (4) bytes read and 1 written per element; 16384 x 1280 fp16: 14 us (4.5 TB/s).
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void k_quant_rows(const typename Elem<DT>::type* __restrict__ x, long M, int K, long ld, uint8_t* __restrict__ q,
                                                     float* __restrict__ s, int Kb) {
@@ -119,7 +119,8 @@ __global__ __launch_bounds__(256) void k_quant_rows(const typename Elem<DT>::typ
 
 // ---- columns: x [M][K] -> qc [K][Mp] with one scale per column and block of 128 rows, sc [Mb][K]; the row form (q, s as above) from the same
 // values where it is wanted too, so that an upstream gradient, which both products read, is read once.  A workgroup takes 128 rows x 128 columns, a
-// thread 4 x 8 of them; the columns' maxima meet in LDS, the bytes are transposed through LDS and leave as 128-byte rows.  HBM-bound.
+// thread 4 x 8 of them; the columns' maxima meet in LDS, the bytes are transposed through LDS and leave as 128-byte rows.  HBM-bound: 8192 x (640 + 640)
+// bf16, the first 640 in both forms: 12 us (3.1 TB/s; four waves a tile and conflicts in the transposition: 14.4).
 struct QuantTileP {
   const void* x;
   int dt, vec;                 // type code; rows 16-byte aligned and K % 8 == 0
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(512) void k_quant_cols(QuantPairP pr, int n0) {
   else quant_tile_of<DT_BF16>(p, t, L);
 }
 
-// ---- weights: w fp32 [N][K] -> q [N][Kp] and its transpose qt [K][Np], s [Nb][Kb]; one workgroup per 128 x 128 block, run once per layer
+// ---- weights: w fp32 [N][K] -> q [N][Kp] and its transpose qt [K][Np], s [Nb][Kb]; one workgroup per 128 x 128 block, run once per layer (640 x 640: 38 us)
 __global__ __launch_bounds__(256) void k_pack_w_f8(const float* __restrict__ w, int N, int K, uint8_t* __restrict__ q, uint8_t* __restrict__ qt,
                                                    float* __restrict__ s) {
   __shared__ unsigned red[256];
@@ -305,6 +306,12 @@ __device__ __forceinline__ int key_w(int r) { return (r & 3) | ((r >> 2) & 4); }
 // Everything that a block needs comes this way: a compiler-counted load would wait for all LDS-DMA behind it.  A workgroup walks over its tiles (or,
 // sliced, one K range of a tile) as one sequence of blocks: the next tile's first stages are under way while the results of this one are rounded and
 // stored.
+// What bounds it: the LDS-DMA of the operands, the fragment reads, the matrix instructions and the VALU that scales every block's result take about as long as
+// each other, and the barrier of a stage lets them overlap only between the two waves of a SIMD.  16384 x 1280 x 10240 fp16 out (256 x 256 tiles, half the
+// operand bytes of 128 x 128): 265 us, 1.6 PFLOP/s, MFMA busy 38 %, VALU 31 %,
+// LDS 28 % and 13 % conflicts of the LDS-DMA's writes with the reads.  Fragments of block b + 1 in registers under the products of
+// b: 256 x 128 tiles spill 68 bytes, 177 against 134 us at 8192 x 1280 x 10240; without spills (eight waves of 32 x 64) 44.7 against 41.6 us at
+// 1024 x 5120 x 1280.  8192 x 320 x 2560 (three blocks a tile): 24 us, 42 MB of stores.
 template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int S>
 struct GemmF8 {
   static constexpr int NWM = BM / WM, NWN = BN / WN, NW = NWM * NWN;
@@ -566,7 +573,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_gemm_f8(GemmF
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   gemm_f8<BM, BN, WM, WN, YDT, SBROW, S>(p, smem, blockIdx.x, gridDim.x, xcd_tile_id());
 }
-// a weight gradient's slices (the longer workgroups, first) and the other gradient's tiles in one launch: either alone leaves CUs idle
+// a weight gradient's slices (the longer workgroups, first) and the other gradient's tiles in one launch: either alone leaves CUs idle.  8192 x 640 x 640
+// bf16: 22 us (the weight's alone 17.7); eight waves and four stages (one workgroup a CU, every fragment widened twice) 30.
 template <int YDT>
 __global__ __launch_bounds__(256, 2) void k_gemm_f8_grads(GemmF8P gw, GemmF8P gx, int nw) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -575,7 +583,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f8_grads(GemmF8P gw, GemmF8P gx
   else gemm_f8<128, 128, 64, 64, YDT, false, 2>(gx, smem, q - nw, gridDim.x - nw, q - nw);
 }
 
-// slices of the K axis, added in order; four outputs a thread
+// slices of the K axis, added in order; four outputs a thread (640 x 640, ten slices: 4.5 us)
 __global__ __launch_bounds__(256) void k_sum_slices(const float* __restrict__ part, float* __restrict__ y, long n, int nslice) {
   const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (i >= n) return;
@@ -661,7 +669,8 @@ int launch_quant_rows(tfmq_handle h, const void* x, int dtype, long M, int K, lo
 
 // ---- few rows (M <= 32 a workgroup): one launch, W read once straight into the fragments, the activations quantised on the way in.  Eight waves
 // share the K blocks of 32 columns; a lane holds row j's elements [32 hh, +32) of each 64-channel half of a block, so a block's largest magnitude
-// is 64 values and one exchange between the two half waves.  The partial sums meet in LDS in the waves' order (no atomics).
+// is 64 values and one exchange between the two half waves.  The partial sums meet in LDS in the waves' order (no atomics).  Bound by two dependent trips to
+// memory per wave and launch: 2 x 1280 x 1280 4.9 us, 154 x 768 x 1280 4.9, 32 x 1280 x 10240 9.7 (1.4 TB/s of W).
 struct SmallF8P {
   const void* x;
   long ld;
@@ -793,7 +802,8 @@ int launch_product(tfmq_handle h, const GemmF8P& p, int y_dtype, hipStream_t st)
     return y_dtype == DT_F16 ? launch_gemm<256, 256, 128, 64, DT_F16, false, 2>(h, p, st) : launch_gemm<256, 256, 128, 64, DT_BF16, false, 2>(h, p, st);
   return y_dtype == DT_F16 ? launch_128<DT_F16, false>(h, p, st) : launch_128<DT_BF16, false>(h, p, st);
 }
-// slices of the token axis of a weight gradient [N][K]: its tiles alone leave CUs idle, every slice costs a write and a read of the result in fp32
+// slices of the token axis of a weight gradient [N][K]: its tiles alone leave CUs idle, every slice costs a write and a read of the result in fp32.
+// 8192 x 640 x 640 (25 tiles): one slice 305 us, ten (one workgroup a CU) 22 with the other gradient, twice and three times as many slower again.
 int grad_slices(tfmq_handle h, long M, int N, int K) {
   const long nt = static_cast<long>(ceil_div(N, 128)) * ceil_div(K, 128), Mb = (M + 127) / 128;
   const long n = h->cu_count / nt;

@@ -1804,8 +1804,6 @@ class PackedFp8:
     def __init__(self, q, qt, scale, bias, N, K):
         self.q, self.qt, self.scale, self.bias, self.N, self.K = q, qt, scale, bias, N, K
         self.Kb = scale.shape[1]
-        # addresses of this object's own tensors, which never change
-        self._q, self._qt, self._scale, self._bias = q.data_ptr(), qt.data_ptr(), scale.data_ptr(), None if bias is None else bias.data_ptr()
 
 
 def quantize_fp8(x: torch.Tensor) -> QuantFp8:
@@ -1902,7 +1900,8 @@ def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> tor
     nb = 0 if quantised else h.lib.tfmq_linear_fp8_ws_bytes(h.h, M, pw.N, pw.K)
     ws = _alloc(nb, dtype=torch.uint8, device=src.device) if nb else None
     xp, qp, sp = (None, src.data_ptr(), x.scale.data_ptr()) if quantised else (x.data_ptr(), None, None)
-    h.call("linear_fp8", xp, dt, M, pw.K, ld, qp, sp, pw._q, pw._scale, pw.Kb, 1, pw._bias, y.data_ptr(), _DT_CODE[out_dtype], pw.N,
+    b = None if pw.bias is None else pw.bias.data_ptr()
+    h.call("linear_fp8", xp, dt, M, pw.K, ld, qp, sp, pw.q.data_ptr(), pw.scale.data_ptr(), pw.Kb, 1, b, y.data_ptr(), _DT_CODE[out_dtype], pw.N,
            None if ws is None else ws.data_ptr(), _stream(d))
     return y
 
@@ -1928,7 +1927,7 @@ def linear_fp8_bwd(x: torch.Tensor, gy: torch.Tensor, pw: PackedFp8, want_gx: bo
         h = handle(d)
         nb = h.lib.tfmq_linear_fp8_bwd_ws_bytes(h.h, M, pw.N, pw.K, int(want_gx), int(want_gw))
         ws = _alloc(nb, dtype=torch.uint8, device=gy.device) if nb else None
-        h.call("linear_fp8_bwd", x.data_ptr(), dx, ldx, gy.data_ptr(), dg, ldg, M, pw.N, pw.K, pw._qt, pw._scale, None if gx is None else gx.data_ptr(),
+        h.call("linear_fp8_bwd", x.data_ptr(), dx, ldx, gy.data_ptr(), dg, ldg, M, pw.N, pw.K, pw.qt.data_ptr(), pw.scale.data_ptr(), None if gx is None else gx.data_ptr(),
                None if gw is None else gw.data_ptr(), None if ws is None else ws.data_ptr(), _stream(d))
     return gx, gw
 
