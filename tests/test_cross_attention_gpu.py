@@ -350,3 +350,19 @@ def test_two_captured_graphs_and_eager_work(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out1, want1[i])), i
         assert all(torch.equal(a, b) for a, b in zip(out2, want2[i])), i
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Tq,Tk,H,G,d", [(1709, 18, 4, 4, 160), (64, 7, 8, 2, 40), (300, 33, 4, 4, 64), (5, 2, 16, 4, 80)])
+def test_few_states_lose_only_the_roundings(ops, Tq, Tk, H, G, d, dt):
+    """Few kept states leave ds = p (dp - D) small against D.  dq and dk round twice, the ds operand and the result: a rounding's error is at most uniform
+    over half a step of eps |x|, rms eps / (2 sqrt 3) of the value, two independent ones sqrt 2 of that (the sum over channels or rows does not add: its
+    terms' errors are as independent as its terms)."""
+    q, k, v, go = _mk(2, Tq, Tk, H, G, d, dt, Tk)
+    lens = torch.tensor([Tk, max(1, Tk // 2)], dtype=torch.int32)
+    mask = torch.rand(2, Tk, generator=torch.Generator().manual_seed(Tk)) < 0.6
+    mask[:, 0] = True
+    o, lse, dq, dk, dv = _run(ops, q, k, v, go, H, d ** -0.5, G, None, lens, mask)
+    R, _ = _ref(q, k, v, H, d ** -0.5, G, None, lens, mask, go=go)
+    for n, t in (("dq", dq), ("dk", dk)):
+        assert float((t.double().cpu() - R[n]).norm() / R[n].norm()) <= 2 ** 0.5 * torch.finfo(dt).eps / (2 * 3 ** 0.5), n

@@ -169,9 +169,12 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
   for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, acc[t], f);
 }
 
-// ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form).  8 x 4096 x 77, 8 heads of 40:
-// 25 us for 84 MB of q, o, go and dq (3.4 TB/s).
-constexpr int dq_short_waves(int D, int NKT) { return D <= 64 ? 4 : D <= 96 ? 3 : 2; }
+// ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form).  A row's probabilities and dp all
+// stay in registers and D is their own sum of p dp.  From o, which the forward has rounded, D is off by that rounding, and few states leave
+// ds = p (dp - D) small against D: bf16 gradients of q and k at 18 states, of which a mask and lengths kept about three, were 1.9 times as far from the exact
+// ones as from one rounding, now 1.4 (the ds operand's and the result's).  8 x 4096 x 77, 8 heads of 40: 24 us for 63 MB of q, go and dq; reading o
+// instead of holding the scores, at four waves a SIMD against three, 25.
+constexpr int dq_short_waves(int D, int NKT) { return D <= 64 && NKT <= 2 ? 4 : NKT <= (D <= 32 ? 4 : D <= 64 ? 3 : D <= 96 ? 2 : 0) ? 3 : 2; }
 template <typename T, int D, int NKT>
 __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(XattnP p) {
   constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_both(D), VS = stride_rows(D), NK = NKT * 32;
@@ -188,15 +191,14 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
   const long brow0 = (static_cast<long>(b) * p.H + g * p.rep) * p.Tq, rows = static_cast<long>(p.B) * p.H * p.Tq;
   const Rsrc rq = buffer_of(static_cast<const T*>(p.q.p) + b * p.q.bs + hc, ((p.Tq - 1) * p.q.ts + rd) * 2);
   const Rsrc rg = buffer_of(static_cast<const T*>(p.go.p) + b * p.go.bs + hc, ((p.Tq - 1) * p.go.ts + rd) * 2);
-  const Rsrc ro = buffer_of(static_cast<const T*>(p.o.p) + b * p.o.bs + hc, ((p.Tq - 1) * p.o.ts + rd) * 2);
   const Rsrc ry = buffer_of(static_cast<T*>(p.y) + b * p.Tq * C + hc, (p.Tq * C - hc) * 2);
   const Rsrc rl = buffer_of(p.lse_in + brow0, p.R * 4), rdl = buffer_of(p.delta + brow0, p.R * 4), rgm = buffer_of(p.delta + rows + brow0, p.R * 4);
-  const unsigned qts = static_cast<unsigned>(p.q.ts) * 2, gts = static_cast<unsigned>(p.go.ts) * 2, ots = static_cast<unsigned>(p.o.ts) * 2;
+  const unsigned qts = static_cast<unsigned>(p.q.ts) * 2, gts = static_cast<unsigned>(p.go.ts) * 2;
   const unsigned yts = static_cast<unsigned>(C) * 2, hs = static_cast<unsigned>(p.d) * 2;
 
   const long r_end = min(p.R, (static_cast<long>(rb) + 1) * p.rows_per);
   RowWalk w(static_cast<long>(rb) * p.rows_per + wid * 32 + j, p.Tq);
-  V8 qf[NKS], gf[NKS], of[NKS];
+  V8 qf[NKS], gf[NKS];
   float lse = 0.0f;
   auto load_rows = [&]() {
     const bool ok = w.row < r_end && w.i < qlen;
@@ -207,7 +209,6 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
       const unsigned col = w.hi * hs + c * 2;
       qf[ks] = load8<V8>(rq, there ? w.i * qts + col : NOWHERE);
       gf[ks] = load8<V8>(rg, there ? w.i * gts + col : NOWHERE);
-      of[ks] = load8<V8>(ro, there ? w.i * ots + col : NOWHERE);
     }
     lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, static_cast<int>(ok ? static_cast<unsigned>(w.row) * 4 : NOWHERE), 0, 0));
   };
@@ -218,24 +219,20 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
     const bool in = w.row < r_end, ok = in && w.i < qlen;
     const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
     float dl = 0.0f, gm = 0.0f;
+    if (is_f16<T>()) {
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks)
+      for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = static_cast<float>(gf[ks][e]);
-        dl = __builtin_fmaf(static_cast<float>(of[ks][e]), x, dl);
-        if (is_f16<T>()) gm = fmaxf(gm, fabsf(x));
-      }
-    dl += __shfl_xor(dl, 32, 64);
+        for (int e = 0; e < 8; ++e) gm = fmaxf(gm, fabsf(static_cast<float>(gf[ks][e])));
+    }
     gm = fmaxf(gm, __shfl_xor(gm, 32, 64));
     const int fe = is_f16<T>() ? inv_exponent(gm) : 0;
     const float sh = (ok && lse != -INFINITY ? lse * LOG2E : INFINITY) - static_cast<float>(fe);
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), rdl, static_cast<int>(loff), 0, 0);
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(gm), rgm, static_cast<int>(loff), 0, 0);
     V8 df[2 * NKT];
+    v16f ps[NKT], dps[NKT];
 #pragma unroll
     for (int kt = 0; kt < NKT; ++kt) {
-      hold_order();                      // (one key tile's scores at a time: all of them at once would spill)
+      hold_order();                      // (one key tile's operands at a time)
       v16f s = start_scores(sB + kt * 32, hh), dp = zero16();
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) {
@@ -243,10 +240,25 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
         dp = mfma16(frag_rows<T>(sV, VS, kt * 32 + j, ks, hh), gf[ks], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -sh)) * (dp[r] - dl);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) df[2 * kt + u] = frag_regs<T>(s, u);
+      for (int r = 0; r < 16; ++r) {
+        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -sh));
+        dl = __builtin_fmaf(pr, dp[r], dl);
+        s[r] = pr;
+      }
+      ps[kt] = s;
+      dps[kt] = dp;
     }
+    dl += __shfl_xor(dl, 32, 64);
+    dl *= __builtin_amdgcn_exp2f(static_cast<float>(-fe));          // (p carries 2^fe)
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ps[kt][r] *= dps[kt][r] - dl;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) df[2 * kt + u] = frag_regs<T>(ps[kt], u);
+    }
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), rdl, static_cast<int>(loff), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(gm), rgm, static_cast<int>(loff), 0, 0);
     hold_order();
     w.step();
     load_rows();
