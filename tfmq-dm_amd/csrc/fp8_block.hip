@@ -450,7 +450,10 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
 #pragma unroll
       for (int u = 0; u < TN; ++u) {
         const v16f z = {};
+        // (a wave that has its operands goes first: 8192 x 1280 x 10240 135 -> 131 us.  With two workgroups a CU it gains nothing, the gradients' launch loses 2)
+        if constexpr (BM == 256) __builtin_amdgcn_s_setprio(1);
         const v16f d = F::mul(wf[u][1], xf[1], F::mul(wf[u][0], xf[0], z));
+        if constexpr (BM == 256) __builtin_amdgcn_s_setprio(0);
         if constexpr (SBROW) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[u][t][r] = __builtin_fmaf(d[r], sx[t] * swr[u][r], acc[u][t][r]);
