@@ -121,3 +121,39 @@ def test_refusals(run, golden):
     fp.prepare()
     with pytest.raises(TfmqError, match="context_mask"):
         fp.forward(x, t, ctx, context_mask=ok)
+
+
+@pytest.mark.parametrize("kind", ["GraphLatentDdimSampler", "GraphLatentPlmsSampler"])
+@pytest.mark.parametrize("pair", ["0", "1"])
+def test_captured_samplers_take_masks(run, kind, pair, monkeypatch):
+    """Samples of prompts of three tokens, padded to five and masked, equal the samples of the three alone; the masks change between runs of one
+    captured sampler; without masks every token counts."""
+    from tfmq_dm_amd._lib import TfmqError
+    from tfmq_dm_amd.ldm import sampler as S
+    monkeypatch.setenv("TFMQ_PAIR_PREFIX", pair)
+    eng, x, t, ctx = run
+    B, L = ctx.shape[:2]
+    cls, n = getattr(S, kind), L - 2
+    uc = ctx.flip(0) * 0.5
+    xT = torch.randn(x.shape, generator=torch.Generator().manual_seed(3)).to(DEV)
+    ac = S.alphas_cumprod_linear()
+
+    def sample(smp, *a, **k):
+        out = smp.sample_nhwc(xT, *a, **k)
+        smp.stream.synchronize()
+        return out.clone()
+    padded = cls(eng, 4, B, (4, 8, 8), (L, ctx.shape[2]), scale=7.5, alphas_cumprod=ac, context_masks=True).capture()
+    junk = lambda c: torch.cat([c[:, :n], torch.full_like(c[:, n:], 9.0)], 1)      # noqa: E731
+    m = lengths(ctx, *[n] * B)
+    every = sample(padded, ctx, uc)
+    a = sample(padded, junk(ctx), junk(uc), cond_mask=m, uncond_mask=m)
+    assert torch.equal(sample(padded, ctx, uc), every) and not torch.equal(a, every)
+    short = cls(eng, 4, B, (4, 8, 8), (n, ctx.shape[2]), scale=7.5, alphas_cumprod=ac, context_masks=True).capture()
+    assert torch.equal(sample(short, ctx[:, :n], uc[:, :n]), a)
+    for bad in (m.float(), m[:, :-1]):
+        with pytest.raises(TfmqError, match="mask"):
+            padded.sample_nhwc(xT, ctx, uc, cond_mask=bad)
+    plain = cls(eng, 4, B, (4, 8, 8), (L, ctx.shape[2]), scale=7.5, alphas_cumprod=ac)
+    with pytest.raises(TfmqError, match="context_masks"):
+        plain.sample_nhwc(xT, ctx, uc, cond_mask=m)
+    assert rel_l2(every, sample(plain, ctx, uc)) <= 8e-2      # (the bar of a guided four-step trajectory: guidance amplifies a step's 3e-2)

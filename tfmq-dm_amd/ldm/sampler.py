@@ -48,8 +48,11 @@ def ddim_coef_table(alphas_cumprod: torch.Tensor, S: int, eta: float = 0.0) -> t
 
 
 class GraphLatentDdimSampler:
+    """context_masks: sample_nhwc takes a mask per context row (cond_mask / uncond_mask, bool [B, L], True: attend; None: all tokens), for
+    prompts of different lengths in one batch (LdmUNetEngine.forward's context_mask)."""
+
     def __init__(self, engine, S: int, batch: int, latent_shape, context_shape, scale: float = 7.5,
-                 alphas_cumprod: Optional[torch.Tensor] = None, eta: float = 0.0):
+                 alphas_cumprod: Optional[torch.Tensor] = None, eta: float = 0.0, context_masks: bool = False):
         self.eng, self.S, self.batch, self.scale = engine, S, batch, float(scale)
         self.eta = float(eta)
         self.dev = engine.dev
@@ -71,6 +74,9 @@ class GraphLatentDdimSampler:
         self.uncond = context_shape is None
         self.x2 = None if self.uncond else torch.empty(2 * batch, H, W, Cc, device=self.dev)
         self.ctx2 = None if self.uncond else torch.empty((2 * batch,) + tuple(context_shape), device=self.dev)
+        if context_masks and self.uncond:
+            raise TfmqError(f"{type(self).__name__}: context_masks need a context")
+        self.mask2 = torch.ones((2 * batch, context_shape[0]), dtype=torch.bool, device=self.dev) if context_masks else None
         self.pair_prefix = (not self.uncond) and os.environ.get("TFMQ_PAIR_PREFIX", "1") != "0" and hasattr(engine, "_dup")
         self.stream = torch.cuda.Stream(self.dev)
         self.arena = ops.Arena()
@@ -93,10 +99,33 @@ class GraphLatentDdimSampler:
         -- everything in front of the first cross attention -- once (`pair_prefix`, TFMQ_PAIR_PREFIX=0: the materialised 2B batch)."""
         B = self.batch
         if self.pair_prefix:
-            return self.eng.forward(xin, None, self.ctx2, pair_prefix=True)
+            return self.eng.forward(xin, None, self.ctx2, pair_prefix=True, **self._masks())
         self.x2[:B].copy_(xin)
         self.x2[B:].copy_(xin)
-        return self.eng.forward(self.x2, None, self.ctx2)
+        return self.eng.forward(self.x2, None, self.ctx2, **self._masks())
+
+    def _masks(self):
+        return {} if self.mask2 is None else {"context_mask": self.mask2}
+
+    def _check_masks(self, *masks):
+        for m in masks:
+            if m is not None and self.mask2 is None:
+                raise TfmqError(f"{type(self).__name__}: masks need context_masks=True at construction")
+            if m is not None and (m.dtype != torch.bool or tuple(m.shape) != (self.batch, self.mask2.shape[1])):
+                raise TfmqError(f"{type(self).__name__}: a mask must be bool [{self.batch}, {self.mask2.shape[1]}], got {m.dtype} {tuple(m.shape)}")
+
+    def _set_context(self, cond, uncond, cond_mask, uncond_mask):
+        """c_in = cat[uc, c] (ddim.py:183) and its masks into the buffers that the captured steps read."""
+        for half, c, m in ((slice(0, self.batch), uncond, uncond_mask), (slice(self.batch, None), cond, cond_mask)):
+            self.ctx2[half].copy_(c, non_blocking=True)
+            if self.mask2 is None:
+                continue
+            if m is None:
+                self.mask2[half].fill_(True)
+            else:
+                self.mask2[half].copy_(m, non_blocking=True)
+                if m.is_cuda:
+                    m.record_stream(self.stream)
 
     def capture(self):
         sp = C.c_void_p(self.stream.cuda_stream)
@@ -131,9 +160,10 @@ class GraphLatentDdimSampler:
         return self
 
     def sample_nhwc(self, x_T: torch.Tensor, cond: Optional[torch.Tensor] = None, uncond: Optional[torch.Tensor] = None,
-                    steps: Optional[int] = None):
+                    steps: Optional[int] = None, cond_mask: Optional[torch.Tensor] = None, uncond_mask: Optional[torch.Tensor] = None):
         """x_T [B,H,W,C]; cond/uncond [B,L,D] (CLIP / class embeddings: glue, computed elsewhere; None for an
         unconditional sampler)."""
+        self._check_masks(cond_mask, uncond_mask)
         if self.gid is None:
             self.capture()
         sp = C.c_void_p(self.stream.cuda_stream)
@@ -141,8 +171,7 @@ class GraphLatentDdimSampler:
         with torch.cuda.stream(self.stream):
             self.x.copy_(x_T, non_blocking=True)
             if not self.uncond:
-                self.ctx2[:self.batch].copy_(uncond, non_blocking=True)   # c_in = cat[uc, c]  (ddim.py:183)
-                self.ctx2[self.batch:].copy_(cond, non_blocking=True)
+                self._set_context(cond, uncond, cond_mask, uncond_mask)
             self.step.zero_()
             # at most 8 step graphs (~10 k kernel dispatches) are enqueued ahead of the GPU: an unbounded run-ahead of
             # the host buys nothing and overflows rocprofv3's dispatch records at large batches
@@ -156,7 +185,7 @@ class GraphLatentDdimSampler:
         if fp16_stream_overflowed(self, lambda: (self.eng.forward(x_T.float().contiguous(), None, None) if self.uncond
                                                  else self._eps_pair(x_T.float().contiguous())),
                                   lambda: (self.eng.forward(self.x.float().clone(), None, None) if self.uncond else self._eps_pair(self.x.float().clone()))):
-            return self.sample_nhwc(x_T, cond, uncond, steps)
+            return self.sample_nhwc(x_T, cond, uncond, steps, cond_mask, uncond_mask)
         return self.x
 
 
@@ -175,8 +204,8 @@ class GraphLatentPlmsSampler(GraphLatentDdimSampler):
     counter, which equals DiffusionWrapper's k = t_max - (t-1)//tot for t and for t_next alike."""
 
     def __init__(self, engine, S: int, batch: int, latent_shape, context_shape, scale: float = 7.5,
-                 alphas_cumprod: Optional[torch.Tensor] = None):
-        super().__init__(engine, S, batch, latent_shape, context_shape, scale, alphas_cumprod, 0.0)
+                 alphas_cumprod: Optional[torch.Tensor] = None, context_masks: bool = False):
+        super().__init__(engine, S, batch, latent_shape, context_shape, scale, alphas_cumprod, 0.0, context_masks)
         if self.coef.shape[0] < 2:
             raise TfmqError("GraphLatentPlmsSampler needs at least two steps")
         mk = lambda: torch.empty_like(self.x)
@@ -243,8 +272,10 @@ class GraphLatentPlmsSampler(GraphLatentDdimSampler):
             self.gid = gids[0]
         return self
 
-    def sample_nhwc(self, x_T: torch.Tensor, cond: torch.Tensor, uncond: torch.Tensor, steps: Optional[int] = None):
+    def sample_nhwc(self, x_T: torch.Tensor, cond: torch.Tensor, uncond: torch.Tensor, steps: Optional[int] = None,
+                    cond_mask: Optional[torch.Tensor] = None, uncond_mask: Optional[torch.Tensor] = None):
         """steps: run only the first `steps` iterations (untill_fake_t - 1 of the drop-in)."""
+        self._check_masks(cond_mask, uncond_mask)
         if self.gids is None:
             self.capture()
         sp = C.c_void_p(self.stream.cuda_stream)
@@ -252,8 +283,7 @@ class GraphLatentPlmsSampler(GraphLatentDdimSampler):
         self.stream.wait_stream(torch.cuda.current_stream(self.dev))      # inputs / set-up produced on the caller's stream
         with torch.cuda.stream(self.stream):
             self.x.copy_(x_T, non_blocking=True)
-            self.ctx2[:self.batch].copy_(uncond, non_blocking=True)
-            self.ctx2[self.batch:].copy_(cond, non_blocking=True)
+            self._set_context(cond, uncond, cond_mask, uncond_mask)
             self.step.zero_()
             sync_every = int(os.environ.get("TFMQ_GRAPH_SYNC_EVERY", "8"))
             for i in range(n):
@@ -263,5 +293,5 @@ class GraphLatentPlmsSampler(GraphLatentDdimSampler):
         if fp16_stream_overflowed(self, lambda: (self.eng.forward(x_T.float().contiguous(), None, None) if self.uncond
                                                  else self._eps_pair(x_T.float().contiguous())),
                                   lambda: (self.eng.forward(self.x.float().clone(), None, None) if self.uncond else self._eps_pair(self.x.float().clone()))):
-            return self.sample_nhwc(x_T, cond, uncond, steps)
+            return self.sample_nhwc(x_T, cond, uncond, steps, cond_mask, uncond_mask)
         return self.x
