@@ -62,3 +62,17 @@ def test_operands_of_two_devices_are_refused(monkeypatch, ops):
     monkeypatch.setattr(ops, "_dev", lambda t: 1 if t.dtype == torch.uint8 else 0)
     with pytest.raises(ops.TfmqError, match="cuda:1"):
         ops.linear_fp8(torch.zeros(4, 40), _pw(ops))
+
+
+def test_operands_of_the_wrong_form_are_refused(ops):
+    from tfmq_dm_amd._lib import TfmqError
+    u8, f32 = (lambda *s: torch.zeros(*s, dtype=torch.uint8)), (lambda *s: torch.zeros(*s))      # noqa: E731
+    ops.QuantFp8(u8(6, 256), f32(2, 6), (2, 3, 200), torch.float16)
+    for q, s in ((u8(5, 256), f32(2, 6)), (u8(6, 128), f32(2, 6)), (u8(6, 256), f32(6, 2)), (u8(6, 256), f32(2, 6).double()), (u8(6, 256).t().contiguous().t(), f32(2, 6))):
+        with pytest.raises(TfmqError, match="QuantFp8"):
+            ops.QuantFp8(q, s, (2, 3, 200), torch.float16)
+    ops.PackedFp8(u8(130, 256), u8(200, 256), f32(2, 2), f32(130), 130, 200)
+    for q, qt, s, b in ((u8(130, 200), u8(200, 256), f32(2, 2), None), (u8(130, 256), u8(256, 200), f32(2, 2), None), (u8(130, 256), u8(200, 256), f32(2, 1), None),
+                        (u8(130, 256), u8(200, 256), f32(2, 2), f32(129))):
+        with pytest.raises(TfmqError, match="PackedFp8"):
+            ops.PackedFp8(q, qt, s, b, 130, 200)

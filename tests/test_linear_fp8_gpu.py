@@ -244,3 +244,13 @@ def test_a_copied_weight_is_its_own(ops):
         t.zero_()
     assert torch.equal(ops.linear_fp8(x, other), y) and not ops.linear_fp8(x, pw).any()
     assert torch.equal(ops.linear_fp8_bwd(x, _x(40, 200, torch.float16, 3).to(DEV), other)[0], g[0])
+
+
+def test_stored_weights_of_other_layouts(ops):
+    """load_w_fp8 takes bytes and scales in any strides."""
+    x = _x(40, 300, torch.float16).to(DEV)
+    pw = ops.pack_w_fp8(_x(200, 300, torch.float32, 1).to(DEV))
+    q = pw.q[:, :300].view(torch.float8_e4m3fn)
+    turned = ops.load_w_fp8(q.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn), pw.scale.t().contiguous().t())
+    assert torch.equal(turned.q, pw.q) and torch.equal(turned.qt, pw.qt) and torch.equal(turned.scale, pw.scale)
+    assert torch.equal(ops.linear_fp8(x, turned), ops.linear_fp8(x, pw))

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import contextvars
+import math
 import os
 import struct
 from typing import Optional, Tuple
@@ -1788,11 +1789,22 @@ def _same_device(d: int, *tensors):
             raise TfmqError(f"operands on cuda:{_dev(t)} and cuda:{d} in one call")
 
 
+def _operand(t: torch.Tensor, dtype, shape, name: str, what: str):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise TfmqError(f"{name} {what}: expected contiguous {dtype} {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
 class QuantFp8:
     """Activations in e4m3 with one fp32 scale per row and block of 128 channels (quantize_fp8).  q: uint8 [M, 128 * ceil(K / 128)] (the e4m3
     bytes, zero padded), scale: fp32 [ceil(K / 128), M]; the value of (m, k) is q[m, k] * scale[k // 128, m]."""
 
     def __init__(self, q, scale, shape, dtype):
+        K = shape[-1]
+        M, Kb = math.prod(shape[:-1]), (K + 127) // 128
+        _operand(q, torch.uint8, (M, Kb * 128), "QuantFp8", "q")
+        _operand(scale, torch.float32, (Kb, M), "QuantFp8", "scale")
+        if scale.device != q.device:
+            raise TfmqError("QuantFp8: q and scale on different devices")
         self.q, self.scale, self.shape, self.dtype = q, scale, tuple(shape), dtype
 
 
@@ -1802,6 +1814,14 @@ class PackedFp8:
     ceil(K / 128)]; bias fp32 [N] or None."""
 
     def __init__(self, q, qt, scale, bias, N, K):
+        Nb, Kb = (N + 127) // 128, (K + 127) // 128
+        _operand(q, torch.uint8, (N, Kb * 128), "PackedFp8", "q")
+        _operand(qt, torch.uint8, (K, Nb * 128), "PackedFp8", "qt")
+        _operand(scale, torch.float32, (Nb, Kb), "PackedFp8", "scale")
+        if bias is not None:
+            _operand(bias, torch.float32, (N,), "PackedFp8", "bias")
+        if any(t is not None and t.device != q.device for t in (qt, scale, bias)):
+            raise TfmqError("PackedFp8: its tensors lie on different devices")
         self.q, self.qt, self.scale, self.bias, self.N, self.K = q, qt, scale, bias, N, K
         self.Kb = scale.shape[1]
 
@@ -1873,7 +1893,7 @@ def load_w_fp8(q: torch.Tensor, scale: torch.Tensor, bias: Optional[torch.Tensor
     qt = torch.zeros(K, Nb * 128, dtype=torch.uint8, device=q.device)
     q8[:, :K].copy_(b)
     qt[:, :N].copy_(b.t())
-    return PackedFp8(q8, qt, scale.detach().clone(), _bias_f32(bias, N, d, "load_w_fp8"), N, K)
+    return PackedFp8(q8, qt, scale.detach().clone(memory_format=torch.contiguous_format), _bias_f32(bias, N, d, "load_w_fp8"), N, K)
 
 
 def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
