@@ -1,4 +1,5 @@
-// Gradients of the cross attention (attention_cross_fwd.hip): with p_ij = exp(scale q_i k_j - lse_i), dp_ij = go_i v_j and D_i = sum_c o_ic go_ic,
+// Gradients of the cross attention (attention_cross_fwd.hip): with p_ij = exp(scale q_i k_j - lse_i), dp_ij = go_i v_j and
+// D_i = sum_c o_ic go_ic = sum_j p_ij dp_ij,
 //     ds_ij = p_ij (dp_ij - D_i),   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij go_i.
 //
 // Two kernels recompute p from the saved lse, each with its sums in registers and no atomics: k_xattn_dq walks the keys of 128 rows (a lane owns a row,
@@ -520,7 +521,7 @@ int launch_bwd(tfmq_handle h, XattnP p, hipStream_t st) {
     auto kk = &k_xattn_dkv<T, D>;
     constexpr int sk = 2 * dkv_rows<D>() * (stride_both(D) + 4) + 16;
     static LdsRoom room_kk;
-  TFMQ_HIP(h, room_kk.ask(h, reinterpret_cast<const void*>(kk), sk));
+    TFMQ_HIP(h, room_kk.ask(h, reinterpret_cast<const void*>(kk), sk));
     const int rc = launch_dq<T, D>(h, p, st);
     if (rc != TFMQ_OK) return rc;
     XattnP c = p;

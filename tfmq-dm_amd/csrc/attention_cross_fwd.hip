@@ -309,7 +309,7 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
     auto kern = &k_xattn_fwd<T, D>;
     constexpr int smem = 64 * (stride_rows(D) + stride_cols(D));
     static LdsRoom room_kern;
-  TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
+    TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
     p.nrb = ceil_div(p.R, 128);
     const long nb = static_cast<long>(p.B) * p.G * p.nrb * p.nsplit;
     TFMQ_CHECK_ARG(h, nb < (1L << 31), "xattn_fwd: too many workgroups");
