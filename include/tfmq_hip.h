@@ -620,9 +620,9 @@ int tfmq_quantize_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, lo
 int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint8_t* q, uint8_t* qt, float* s, void* stream);
 /* y[m][n] = sum_kb sx[kb][m] sw(n / 128, kb) (sum_{k in kb} qx[m][k] qw[n][k]) + bias[n], y [M][N] contiguous of y_dtype (16-byte aligned), fp32 sums.
  * x [M][K] of dtype, row stride ld, is quantised here; or x = NULL and xq / xs as tfmq_quantize_fp8 leaves them.  w as tfmq_pack_w_fp8 leaves it; the
- * scale of (column block nb, k block kb) at ws[nb * ws_n + kb * ws_k].  work: tfmq_linear_fp8_ws_bytes (0 where one launch
- * does it: up to 32 rows, or few outputs). */
-size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K);
+ * scale of (column block nb, k block kb) at ws[nb * ws_n + kb * ws_k].  work: tfmq_linear_fp8_ws_bytes, quantised != 0 for
+ * xq / xs (may be 0: then work may be NULL). */
+size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K, int quantised);
 int tfmq_linear_fp8(tfmq_handle h, const void* x, int dtype, long M, int K, long ld, const uint8_t* xq, const float* xs, const uint8_t* w,
                     const float* ws, long ws_n, long ws_k, const float* bias, void* y, int y_dtype, int N, void* work, void* stream);
 /* gx [M][K] (of gy's type) = product of gy, quantised by rows, with the transposed weight wt (tfmq_pack_w_fp8's qt; ws its s [ceil(N / 128)][Kb]);

@@ -254,3 +254,20 @@ def test_stored_weights_of_other_layouts(ops):
     turned = ops.load_w_fp8(q.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn), pw.scale.t().contiguous().t())
     assert torch.equal(turned.q, pw.q) and torch.equal(turned.qt, pw.qt) and torch.equal(turned.scale, pw.scale)
     assert torch.equal(ops.linear_fp8(x, turned), ops.linear_fp8(x, pw))
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("M,K,N", [(600, 2600, 333), (900, 2600, 333), (400, 5120, 640), (257, 3900, 1001)])
+def test_slices_of_a_long_reduction(ops, M, K, N, out):
+    """Few tiles under a long K axis: its slices' fp32 sums and the bias are added before the one rounding (bound: the sum over the blocks has the same
+    additions in another order, and one more per slice, within the 128 of a block counted twice)."""
+    h = ops.handle(0)
+    sliced = M != 600          # (there one launch of small tiles does it)
+    assert (h.lib.tfmq_linear_fp8_ws_bytes(h.h, M, N, K, 1) > 0) == sliced          # (only slices need room for operands that are quantised already)
+    x, w, b = _x(M, K, torch.float16), _x(N, K, torch.float32, 1), torch.randn(N, generator=torch.Generator().manual_seed(5))
+    pw = ops.pack_w_fp8(w.to(DEV), b.to(DEV))
+    y = ops.linear_fp8(x.to(DEV), pw, out)
+    assert y.dtype == out and (not sliced or torch.equal(y, ops.linear_fp8(ops.quantize_fp8(x.to(DEV)), pw, out)))
+    qx, qw = O.dequant(*O.quant_rows(x)), O.dequant(*O.quant(w, 128))
+    A = _terms(qx, qw)
+    _check(y, qx @ qw.t() + b.double(), (A[0] + b.double().abs(), A[1]), (K + 127) // 128 + 1, out)

@@ -201,7 +201,7 @@ _SIGS = {
     "tfmq_fisher_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_int, c_size_t, c_void_p, c_void_p, c_void_p]),
     "tfmq_quantize_fp8": (c_int, [c_void_p, c_void_p, c_int, C.c_long, c_int, C.c_long, c_int, c_void_p, c_void_p, c_void_p]),
     "tfmq_pack_w_fp8": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "tfmq_linear_fp8_ws_bytes": (c_size_t, [c_void_p, C.c_long, c_int, c_int]),
+    "tfmq_linear_fp8_ws_bytes": (c_size_t, [c_void_p, C.c_long, c_int, c_int, c_int]),
     "tfmq_linear_fp8": (c_int, [c_void_p, c_void_p, c_int, C.c_long, c_int, C.c_long, c_void_p, c_void_p, c_void_p, c_void_p, C.c_long, C.c_long, c_void_p,
                                 c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "tfmq_linear_fp8_bwd_ws_bytes": (c_size_t, [c_void_p, C.c_long, c_int, c_int, c_int, c_int]),

@@ -12,6 +12,7 @@
 // it.  fp32 outputs (a weight's gradient among them) do not: their fragments are widened in registers to fp16, which holds every e4m3 value,
 // and multiplied by v_mfma_f32_32x32x16_f16 (6e-9 in the same measurement), at half the matrix rate and two conversions per four bytes.
 #include "conv_common.hpp"
+#include <algorithm>
 #include <type_traits>
 
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -24,11 +25,12 @@ namespace {
 constexpr float F8_MAX = 448.0f;
 constexpr float AMAX_MIN = 7.888609052210118e-31f;      // 2^-100: keeps both the scale and its reciprocal normal numbers
 
-enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
+enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2, DT_PART = 3 };          // DT_PART: fp32 partial sums of a 16-bit result (its products)
 template <int DT> struct Elem;
 template <> struct Elem<DT_F32> { using type = float; };
 template <> struct Elem<DT_F16> { using type = _Float16; };
 template <> struct Elem<DT_BF16> { using type = __bf16; };
+template <> struct Elem<DT_PART> { using type = float; };
 
 // magnitudes compare as integers: a NaN is larger than an infinity, so the maximum carries it
 __device__ __forceinline__ unsigned mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -481,7 +483,7 @@ __device__ __forceinline__ void gemm_f8(const GemmF8P& p, unsigned char* smem, i
   for (int s = 0; s < S - 1; ++s) fetch_next(s);
   // waits for the oldest stage: what was issued behind it may be under way -- `ahead` - 1 stages and, for S - 1 blocks behind a tile whose stores are
   // known (every lane, whole lines), those
-  constexpr int NST = TM * TN * (YDT == DT_F32 ? 4 : 2);
+  constexpr int NST = TM * TN * static_cast<int>(sizeof(YT));
   static_assert((S - 2) * PER + NST < 64, "the counter's range");
   auto arrive = [&](bool stores) {
     if (stores) {
@@ -586,22 +588,33 @@ __global__ __launch_bounds__(256, 2) void k_gemm_f8_grads(GemmF8P gw, GemmF8P gx
   else gemm_f8<128, 128, 64, 64, YDT, false, 2>(gx, smem, q - nw, gridDim.x - nw, q - nw);
 }
 
-// slices of the K axis, added in order; four outputs a thread (640 x 640, ten slices: 4.5 us)
-__global__ __launch_bounds__(256) void k_sum_slices(const float* __restrict__ part, float* __restrict__ y, long n, int nslice) {
+// slices of the K axis, added in order (and the bias), rounded once; four outputs a thread (640 x 640 fp32, ten slices: 4.5 us)
+template <int YDT>
+__global__ __launch_bounds__(256) void k_sum_slices(const float* __restrict__ part, const float* __restrict__ bias, typename Elem<YDT>::type* __restrict__ y, long n, int N,
+                                                    int nslice) {
+  using YT = typename Elem<YDT>::type;
   const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (i >= n) return;
-  if (n % 4 == 0) {
+  if (n % 4 == 0 && N % 4 == 0) {
     float4 a = make_float4(0, 0, 0, 0);
     for (int s = 0; s < nslice; ++s) {
       const float4 v = *reinterpret_cast<const float4*>(part + s * n + i);
       a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
-    *reinterpret_cast<float4*>(y + i) = a;
+    if (bias) {
+      const int c = static_cast<int>(i % N);
+      a.x += bias[c]; a.y += bias[c + 1]; a.z += bias[c + 2]; a.w += bias[c + 3];
+    }
+    typedef YT v4t __attribute__((ext_vector_type(4)));
+    v4t o;
+    o[0] = static_cast<YT>(a.x); o[1] = static_cast<YT>(a.y); o[2] = static_cast<YT>(a.z); o[3] = static_cast<YT>(a.w);
+    *reinterpret_cast<v4t*>(y + i) = o;
   } else {
     for (long e = i; e < min(n, i + 4); ++e) {
       float a = 0.0f;
       for (int s = 0; s < nslice; ++s) a += part[s * n + e];
-      y[e] = a;
+      if (bias) a += bias[e % N];
+      y[e] = static_cast<YT>(a);
     }
   }
 }
@@ -796,10 +809,37 @@ bool big_tiles(tfmq_handle h, long M, int N) {
 // per CU -- from there the 128 x 128 tiles' reuse counts for more than their idle CUs.  us, one launch against two: 154 x 1280 x 1280 6.2 / 14.5,
 // 256 x 1280 x 1280 9.9 / 14.6, 256 x 5120 x 1280 31 / 42, 512 x 1280 x 1280 (2.5 per CU) 13.6 / 15.3, 512 x 5120 x 1280 45.6 / 44.5,
 // 1024 x 1280 x 1280 21 / 16.5, 154 x 1280 x 10240 (6 per CU) 26.7 / 15.4.
-bool one_launch(tfmq_handle h, long M, int N) {
-  return M <= 32 || static_cast<long>(ceil_div(M, 32)) * ceil_div(N, 32) <= 2L * h->cu_count;
+// From 20 blocks on the slices below beat it earlier: 256 x 5120 x 1280 31 / 19.
+bool one_launch(tfmq_handle h, long M, int N, int K) {
+  return M <= 32 || static_cast<long>(ceil_div(M, 32)) * ceil_div(N, 32) <= (K > 19 * 128 ? 1L : 2L) * h->cu_count;
 }
-int launch_product(tfmq_handle h, const GemmF8P& p, int y_dtype, hipStream_t st) {
+// slices of the K axis of a product whose tiles leave half the CUs idle: at least ten blocks each, a slice costs a write and a read of the result in fp32
+// and all of them a launch.  us, whole against sliced: 1024 x 5120 x 1280 (80 tiles, 40 blocks) 41.6 / 28.7, 512 x 5120 x 1280 40.5 / 21.6; with three
+// blocks a slice 1024 x 1280 x 1280 15.3 / 20.7, 512 x 768 x 1280 10.6 / 12.8.
+int product_slices(tfmq_handle h, long M, int N, int K) {
+  if (one_launch(h, M, N, K)) return 1;
+  const long nt = static_cast<long>(ceil_div(M, 128)) * ceil_div(N, 128), Kb = (K + 127) / 128;
+  const long n = std::min(h->cu_count / nt, Kb / 10);
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+template <int YDT>
+int launch_sum(tfmq_handle h, const float* part, const float* bias, void* y, long n, int N, int nslice, hipStream_t st) {
+  hipLaunchKernelGGL((k_sum_slices<YDT>), dim3(static_cast<unsigned>((n + 1023) / 1024)), dim3(256), 0, st, part, bias, static_cast<typename Elem<YDT>::type*>(y), n, N, nslice);
+  TFMQ_LAUNCH_CHECK(h);
+  return TFMQ_OK;
+}
+// part: room for p.nslice partial results, or null (one slice)
+int launch_product(tfmq_handle h, const GemmF8P& p, int y_dtype, float* part, hipStream_t st) {
+  if (p.nslice > 1) {
+    GemmF8P q = p;
+    q.y = part;
+    q.bias = nullptr;
+    const int rc = y_dtype == DT_F32 ? launch_128<DT_F32, false>(h, q, st) : launch_128<DT_PART, false>(h, q, st);
+    if (rc != TFMQ_OK) return rc;
+    const long n = p.M * p.N;
+    if (y_dtype == DT_F32) return launch_sum<DT_F32>(h, part, p.bias, p.y, n, p.N, p.nslice, st);
+    return y_dtype == DT_F16 ? launch_sum<DT_F16>(h, part, p.bias, p.y, n, p.N, p.nslice, st) : launch_sum<DT_BF16>(h, part, p.bias, p.y, n, p.N, p.nslice, st);
+  }
   if (y_dtype == DT_F32) return launch_128<DT_F32, false>(h, p, st);
   if (big_tiles(h, p.M, p.N))
     return y_dtype == DT_F16 ? launch_gemm<256, 256, 128, 64, DT_F16, false, 2>(h, p, st) : launch_gemm<256, 256, 128, 64, DT_BF16, false, 2>(h, p, st);
@@ -826,12 +866,17 @@ struct Carve {
   }
 };
 struct LinWs {
-  uint8_t* q;
-  float* s;
-  LinWs(Carve& c, long M, int K) {
+  uint8_t* q = nullptr;
+  float *s = nullptr, *part = nullptr;
+  int slices;
+  LinWs(Carve& c, tfmq_handle h, long M, int N, int K, bool quantise) {
     const long Kb = (K + 127) / 128;
-    q = c.take<uint8_t>(static_cast<size_t>(M) * Kb * 128);
-    s = c.take<float>(static_cast<size_t>(M) * Kb);
+    slices = product_slices(h, M, N, K);
+    if (quantise && !one_launch(h, M, N, K)) {
+      q = c.take<uint8_t>(static_cast<size_t>(M) * Kb * 128);
+      s = c.take<float>(static_cast<size_t>(M) * Kb);
+    }
+    if (slices > 1) part = c.take<float>(static_cast<size_t>(slices) * M * N);
   }
 };
 struct BwdWs {
@@ -840,7 +885,7 @@ struct BwdWs {
   int slices;
   BwdWs(Carve& c, tfmq_handle h, long M, int N, int K, bool gx, bool gw) {
     const long Mb = (M + 127) / 128, Nb = (N + 127) / 128;
-    if (gx && !one_launch(h, M, K)) {
+    if (gx && !one_launch(h, M, K, N)) {
       gq = c.take<uint8_t>(static_cast<size_t>(M) * Nb * 128);
       gs = c.take<float>(static_cast<size_t>(M) * Nb);
     }
@@ -878,10 +923,10 @@ extern "C" int tfmq_pack_w_fp8(tfmq_handle h, const float* w, int N, int K, uint
   return TFMQ_OK;
 }
 
-extern "C" size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K) {
-  if (!h || !shape_ok(M, N, K) || one_launch(h, M, N)) return 0;
+extern "C" size_t tfmq_linear_fp8_ws_bytes(tfmq_handle h, long M, int N, int K, int quantised) {
+  if (!h || !shape_ok(M, N, K)) return 0;
   Carve c{nullptr};
-  LinWs w(c, M, K);
+  LinWs w(c, h, M, N, K, !quantised);
   return c.at;
 }
 
@@ -893,17 +938,17 @@ extern "C" int tfmq_linear_fp8(tfmq_handle h, const void* x, int dtype, long M, 
   TFMQ_CHECK_ARG(h, aligned16(w) && aligned16(xq) && aligned16(y) && aligned16(work), "linear_fp8: operands, output and workspace must be 16-byte aligned");
   hipStream_t st = as_stream(stream);
   const int Kb = (K + 127) / 128;
-  if (x && one_launch(h, M, N)) return launch_small(h, SmallF8P{x, ld, static_cast<int>(M), K, w, ws, ws_n, ws_k, bias, y, N, Kb}, dtype, y_dtype, st);
+  if (x && one_launch(h, M, N, K)) return launch_small(h, SmallF8P{x, ld, static_cast<int>(M), K, w, ws, ws_n, ws_k, bias, y, N, Kb}, dtype, y_dtype, st);
+  Carve c{static_cast<char*>(work)};
+  const LinWs b(c, h, M, N, K, x != nullptr);
+  TFMQ_CHECK_ARG(h, c.at == 0 || work, "linear_fp8: null workspace");
   if (x) {
-    TFMQ_CHECK_ARG(h, work, "linear_fp8: null workspace");
-    Carve c{static_cast<char*>(work)};
-    const LinWs b(c, M, K);
     const int rc = launch_quant_rows(h, x, dtype, M, K, ld, b.q, b.s, st);
     if (rc != TFMQ_OK) return rc;
     xq = b.q;
     xs = b.s;
   }
-  return launch_product(h, GemmF8P{xq, w, xs, ws, ws_n, ws_k, bias, y, M, N, Kb, 0, 0, 1}, y_dtype, st);
+  return launch_product(h, GemmF8P{xq, w, xs, ws, ws_n, ws_k, bias, y, M, N, Kb, 0, 0, b.slices}, y_dtype, b.part, st);
 }
 
 extern "C" size_t tfmq_linear_fp8_bwd_ws_bytes(tfmq_handle h, long M, int N, int K, int want_gx, int want_gw) {
@@ -941,15 +986,11 @@ extern "C" int tfmq_linear_fp8_bwd(tfmq_handle h, const void* x, int x_dtype, lo
     else rc = gy_dtype == DT_F16 ? launch_grads<DT_F16>(h, pw, px, st) : launch_grads<DT_BF16>(h, pw, px, st);
   } else {
     if (gx)
-      rc = b.gq ? launch_product(h, px, gy_dtype, st)
+      rc = b.gq ? launch_product(h, px, gy_dtype, nullptr, st)
                 : launch_small(h, SmallF8P{gy, gy_ld, static_cast<int>(M), N, wt, ws, 1, Kb, nullptr, gx, K, Nb}, gy_dtype, gy_dtype, st);
     if (rc == TFMQ_OK && gw) rc = launch_128<DT_F32, true>(h, pw, st);
   }
   if (rc != TFMQ_OK) return rc;
-  if (gw && b.part) {
-    const long n = static_cast<long>(N) * K;
-    hipLaunchKernelGGL(k_sum_slices, dim3(static_cast<unsigned>((n + 1023) / 1024)), dim3(256), 0, st, b.part, gw, n, b.slices);
-    TFMQ_LAUNCH_CHECK(h);
-  }
+  if (gw && b.part) rc = launch_sum<DT_F32>(h, b.part, nullptr, gw, static_cast<long>(N) * K, K, b.slices, st);
   return rc;
 }

@@ -1917,7 +1917,7 @@ def linear_fp8(x, pw: PackedFp8, out_dtype: Optional[torch.dtype] = None) -> tor
     if M == 0:
         return y
     h = handle(d)
-    nb = 0 if quantised else h.lib.tfmq_linear_fp8_ws_bytes(h.h, M, pw.N, pw.K)
+    nb = h.lib.tfmq_linear_fp8_ws_bytes(h.h, M, pw.N, pw.K, int(quantised))
     ws = _alloc(nb, dtype=torch.uint8, device=src.device) if nb else None
     xp, qp, sp = (None, src.data_ptr(), x.scale.data_ptr()) if quantised else (x.data_ptr(), None, None)
     b = None if pw.bias is None else pw.bias.data_ptr()
