@@ -636,7 +636,8 @@ int tfmq_linear_fp8_bwd(tfmq_handle h, const void* x, int x_dtype, long x_ld, co
  * q [B][Tq][H d], k / v [B][Tk][G d]: batch and token strides in elements (multiples of 8, 16-byte aligned rows), unit channel stride; o / dq
  * contiguous [B][Tq][H d], dk / dv contiguous [B][Tk][G d], lse fp32 [B][H][Tq].  d % 8 == 0, d <= 160.  Query head h reads key head h / (H / G).
  * A key is kept if its index is below kv_lens[b] (null: Tk) and mask[b][key] != 0 (null: all); a query row from q_lens[b] on, and a row that
- * keeps no key, is zero with lse = -inf, and its gradients are zero.  What masked places hold (NaN, infinities) is never read into a sum. */
+ * keeps no key, is zero with lse = -inf, and its gradients are zero.  What masked places hold (NaN, infinities) is never read into a sum.
+ * The forward takes Tk = 0 (k and v may be null: zeros and -inf); the backward wants Tk > 0. */
 typedef struct tfmq_xattn_desc {
   int32_t dtype;                 /* 1 fp16, 2 bf16 */
   int32_t B, H, G, Tq, Tk, d;

@@ -1,0 +1,107 @@
+"""K18 where it can go wrong: values that are not finite, the range of the fp16 gradients, few kept states in a long buffer, long tails.
+
+Bounds, u = eps / 2 of the operand type, n kept states, f = e + (d + n + 8) 2^-24 with e the score's share (test_cross_attention_gpu):
+ * o: (u + e) sum p |v| + u |o|; fp16 probabilities are carried with 2^7, so one below 2^-21 of the row's largest loses at most 2^-32 of it.
+ * D = sum_j p_j dp_j in fp32: with a_j = sum_c |go v_j|, A = sum_j p_j a_j its error is at most 2 f A, that of ds = p (dp - D) before its rounding
+   3 f p (a + A).  ds is rounded once to the operand type (u |ds|).  Over more than 128 states the walk starts from the D0 of the rounded o,
+   |D - D0| <= (u + 2 f) A, and the difference is put right with p rounded: 2 u (u + 2 f) A p more.
+ * fp16 carries ds with a power of two by the row's (dq) or slice's (dk) largest |dp - D|: what underflows is below 2^-33 of that.
+ * results are rounded once more; sums over n states or m rows in fp32 add n (m) 2^-24 of their terms' magnitudes.
+"""
+import math
+
+import pytest
+import torch
+
+from test_cross_attention_gpu import DEV, TYPES, _check, _dev, _fused_dev, _mk
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import tfmq_dm_amd.ops as ops
+    return ops
+
+
+def _exact(q, k, v, go, H, scale, G=None, kv_lens=None, mask=None):
+    """64-bit results and the bounds above."""
+    dt = q.dtype
+    u = torch.finfo(dt).eps / 2
+    half = dt == torch.float16
+    tiny = 2.0 ** -25 if half else 0.0
+    G = H if G is None else G
+    (B, Tq, Cq), Tk, rep = q.shape, k.shape[1], H // G
+    d = Cq // H
+    Z = lambda *s: torch.zeros(*s, dtype=torch.float64)      # noqa: E731
+    R = {"o": Z(B, Tq, Cq), "lse": torch.full((B, H, Tq), -math.inf, dtype=torch.float64), "dq": Z(B, Tq, Cq), "dk": Z(B, Tk, G * d), "dv": Z(B, Tk, G * d)}
+    E = {n: torch.zeros_like(t) for n, t in R.items()}
+    for b in range(B):
+        idx = torch.arange(Tk if kv_lens is None else int(kv_lens[b]))
+        if mask is not None:
+            idx = idx[mask[b, idx]]
+        n = idx.numel()
+        if n == 0:
+            continue
+        for h in range(H):
+            cq, ck = slice(h * d, (h + 1) * d), slice(h // rep * d, (h // rep + 1) * d)
+            qq, kk, vv, gg = q[b, :, cq].double(), k[b, idx, ck].double(), v[b, idx, ck].double(), go[b, :, cq].double()
+            s = qq @ kk.t() * scale
+            lse = torch.logsumexp(s, -1)
+            p = torch.exp(s - lse[:, None])
+            o = p @ vv
+            e = (2 * (d + 2) * 2.0 ** -24 * scale * (qq.abs() @ kk.abs().t()).amax(-1) + (n + 8) * 2.0 ** -24 + 2.0 ** -21)[:, None]
+            f = e + (d + n + 8) * 2.0 ** -24
+            R["o"][b, :, cq], R["lse"][b, h] = o, lse
+            E["o"][b, :, cq] = (u + e) * (p @ vv.abs()) + u * o.abs() + tiny + (2.0 ** -32 if half else 2.0 ** -126) * vv.abs().sum(0)
+            E["lse"][b, h] = e[:, 0] + 2.0 ** -23 * lse.abs()
+            dp, a = gg @ vv.t(), gg.abs() @ vv.abs().t()
+            A, diff = (p * a).sum(-1, keepdim=True), dp - (p * dp).sum(-1, keepdim=True)
+            ds, low = p * diff, 2.0 ** -126 * (a + (p * a).sum(-1, keepdim=True))
+            und = 2.0 ** -33 * diff.abs() if half else torch.zeros_like(diff)
+            Ed = u * ds.abs() + 3 * f * p * (a + A) + low
+            late = 2 * u * (u + 2 * f) * A * p + (u * A * 2.0 ** -25 if half else 0.0) if Tk > 128 else 0.0
+            R["dq"][b, :, cq] = scale * ds @ kk
+            E["dq"][b, :, cq] = scale * (Ed + late + und.amax(-1, keepdim=True) + n * 2.0 ** -24 * ds.abs()) @ kk.abs() + tiny
+            R["dk"][b, idx, ck] += scale * ds.t() @ qq
+            R["dv"][b, idx, ck] += p.t() @ gg
+            E["dk"][b, idx, ck] += scale * (Ed + und.amax() + rep * Tq * 2.0 ** -24 * ds.abs()).t() @ qq.abs()
+            E["dv"][b, idx, ck] += ((u + e + rep * Tq * 2.0 ** -24) * p + 2.0 ** -126).t() @ gg.abs() + tiny * 2.0 ** -12 * gg.abs().sum(0)
+    E["dq"] += u * R["dq"].abs()
+    for n in ("dk", "dv"):
+        E[n] += u * R[n].abs() + tiny
+    return R, E
+
+
+def _all(ops, q, k, v, go, H, scale, G=None, kv_lens=None, mask=None):
+    """(o, lse, dq, dk, dv) on the device; the same bits (NaN counted as equal) from a second call."""
+    how = dict(kv_heads=G, **dict(zip(("kv_lens", "mask"), _dev(kv_lens, mask))))
+    (qd, gd), (kd, vd) = _dev(q, go), _fused_dev(k, v)
+
+    def once():
+        o, lse = ops.cross_attention(qd, kd, vd, H, scale, want_lse=True, **how)
+        return dict(zip(("o", "lse", "dq", "dk", "dv"), (o, lse) + tuple(ops.cross_attention_bwd(qd, kd, vd, o, lse, gd, H, scale, **how))))
+    got, again = once(), once()
+    for n in got:
+        _same(got[n], again[n], n)
+    return got
+
+
+def _same(a, b, what):
+    a, b = a.float().cpu(), b.float().cpu()
+    assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)), what
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("dt", TYPES)
+def test_c_entry_without_states(ops, dt, splits):
+    """tfmq_xattn_fwd takes Tk = 0 with k and v null: zeros and -inf, nothing read."""
+    B, H, Tq, d = 2, 3, 5, 40
+    q = torch.ones(B, Tq, H * d, dtype=dt, device=DEV)
+    o, lse = torch.full_like(q, 7.0), torch.zeros(B, H, Tq, device=DEV)
+    ws = torch.empty(splits * B * H * Tq * (d + 2), device=DEV)
+    h = ops.handle(0)
+    desc = ops._XATTN.pack(ops._DT_CODE[dt], B, H, H, Tq, 0, d, 1.0, q.data_ptr(), 0, 0, Tq * H * d, H * d, 0, 0, 0, 0, 0, 0, 0, 0, o.data_ptr(), 0, 0,
+                           lse.data_ptr(), 0, 0, 0, 0, 0, 0, ws.data_ptr(), splits)
+    h.call("xattn_fwd", desc, ops._stream(0))
+    assert (o == 0).all() and (lse == -math.inf).all()

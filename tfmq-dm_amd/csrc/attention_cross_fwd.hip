@@ -300,7 +300,7 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
   return for_head_dim(p.d, [&](auto dc) {
     constexpr int D = decltype(dc)::value;
     const int nkt = (p.Tk + 31) / 32;
-    if (p.nsplit == 1 && nkt <= 4 && rows_fit(p)) {
+    if (p.nsplit == 1 && nkt >= 1 && nkt <= 4 && rows_fit(p)) {          // (no states at all: the tiled kernel reads none)
       if (nkt == 1) return launch_short<T, D, 1>(h, p, st);
       if (nkt == 2) return launch_short<T, D, 2>(h, p, st);
       if (nkt == 3) return launch_short<T, D, 3>(h, p, st);
