@@ -105,3 +105,27 @@ def test_c_entry_without_states(ops, dt, splits):
                            lse.data_ptr(), 0, 0, 0, 0, 0, 0, ws.data_ptr(), splits)
     h.call("xattn_fwd", desc, ops._stream(0))
     assert (o == 0).all() and (lse == -math.inf).all()
+
+
+BAD = [float("nan"), float("inf"), -float("inf")]
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("where", ["q", "go"])
+@pytest.mark.parametrize("Tq,Tk", [(40, 100), (40, 200), (3000, 100)])
+def test_dropped_keys_have_zero_gradients_whatever_live_rows_hold(ops, Tq, Tk, where, bad):
+    """A live row that is not finite (a loss scale too large) spoils the kept keys of its item; masked ones and those behind the length stay zero, with
+    the rows in one slice or in several."""
+    B, H, d = 3, 2, 64
+    h = ops.handle(0)
+    assert Tq < 3000 or h.lib.tfmq_xattn_bwd_splits(h.h, B, H, H, Tq, Tk) > 1
+    q, k, v, go = _mk(B, Tq, Tk, H, H, d, torch.float16)
+    mask = torch.rand(B, Tk, generator=torch.Generator().manual_seed(1)) < 0.7
+    kv_lens = torch.tensor([Tk, Tk - 30, 0], dtype=torch.int32)
+    (q if where == "q" else go)[:, 3, 5] = bad
+    got = _all(ops, q, k, v, go, H, 0.125, None, kv_lens, mask)
+    keep = mask & (torch.arange(Tk)[None] < kv_lens[:, None])
+    for n in ("dk", "dv"):
+        assert (got[n].cpu()[~keep] == 0).all(), n
+        clean = slice(d, None)          # the other head
+        assert torch.isfinite(got[n][..., clean]).all(), n

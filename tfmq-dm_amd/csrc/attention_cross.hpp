@@ -299,7 +299,7 @@ __device__ __forceinline__ v16f start_scores(const float* bias, int hh) {
   return s;
 }
 
-// what a row that is not there (or has no query) leaves: zeros, whatever its lanes computed
+// what a row that is not there (or has no query), or a dropped key, leaves: zeros, whatever its lanes computed
 template <int N>
 __device__ __forceinline__ void zero_unless(bool ok, v16f (&a)[N]) {
   if (!ok) {

@@ -439,6 +439,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
     }
   }
   if (key >= (p.nsplit > 1 ? klen : p.Tk)) return;
+  zero_unless(keep, ak);          // (a live row that is not finite makes 0 * inf of a dropped key's zeros)
+  zero_unless(keep, av);
   const float fk = p.scale * unf, fv = is_f16<T>() ? 1.0f / 4096.0f : 1.0f;
   const long krow = (static_cast<long>(b) * p.Tk + key) * p.G + g;
   if (p.nsplit > 1) {
