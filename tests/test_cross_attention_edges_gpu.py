@@ -129,3 +129,40 @@ def test_dropped_keys_have_zero_gradients_whatever_live_rows_hold(ops, Tq, Tk, w
         assert (got[n].cpu()[~keep] == 0).all(), n
         clean = slice(d, None)          # the other head
         assert torch.isfinite(got[n][..., clean]).all(), n
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("Tk", [20, 100, 128, 129, 200])
+def test_rows_without_keys_are_zero_whatever_they_hold(ops, Tk, bad):
+    B, Tq, H, d = 3, 40, 2, 64
+    q, k, v, go = _mk(B, Tq, Tk, H, H, d, torch.float16)
+    mask = torch.rand(B, Tk, generator=torch.Generator().manual_seed(2)) < 0.7
+    mask[1] = False
+    kv_lens = torch.tensor([Tk, Tk, 0], dtype=torch.int32)
+    q[1:, 3], go[1:, 4] = bad, bad
+    want = _all(ops, q.nan_to_num(1.0, 1.0, 1.0), k, v, go.nan_to_num(1.0, 1.0, 1.0), H, 0.125, None, kv_lens, mask)
+    for n, t in _all(ops, q, k, v, go, H, 0.125, None, kv_lens, mask).items():
+        assert torch.equal(t[0], want[n][0]), n
+        assert (t[1:] == (-math.inf if n == "lse" else 0)).all(), n
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("Tk,n", [(60, 33), (100, 64), (100, 70), (128, 65), (300, 128), (300, 200)])
+def test_a_dropped_key_is_as_if_absent_also_for_values_that_are_not_finite(ops, Tk, n, bad):
+    """Rows of q, k, v and go that are not finite give what the formula gives over the kept keys alone, whether others are masked, lie behind the length
+    or are not stored at all: the same bits from the same kernel, NaN in the same places from another.  (Row 2's infinity meets one sign in every kept
+    key: a score of +inf or -inf without a NaN of its own.)"""
+    B, Tq, H, d = 4, 40, 1, 64
+    q, k, v, go = _mk(B, Tq, Tk, H, H, d, torch.bfloat16)
+    k[..., 7] = k[..., 7].abs() + 1
+    q[:, 2, 7], q[1, 5], go[:, 9, 3] = bad, bad, bad
+    k[2, 1, 0], v[3, 0, 0] = bad, bad
+    lens, mask = torch.full((B,), n, dtype=torch.int32), torch.arange(Tk)[None].expand(B, -1) < n
+    want = _all(ops, q, k[:, :n], v[:, :n], go, H, 0.125)
+    for how in (dict(kv_lens=lens), dict(mask=mask)):
+        got = _all(ops, q, k, v, go, H, 0.125, **how)
+        for name in ("o", "lse", "dq"):
+            if (n <= 128) == (Tk <= 128):
+                _same(got[name], want[name], (name, tuple(how)))
+            else:          # (two kernels, whose roundings differ)
+                _same(got[name].float() * 0, want[name].float() * 0, (name, tuple(how)))

@@ -90,10 +90,19 @@ struct KeyTile {
     const char* p = reinterpret_cast<const char*>(base + k0 * ts);
     const int last = Tk - 1 - k0;
 #pragma unroll
+    for (int it = 0; it < PT; ++it) reg[it] = *reinterpret_cast<const uint4*>(p + offset(it, min(row_of(it), last), ts, d));
+  }
+  // the same keys, those not kept (bits of `keep`) read from key `kept` of the tensor instead
+  __device__ __forceinline__ void load_kept(const T* base, long ts, int k0, int kept, unsigned keep, int d) {
+    const char *p = reinterpret_cast<const char*>(base + k0 * ts), *q = reinterpret_cast<const char*>(base + kept * ts);
+#pragma unroll
     for (int it = 0; it < PT; ++it) {
-      const unsigned off = static_cast<unsigned>(min(row_of(it), last)) * static_cast<unsigned>(ts * 2) + static_cast<unsigned>(min(piece_of(it) * 8, d - 8) * 2);
-      reg[it] = *reinterpret_cast<const uint4*>(p + off);
+      const bool own = (keep >> row_of(it)) & 1;
+      reg[it] = *reinterpret_cast<const uint4*>((own ? p : q) + offset(it, own ? row_of(it) : 0, ts, d));
     }
+  }
+  __device__ __forceinline__ static unsigned offset(int it, int row, long ts, int d) {
+    return static_cast<unsigned>(row) * static_cast<unsigned>(ts * 2) + static_cast<unsigned>(min(piece_of(it) * 8, d - 8) * 2);
   }
   __device__ __forceinline__ void store(unsigned char* lds, unsigned long long keep, unsigned long long all, int d) {
     if (keep != all || d != D) {
@@ -259,9 +268,11 @@ struct RowWalk {
   }
 };
 
-// all of up to 128 states into LDS: K and V rows (dropped keys and channels from d on: zeros) and 0 / -inf per key; a barrier behind it
+// all of up to 128 states into LDS and 0 / -inf per key; a barrier behind it.  -> whether any key is kept.  Channels from d on, and dropped keys' rows of V, are
+// zeros.  A dropped key's row of K is a kept one's: its score is -inf plus a finite number or what that key's is, so a query that is not finite (0 * inf
+// with zeros) gives what it gives over the kept keys alone.
 template <typename T, int D, int NKT, int KS, int VS>
-__device__ __forceinline__ void stage_short(const XattnP& p, int b, int g, int klen, unsigned char* sK, unsigned char* sV, float* sB) {
+__device__ __forceinline__ bool stage_short(const XattnP& p, int b, int g, int klen, unsigned char* sK, unsigned char* sV, float* sB) {
   const int lane = threadIdx.x & 63;
   const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
   const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
@@ -274,21 +285,23 @@ __device__ __forceinline__ void stage_short(const XattnP& p, int b, int g, int k
     keep[w] = __ballot(kept);
     if (threadIdx.x < 64 && key < NKT * 32) sB[key] = kept ? 0.0f : -INFINITY;
   }
+  const int first = keep[0] ? __ffsll(keep[0]) - 1 : keep[1] ? 63 + __ffsll(keep[1]) : 0;
 #pragma unroll
   for (int t = 0; t < NKT; ++t) {
     KeyTile<T, D, 32, KS> tk;
     KeyTile<T, D, 32, VS> tv;
     const int k0 = min(t * 32, p.Tk - 1);
-    tk.load(kb, p.k.ts, k0, p.Tk, p.d);
+    const unsigned kk = static_cast<unsigned>(keep[t >> 1] >> (32 * (t & 1)));
+    tk.load_kept(kb, p.k.ts, k0, first, kk, p.d);
     tv.load(vb, p.v.ts, k0, p.Tk, p.d);
-    const unsigned long long kk = (keep[t >> 1] >> (32 * (t & 1))) & 0xffffffffull;
-    tk.store(sK + t * 32 * KS, kk, 0xffffffffull, p.d);
+    tk.store(sK + t * 32 * KS, 0xffffffffull, 0xffffffffull, p.d);
     tv.store(sV + t * 32 * VS, kk, 0xffffffffull, p.d);
   }
   __syncthreads();
+  return (keep[0] | keep[1]) != 0;
 }
 
-// scores start from 0 for kept keys and from -inf for dropped ones (whose rows of K are zeros): a mask costs no arithmetic
+// scores start from 0 for kept keys and from -inf for dropped ones: a mask costs no arithmetic
 __device__ __forceinline__ v16f start_scores(const float* bias, int hh) {
   v16f s;
 #pragma unroll

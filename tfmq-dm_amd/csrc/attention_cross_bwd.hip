@@ -214,10 +214,10 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
     lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, static_cast<int>(ok ? static_cast<unsigned>(w.row) * 4 : NOWHERE), 0, 0));
   };
   load_rows();
-  stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);
+  const bool any = stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);
   const float c2 = p.scale * LOG2E;
   while (w.row - j < r_end) {
-    const bool in = w.row < r_end, ok = in && w.i < qlen;
+    const bool in = w.row < r_end, ok = any && in && w.i < qlen;
     const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
     float dl = 0.0f, gm = 0.0f;
     if (is_f16<T>()) {

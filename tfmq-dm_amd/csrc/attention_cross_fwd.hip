@@ -182,10 +182,10 @@ __global__ __launch_bounds__(256, short_waves(D, NKT)) void k_xattn_short(XattnP
     }
   };
   load_q();
-  stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);
+  const bool any = stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);          // (an item that keeps nothing: zeros, whatever its rows hold)
   const float c2 = p.scale * LOG2E;
   while (w.row - j < r_end) {
-    const bool in = w.row < r_end, ok = in && w.i < qlen;
+    const bool in = w.row < r_end, ok = any && in && w.i < qlen;
     const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
     v16f s[NKT];
 #pragma unroll
