@@ -166,3 +166,33 @@ def test_a_dropped_key_is_as_if_absent_also_for_values_that_are_not_finite(ops, 
                 _same(got[name], want[name], (name, tuple(how)))
             else:          # (two kernels, whose roundings differ)
                 _same(got[name].float() * 0, want[name].float() * 0, (name, tuple(how)))
+
+
+def _scaled(kind, B, Tq, Tk, H, d, dt):
+    q, k, v, go = [t.float() for t in _mk(B, Tq, Tk, H, H, d, dt)]
+    if kind == "large":               # states of thousands that line up with a small upstream gradient
+        sign = torch.where(torch.rand(B, Tk, 1, generator=torch.Generator().manual_seed(Tk)) < 0.5, -1.0, 1.0)
+        v, go = sign * (3000 + 100 * v), 1e-3 * (1 + go.abs())
+    elif kind == "small":             # and small states
+        q, k, v = q / 64, k * 64, v * 2.0 ** -10
+    elif kind == "small_q":
+        q, k, v = q * 64, k / 64, v * 2.0 ** -10
+    elif kind == "rising":            # each tile's states larger than all before; the first ones are zero
+        v = v * (torch.arange(Tk).float() / 8)[None, :, None] ** 2 / 4
+        v[:, :5] = 0
+    else:                             # falling
+        v = v * 2000 / (1 + torch.arange(Tk).float())[None, :, None]
+    return [t.to(dt) for t in (q, k, v, go)]
+
+
+@pytest.mark.parametrize("kind", ["large", "small", "small_q", "rising", "falling"])
+@pytest.mark.parametrize("Tq,Tk,d", [(5, 2, 64), (64, 77, 40), (40, 200, 64), (33, 300, 128), (2500, 70, 64), (130, 129, 160)])
+def test_fp16_gradients_keep_their_range(ops, Tq, Tk, d, kind):
+    """ds = p (go v - D) has the size of go v: an operand that only go's size places in fp16's range is infinite for large states, though every gradient is
+    finite, and subnormal for small ones."""
+    H = 2
+    q, k, v, go = _scaled(kind, 2, Tq, Tk, H, d, torch.float16)
+    R, E = _exact(q, k, v, go, H, d ** -0.5)
+    assert all(float(R[n].abs().max()) < 6e4 for n in ("dq", "dk", "dv"))
+    for n, t in _all(ops, q, k, v, go, H, d ** -0.5).items():
+        _check(n, t, R, E)

@@ -268,10 +268,11 @@ struct RowWalk {
   }
 };
 
-// all of up to 128 states into LDS and 0 / -inf per key; a barrier behind it.  -> whether any key is kept.  Channels from d on, and dropped keys' rows of V, are
-// zeros.  A dropped key's row of K is a kept one's: its score is -inf plus a finite number or what that key's is, so a query that is not finite (0 * inf
-// with zeros) gives what it gives over the kept keys alone.
-template <typename T, int D, int NKT, int KS, int VS>
+// all of up to 128 states into LDS and 0 / -inf per key; a barrier behind it.  -> whether any key is kept.  Channels from d on are zeros.  A dropped key's
+// row of K is a kept one's: its score is -inf plus a finite number or what that key's is, so a query that is not finite (0 * inf with zeros) gives what it
+// gives over the kept keys alone.  Its row of V is zeros in the forward (p v adds nothing whatever the kept ones hold), a kept one's in the gradients
+// (VKEPT: go v then has no value that no kept key has).
+template <typename T, int D, int NKT, int KS, int VS, bool VKEPT>
 __device__ __forceinline__ bool stage_short(const XattnP& p, int b, int g, int klen, unsigned char* sK, unsigned char* sV, float* sB) {
   const int lane = threadIdx.x & 63;
   const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
@@ -293,9 +294,10 @@ __device__ __forceinline__ bool stage_short(const XattnP& p, int b, int g, int k
     const int k0 = min(t * 32, p.Tk - 1);
     const unsigned kk = static_cast<unsigned>(keep[t >> 1] >> (32 * (t & 1)));
     tk.load_kept(kb, p.k.ts, k0, first, kk, p.d);
-    tv.load(vb, p.v.ts, k0, p.Tk, p.d);
+    if (VKEPT) tv.load_kept(vb, p.v.ts, k0, first, kk, p.d);
+    else tv.load(vb, p.v.ts, k0, p.Tk, p.d);
     tk.store(sK + t * 32 * KS, 0xffffffffull, 0xffffffffull, p.d);
-    tv.store(sV + t * 32 * VS, kk, 0xffffffffull, p.d);
+    tv.store(sV + t * 32 * VS, VKEPT ? 0xffffffffull : kk, 0xffffffffull, p.d);
   }
   __syncthreads();
   return (keep[0] | keep[1]) != 0;

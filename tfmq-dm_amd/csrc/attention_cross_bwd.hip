@@ -7,9 +7,10 @@
 // further rows).  Seven products instead of the five of a fused pass, for results that are the same bits every time.  Where few key blocks face
 // many rows -- 77 states under 4096 tokens -- the rows are cut into slices whose fp32 sums are added in order.
 //
-// fp16 range: ds has the size of go p, far below fp16's normal numbers when a loss is averaged over many tokens.  The ds operand is therefore
-// carried with a power of two that brings go's largest magnitude (of the row in dq, of the slice's rows in dkv) to 1 ... 2, and p in dv with 2^12;
-// both are exact and taken out of the fp32 sums.  bf16 has the range.
+// fp16 range: ds has the size of p go v, which may lie far below fp16's normal numbers (a loss averaged over many tokens, small states) or above its largest
+// (states of thousands).  The ds operand is therefore carried with a power of two by the largest |dp - D| itself -- of the row in dq, of the slice's rows in
+// dkv -- so that it stays below 2^15 and what underflows below 2^-33 of that largest; and p in dv with 2^12.  All are exact and taken out of the fp32
+// sums.  bf16 has the range.
 #include "attention_cross.hpp"
 
 using namespace xattn;
@@ -18,11 +19,12 @@ namespace {
 
 template <typename T> constexpr bool is_f16() { return std::is_same<T, _Float16>::value; }
 
-// 2^-exponent of a magnitude (1 for zero; finite for every input)
+// the power of two that brings a magnitude to 1 ... 2 (2^0 for zero; within 2^+-72 for every input: products of fp16 values lie in that)
 __device__ __forceinline__ int inv_exponent(float a) {
   const int e = static_cast<int>((__float_as_uint(a) >> 23) & 255);
-  return e == 0 ? 0 : 127 - min(max(e, 27), 227);
+  return e == 0 ? 0 : 127 - min(max(e, 55), 199);
 }
+constexpr int DS_TOP = 13;          // where the operand's largest |dp - D| is put when it is known beforehand: 2^13 ... 2^14
 
 // Three products and the exponentials per score; operand reads run ahead of the products (dealt between them).  One wave a SIMD at d = 128 (315 registers; at
 // 256 it spills).  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 67 us.
@@ -44,7 +46,7 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
   const int head = g * p.rep + hi;
 
   V8 qf[NKS], gf[NKS];
-  float dl = 0.0f, gm = 0.0f;
+  float dl = 0.0f;
   {
     const long hc = static_cast<long>(head) * p.d;
     const T* qrow = static_cast<const T*>(p.q.p) + b * p.q.bs + i * p.q.ts + hc;
@@ -63,26 +65,19 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
       gf[ks] = __builtin_bit_cast(V8, w);
       const V8 of = __builtin_bit_cast(V8, z);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = static_cast<float>(gf[ks][e]);
-        dl = __builtin_fmaf(static_cast<float>(of[e]), x, dl);
-        gm = fmaxf(gm, fabsf(x));
-      }
+      for (int e = 0; e < 8; ++e) dl = __builtin_fmaf(static_cast<float>(of[e]), static_cast<float>(gf[ks][e]), dl);
     }
   }
   dl += __shfl_xor(dl, 32, 64);
-  gm = fmaxf(gm, __shfl_xor(gm, 32, 64));
   float lse2 = INFINITY;
   if (ok) {
     const float v = p.lse_in[brow];
     lse2 = v == -INFINITY ? INFINITY : v * LOG2E;
   }
-  if (in && hh == 0) {
-    p.delta[brow] = dl;
-    p.delta[static_cast<long>(p.B) * p.H * p.Tq + brow] = gm;
-  }
-  const int fe = is_f16<T>() ? inv_exponent(gm) : 0;
-  const float sh = lse2 - static_cast<float>(fe);
+  if (in && hh == 0) p.delta[brow] = dl;
+  // fp16: the operand's power of two, by the largest |dp - D| so far: 2^8 ... 2^9 in the first tile that has one; a larger one moves it down only past
+  // 2^15 (and the sums with it: exact, and rare)
+  float f = 1.0f, dlf = dl, top = 0.0f, lim = 0.0f;
 
   const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
   const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
@@ -144,10 +139,38 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
         const unsigned bits = static_cast<unsigned>(cur >> (32 * kt)) >> (4 * hh);
         if (cur != ~0ull) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = ((bits >> crow(r, 0)) & 1) ? s[r] : -INFINITY;
+          for (int r = 0; r < 16; ++r) {
+            const bool kept = (bits >> crow(r, 0)) & 1;
+            s[r] = kept ? s[r] : -INFINITY;
+            if (is_f16<T>()) dp[r] = kept ? dp[r] : dl;
+          }
+        }
+        if constexpr (is_f16<T>()) {
+          float mx = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            dp[r] = __builtin_fmaf(dp[r], f, -dlf);
+            mx = fmaxf(mx, fabsf(dp[r]));
+          }
+          if (__any(mx > lim)) {
+            const float row = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float ratio = row > lim ? __builtin_amdgcn_exp2f(static_cast<float>(inv_exponent(row) + 8)) : 1.0f;
+            lim = row > lim ? 32768.0f : lim;
+            f *= ratio, dlf *= ratio, top *= ratio, mx *= ratio;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] *= ratio;
+#pragma unroll
+            for (int t2 = 0; t2 < NRT; ++t2)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) acc[t2][r] *= ratio;
+          }
+          top = fmaxf(top, mx);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] -= dl;
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -sh)) * (dp[r] - dl);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2)) * dp[r];
         V8 df[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) df[u] = frag_regs<T>(s, u);
@@ -162,12 +185,13 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
     }
     cur = nxt;
   }
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
   if (!in) return;
   zero_unless(ok, acc);
-  const float f = p.scale * __builtin_amdgcn_exp2f(static_cast<float>(-fe));
+  if (is_f16<T>() && hh == 0) p.delta[static_cast<long>(p.B) * p.H * p.Tq + brow] = ok ? top / f : 0.0f;          // (k_xattn_dkv's range)
   T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
 #pragma unroll
-  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, acc[t], f);
+  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, acc[t], p.scale / f);
 }
 
 // ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form).  A row's probabilities and dp all
@@ -193,7 +217,7 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
   const Rsrc rq = buffer_of(static_cast<const T*>(p.q.p) + b * p.q.bs + hc, ((p.Tq - 1) * p.q.ts + rd) * 2);
   const Rsrc rg = buffer_of(static_cast<const T*>(p.go.p) + b * p.go.bs + hc, ((p.Tq - 1) * p.go.ts + rd) * 2);
   const Rsrc ry = buffer_of(static_cast<T*>(p.y) + b * p.Tq * C + hc, (p.Tq * C - hc) * 2);
-  const Rsrc rl = buffer_of(p.lse_in + brow0, p.R * 4), rdl = buffer_of(p.delta + brow0, p.R * 4), rgm = buffer_of(p.delta + rows + brow0, p.R * 4);
+  const Rsrc rl = buffer_of(p.lse_in + brow0, p.R * 4), rdl = buffer_of(p.delta + brow0, p.R * 4), rmx = buffer_of(p.delta + rows + brow0, p.R * 4);
   const unsigned qts = static_cast<unsigned>(p.q.ts) * 2, gts = static_cast<unsigned>(p.go.ts) * 2;
   const unsigned yts = static_cast<unsigned>(C) * 2, hs = static_cast<unsigned>(p.d) * 2;
 
@@ -214,21 +238,13 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
     lse = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, static_cast<int>(ok ? static_cast<unsigned>(w.row) * 4 : NOWHERE), 0, 0));
   };
   load_rows();
-  const bool any = stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);
+  const bool any = stage_short<T, D, NKT, KS, VS, true>(p, b, g, klen, sK, sV, sB);
   const float c2 = p.scale * LOG2E;
   while (w.row - j < r_end) {
     const bool in = w.row < r_end, ok = any && in && w.i < qlen;
     const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
-    float dl = 0.0f, gm = 0.0f;
-    if (is_f16<T>()) {
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gm = fmaxf(gm, fabsf(static_cast<float>(gf[ks][e])));
-    }
-    gm = fmaxf(gm, __shfl_xor(gm, 32, 64));
-    const int fe = is_f16<T>() ? inv_exponent(gm) : 0;
-    const float sh = (ok && lse != -INFINITY ? lse * LOG2E : INFINITY) - static_cast<float>(fe);
+    const float lse2 = ok && lse != -INFINITY ? lse * LOG2E : INFINITY;
+    float dl = 0.0f, hi = -INFINITY, lo = INFINITY;
     V8 df[2 * NKT];
     v16f ps[NKT], dps[NKT];
 #pragma unroll
@@ -242,24 +258,31 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -sh));
+        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2));
         dl = __builtin_fmaf(pr, dp[r], dl);
+        if (is_f16<T>()) hi = fmaxf(hi, dp[r]), lo = fminf(lo, dp[r]);          // (a dropped key's dp is a kept one's)
         s[r] = pr;
       }
       ps[kt] = s;
       dps[kt] = dp;
     }
     dl += __shfl_xor(dl, 32, 64);
-    dl *= __builtin_amdgcn_exp2f(static_cast<float>(-fe));          // (p carries 2^fe)
+    float f = 1.0f, inv_f = 1.0f;
+    if (is_f16<T>()) {
+      const float mx = fmaxf(fmaxf(hi, __shfl_xor(hi, 32, 64)) - dl, dl - fminf(lo, __shfl_xor(lo, 32, 64)));
+      const float fe = static_cast<float>(inv_exponent(mx) + DS_TOP);
+      f = __builtin_amdgcn_exp2f(fe);
+      inv_f = __builtin_amdgcn_exp2f(-fe);
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(ok ? mx : 0.0f), rmx, static_cast<int>(loff), 0, 0);          // (k_xattn_dkv's range)
+    }
 #pragma unroll
     for (int kt = 0; kt < NKT; ++kt) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ps[kt][r] *= dps[kt][r] - dl;
+      for (int r = 0; r < 16; ++r) ps[kt][r] *= is_f16<T>() ? __builtin_fmaf(dps[kt][r], f, -dl * f) : dps[kt][r] - dl;
 #pragma unroll
       for (int u = 0; u < 2; ++u) df[2 * kt + u] = frag_regs<T>(ps[kt], u);
     }
     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(dl), rdl, static_cast<int>(loff), 0, 0);
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(gm), rgm, static_cast<int>(loff), 0, 0);
     hold_order();
     w.step();
     load_rows();
@@ -271,9 +294,8 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
 #pragma unroll
       for (int t = 0; t < NRT; ++t) acc[t] = mfma16(frag_cols<T>(sK, KS, u * 16, t, lane), df[u], acc[t]);
     zero_unless(ok, acc);
-    const float f = p.scale * __builtin_amdgcn_exp2f(static_cast<float>(-fe));
 #pragma unroll
-    for (int t = 0; t < NRT; ++t) store16<T>(ry, yoff, in, t * 32, hh, p.d, acc[t], f);
+    for (int t = 0; t < NRT; ++t) store16<T>(ry, yoff, in, t * 32, hh, p.d, acc[t], p.scale * inv_f);
   }
 }
 
@@ -301,7 +323,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
   const bool keep = key < klen && (!p.mask || p.mask[b * p.mask_bs + key] != 0);
   const bool work = __any(keep);
   const long brow0 = (static_cast<long>(b) * p.H + g * p.rep) * p.Tq;          // the row space of (b, g) inside [B][H][Tq]
-  const float* gmax = p.delta + static_cast<long>(p.B) * p.H * p.Tq + brow0;
+  const float* dmax = p.delta + static_cast<long>(p.B) * p.H * p.Tq + brow0;          // fp16: the rows' largest |dp - D|
 
   const int nt = static_cast<int>((p.R + NR - 1) / NR), per = (nt + p.nsplit - 1) / p.nsplit;
   const int t0 = sp * per;
@@ -329,11 +351,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dkv(XattnP p) {
   float ff = 1.0f, unf = 1.0f;          // the power of two in ds, relative to the one in p, and what takes it out again
   if (is_f16<T>() && t0 < t1) {
     float mx = 0.0f;
-    for (long r = static_cast<long>(t0) * NR + tid; r < min(p.R, static_cast<long>(t1) * NR); r += 256) mx = fmaxf(mx, gmax[r]);
+    for (long r = static_cast<long>(t0) * NR + tid; r < min(p.R, static_cast<long>(t1) * NR); r += 256) mx = fmaxf(mx, dmax[r]);
     mx = wave_reduce_max(mx);
     if (lane == 0) sM[wid] = mx;
     __syncthreads();
-    const int fe = inv_exponent(fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3])));
+    const int fe = inv_exponent(fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]))) + DS_TOP;
     ff = __builtin_amdgcn_exp2f(static_cast<float>(fe) - PSHIFT);
     unf = __builtin_amdgcn_exp2f(static_cast<float>(-fe));
   }

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, short_waves(D, NKT)) void k_xattn_short(XattnP
     }
   };
   load_q();
-  const bool any = stage_short<T, D, NKT, KS, VS>(p, b, g, klen, sK, sV, sB);          // (an item that keeps nothing: zeros, whatever its rows hold)
+  const bool any = stage_short<T, D, NKT, KS, VS, false>(p, b, g, klen, sK, sV, sB);          // (an item that keeps nothing: zeros, whatever its rows hold)
   const float c2 = p.scale * LOG2E;
   while (w.row - j < r_end) {
     const bool in = w.row < r_end, ok = any && in && w.i < qlen;
