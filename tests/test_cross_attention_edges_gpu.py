@@ -196,3 +196,48 @@ def test_fp16_gradients_keep_their_range(ops, Tq, Tk, d, kind):
     assert all(float(R[n].abs().max()) < 6e4 for n in ("dq", "dk", "dv"))
     for n, t in _all(ops, q, k, v, go, H, d ** -0.5).items():
         _check(n, t, R, E)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Tq,Tk,H,G,d,kept", [(200, 129, 4, 4, 64, 2), (64, 300, 8, 2, 40, 3), (300, 1500, 4, 4, 64, 2), (100, 700, 4, 2, 128, 4), (100, 400, 2, 2, 160, 3),
+                                              (100, 400, 2, 2, 24, 2), (90, 260, 2, 2, 96, 2)])
+def test_few_kept_states_of_many_lose_only_the_roundings(ops, Tq, Tk, H, G, d, kept, dt):
+    """The bar of few stored states (test_cross_attention_gpu) for few kept ones: two roundings, the ds operand's and the result's."""
+    q, k, v, go = _mk(2, Tq, Tk, H, G, d, dt, Tk)
+    mask = torch.zeros(2, Tk, dtype=torch.bool)
+    for b in range(2):
+        mask[b, torch.randperm(Tk, generator=torch.Generator().manual_seed(Tk + b))[:kept]] = True
+    got = _all(ops, q, k, v, go, H, d ** -0.5, G, None, mask)
+    R, E = _exact(q, k, v, go, H, d ** -0.5, G, None, mask)
+    for n, t in got.items():
+        _check(n, t, R, E)
+    for n in ("dq", "dk"):
+        assert float((got[n].double().cpu() - R[n]).norm() / R[n].norm()) <= 2 ** 0.5 * torch.finfo(dt).eps / (2 * 3 ** 0.5), n
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Tk,d", [(200, 64), (400, 40), (700, 128), (300, 160), (300, 96)])
+def test_peaked_rows_of_many_states_lose_only_the_roundings(ops, Tk, d, dt):
+    """Rows whose softmax is nearly one key: ds = p (dp - D) is small against D whatever the number of states."""
+    H = 2
+    q, k, v, go = _mk(2, 100, Tk, H, H, d, dt, Tk)
+    q = (q.float() * 3).to(dt)
+    got = _all(ops, q, k, v, go, H, d ** -0.5)
+    R, E = _exact(q, k, v, go, H, d ** -0.5)
+    for n, t in got.items():
+        _check(n, t, R, E)
+    for n in ("dq", "dk"):
+        assert float((got[n].double().cpu() - R[n]).norm() / R[n].norm()) <= 2 ** 0.5 * torch.finfo(dt).eps / (2 * 3 ** 0.5), n
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Tq,Tk,H,G,d", [(1, 129, 1, 1, 8), (130, 200, 2, 2, 24), (33, 150, 4, 2, 32), (70, 260, 2, 1, 136), (140, 193, 2, 2, 160), (3, 640, 4, 1, 152)])
+def test_tiled_kernels_at_the_ends_of_the_head_dims(ops, Tq, Tk, H, G, d, dt):
+    """Over more than 128 states at the smallest and the largest head dims, with a mask and lengths that end inside a tile."""
+    q, k, v, go = _mk(3, Tq, Tk, H, G, d, dt)
+    lens = torch.tensor([Tk, Tk - 5, 1], dtype=torch.int32)
+    mask = torch.rand(3, Tk, generator=torch.Generator().manual_seed(d)) < 0.8
+    mask[2, 0] = True
+    R, E = _exact(q, k, v, go, H, d ** -0.5, G, lens, mask)
+    for n, t in _all(ops, q, k, v, go, H, d ** -0.5, G, lens, mask).items():
+        _check(n, t, R, E)

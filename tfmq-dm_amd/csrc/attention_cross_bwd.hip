@@ -28,8 +28,13 @@ constexpr int DS_TOP = 13;          // where the operand's largest |dp - D| is p
 
 // Three products and the exponentials per score; operand reads run ahead of the products (dealt between them).  One wave a SIMD at d = 128 (315 registers; at
 // 256 it spills).  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 67 us.
+//
+// D comes from the row's own p dp, as over few states (below), without a walk of its own: the walk starts from the D0 of the rounded o, sums
+// delta = sum_j ds_j = D - D0 in fp32 and B = sum_j p_j k_j beside sum_j ds_j k_j, and dq loses delta B at its end.  (D0's rounding is small against
+// D but not against p (dp - D) where few states hold a row's weight: two kept of 1500, bf16, dq 2.5 ... 3.4 times one rounding's bound.)
 template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
+  constexpr float PSHIFT = is_f16<T>() ? 12.0f : 0.0f, UNSHIFT = is_f16<T>() ? 1.0f / 4096.0f : 1.0f;          // p carries 2^PSHIFT
   constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_both(D), VS = stride_rows(D);
   using V8 = typename Vec8<T>::type;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -74,10 +79,10 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
     const float v = p.lse_in[brow];
     lse2 = v == -INFINITY ? INFINITY : v * LOG2E;
   }
-  if (in && hh == 0) p.delta[brow] = dl;
-  // fp16: the operand's power of two, by the largest |dp - D| so far: 2^8 ... 2^9 in the first tile that has one; a larger one moves it down only past
-  // 2^15 (and the sums with it: exact, and rare)
-  float f = 1.0f, dlf = dl, top = 0.0f, lim = 0.0f;
+  lse2 -= PSHIFT;
+  // fp16: the operand's power of two, by the largest |dp - D0| so far: 2^8 ... 2^9 (with p's) in the first tile that has one; a larger one moves it down
+  // only past 2^15 (and the sums with it: exact, and rare)
+  float f = 1.0f, dlf = dl, top = 0.0f, lim = 0.0f, dsum[2] = {0.0f, 0.0f};
 
   const T* kb = static_cast<const T*>(p.k.p) + b * p.k.bs + static_cast<long>(g) * p.d;
   const T* vb = static_cast<const T*>(p.v.p) + b * p.v.bs + static_cast<long>(g) * p.d;
@@ -92,9 +97,9 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
     tv.load(vb, p.v.ts, t * 64, p.Tk, p.d);
   };
   const float c2 = p.scale * LOG2E;
-  v16f acc[NRT];
+  v16f acc[NRT], pk[NRT];
 #pragma unroll
-  for (int t = 0; t < NRT; ++t) acc[t] = zero16();
+  for (int t = 0; t < NRT; ++t) acc[t] = zero16(), pk[t] = zero16();
   if (nt > 0) {
     cur = __ballot(keep_bit(0));
     fetch(0);
@@ -122,6 +127,7 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
       read_rows(0);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
+        if (kt == 1 && D > 128) read_rows(1);          // (at 160 the registers hold the rows or the transposed tiles, not both)
         hold_order();
         v16f s = zero16(), dp = zero16();
 #pragma unroll
@@ -154,9 +160,9 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
           }
           if (__any(mx > lim)) {
             const float row = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float ratio = row > lim ? __builtin_amdgcn_exp2f(static_cast<float>(inv_exponent(row) + 8)) : 1.0f;
-            lim = row > lim ? 32768.0f : lim;
-            f *= ratio, dlf *= ratio, top *= ratio, mx *= ratio;
+            const float ratio = row > lim ? __builtin_amdgcn_exp2f(static_cast<float>(inv_exponent(row) + 8) - PSHIFT) : 1.0f;
+            lim = row > lim ? 32768.0f * UNSHIFT : lim;
+            f *= ratio, dlf *= ratio, top *= ratio, mx *= ratio, dsum[0] *= ratio, dsum[1] *= ratio;
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] *= ratio;
 #pragma unroll
@@ -170,28 +176,44 @@ __global__ __launch_bounds__(256, D <= 96 ? 2 : 1) void k_xattn_dq(XattnP p) {
           for (int r = 0; r < 16; ++r) dp[r] -= dl;
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2)) * dp[r];
-        V8 df[2];
+        for (int r = 0; r < 16; ++r) {
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2));
+          dp[r] *= s[r];
+          dsum[r & 1] += dp[r];
+        }
+        V8 pf[2], df[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) df[u] = frag_regs<T>(s, u);
+        for (int u = 0; u < 2; ++u) pf[u] = frag_regs<T>(s, u), df[u] = frag_regs<T>(dp, u);
         hold_order();
-        if (kt == 0) read_rows(1);
+        if (kt == 0 && D <= 128) read_rows(1);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int t2 = 0; t2 < NRT; ++t2) acc[t2] = mfma16(ct[u][t2], df[u], acc[t2]);
-        if (kt == 0) deal_reads<2 * NRT, 2>();
+          for (int t2 = 0; t2 < NRT; ++t2) {
+            acc[t2] = mfma16(ct[u][t2], df[u], acc[t2]);
+            pk[t2] = mfma16(ct[u][t2], pf[u], pk[t2]);
+          }
+        if (kt == 0 && D <= 128) deal_reads<4 * NRT, 1>();
       }
     }
     cur = nxt;
   }
   top = fmaxf(top, __shfl_xor(top, 32, 64));
+  float dd = dsum[0] + dsum[1];
+  dd = (dd + __shfl_xor(dd, 32, 64)) * UNSHIFT;
   if (!in) return;
+#pragma unroll
+  for (int t = 0; t < NRT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] = __builtin_fmaf(-dd, pk[t][r], acc[t][r]);
   zero_unless(ok, acc);
-  if (is_f16<T>() && hh == 0) p.delta[static_cast<long>(p.B) * p.H * p.Tq + brow] = ok ? top / f : 0.0f;          // (k_xattn_dkv's range)
+  if (hh == 0) {
+    p.delta[brow] = dl + dd / f;
+    if (is_f16<T>()) p.delta[static_cast<long>(p.B) * p.H * p.Tq + brow] = ok ? (top + fabsf(dd)) / f : 0.0f;          // (k_xattn_dkv's range)
+  }
   T* yrow = static_cast<T*>(p.y) + (static_cast<long>(b) * p.Tq + i) * p.H * p.d + static_cast<long>(head) * p.d;
 #pragma unroll
-  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, acc[t], p.scale / f);
+  for (int t = 0; t < NRT; ++t) store16<T>(yrow, t * 32, hh, p.d, acc[t], p.scale * UNSHIFT / f);
 }
 
 // ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form).  A row's probabilities and dp all
