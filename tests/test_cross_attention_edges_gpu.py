@@ -241,3 +241,18 @@ def test_tiled_kernels_at_the_ends_of_the_head_dims(ops, Tq, Tk, H, G, d, dt):
     R, E = _exact(q, k, v, go, H, d ** -0.5, G, lens, mask)
     for n, t in _all(ops, q, k, v, go, H, d ** -0.5, G, lens, mask).items():
         _check(n, t, R, E)
+
+
+@pytest.mark.parametrize("Tq,Tk", [(1, 32768), (200, 20000)])
+def test_a_long_tail_of_small_probabilities_counts(ops, Tq, Tk):
+    """One key holds nearly all of a row's weight and the others, each below fp16's smallest number beside it, hold 2^-10 of it together."""
+    H, d = 2, 32
+    q = torch.ones(1, Tq, H * d).half()
+    k, v = torch.full((1, Tk, H * d), -17.5 / d).half(), torch.ones(1, Tk, H * d).half()
+    k[0, 5], v[0, 5] = 0.0, 0.0
+    v[0, :, ::3] = -2.0
+    got = _all(ops, q, k, v, q, H, 1.0)
+    R, E = _exact(q, k, v, q, H, 1.0)
+    assert float(R["o"].abs().min()) > 2.0 ** -12
+    for n in ("o", "lse"):
+        _check(n, got[n], R, E)

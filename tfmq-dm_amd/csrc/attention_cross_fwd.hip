@@ -5,7 +5,8 @@
 // One pass over the keys with the running maximum and sum.  A wave owns 32 rows as the COLUMNS of S^T = K Q^T: a lane has one row, its maximum and
 // sum are registers, and the probabilities are already the operand that O^T = V^T P^T wants.  K and V tiles of 64 keys are loaded into registers
 // while the previous tile is multiplied, and stored to LDS row-major; V is read transposed by ds_read_b64_tr_b16.  Scores, statistics and sums are fp32;
-// the probabilities are rounded to the operand type for the second product (they are at most 2^8, the sum takes them unrounded).
+// the probabilities are rounded to the operand type for the second product (the sum takes them unrounded).  They are taken against a reference below the
+// maximum: fp16 ones lie up to 2^15, so that a long tail of small ones beside one large counts down to 2^-32 of it and not 2^-25.
 #include "attention_cross.hpp"
 
 using namespace xattn;
@@ -58,7 +59,8 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
     tv.load(vb, p.v.ts, t * 64, p.Tk, p.d);
   };
   const float c2 = p.scale * LOG2E;
-  float m = -INFINITY, l = 0.0f;
+  constexpr float BELOW = std::is_same<T, _Float16>::value ? 7.0f : 0.0f;          // (with the late rescaling's 2^8 below fp16's largest)
+  float m = -INFINITY, l = 0.0f;          // the reference, 2^BELOW under the maximum, and the sum against it
   v16f o[NRT];
 #pragma unroll
   for (int t = 0; t < NRT; ++t) o[t] = zero16();
@@ -92,8 +94,9 @@ __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;          // (scale > 0)
-      // the sums move to a new maximum only where one has risen by more than 2^8 since (or there was none): probabilities up to 256 are as exact as
-      // those up to 1, and past the first tile this is rare
+      mx -= BELOW;
+      // the sums move to a new maximum only where one has risen by more than 2^8 since (or there was none): probabilities up to 256 times those of the
+      // maximum are as exact as those, and past the first tile this is rare
       if (__any(mx > m + 8.0f)) {
         const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
         m = mn;
