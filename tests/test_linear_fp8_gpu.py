@@ -271,3 +271,15 @@ def test_slices_of_a_long_reduction(ops, M, K, N, out):
     qx, qw = O.dequant(*O.quant_rows(x)), O.dequant(*O.quant(w, 128))
     A = _terms(qx, qw)
     _check(y, qx @ qw.t() + b.double(), (A[0] + b.double().abs(), A[1]), (K + 127) // 128 + 1, out)
+
+
+def test_a_packed_bias_is_a_copy(ops):
+    """pack_w_fp8 and load_w_fp8 lay a layer out once: an update in place of the bias they were given changes the packed layer no more than one of the weight."""
+    x = _x(40, 300, torch.float16).to(DEV)
+    w, b = _x(200, 300, torch.float32, 1).to(DEV), torch.randn(200, generator=torch.Generator().manual_seed(3)).to(DEV)
+    pw = ops.pack_w_fp8(w, b)
+    ld = ops.load_w_fp8(pw.q[:, :300].view(torch.float8_e4m3fn), pw.scale, b)
+    y = ops.linear_fp8(x, pw)
+    w.zero_()
+    b.zero_()
+    assert torch.equal(ops.linear_fp8(x, pw), y) and torch.equal(ops.linear_fp8(x, ld), y)

@@ -1858,7 +1858,7 @@ def _bias_f32(bias, N: int, d: int, name: str):
     if tuple(bias.shape) != (N,):
         raise TfmqError(f"{name}: bias must be [{N}], got {tuple(bias.shape)}")
     _same_device(d, bias)
-    return bias.detach().float().contiguous()
+    return bias.detach().to(torch.float32, copy=True).contiguous()          # (the layer's own, as the weight's bytes are)
 
 
 def pack_w_fp8(w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> PackedFp8:
