@@ -157,3 +157,23 @@ def test_captured_samplers_take_masks(run, kind, pair, monkeypatch):
     with pytest.raises(TfmqError, match="context_masks"):
         plain.sample_nhwc(xT, ctx, uc, cond_mask=m)
     assert rel_l2(every, sample(plain, ctx, uc)) <= 8e-2      # (the bar of a guided four-step trajectory: guidance amplifies a step's 3e-2)
+
+
+def test_a_refused_forward_leaves_no_mask_behind(run, golden):
+    """A forward that raises inside a block (here: a layer that is not quantised cannot take a mask) ends like any other: a block run on its own afterwards
+    takes no mask."""
+    from tfmq_dm_amd._lib import TfmqError
+    from tfmq_dm_amd.engine import LdmUNetEngine
+    eng, x, t, ctx = run
+    g = golden("f11_ldm_tiny")
+    fp = LdmUNetEngine({k[3:]: T(g[k]) for k in g.files if k.startswith("sd/")}, CFG, DEV)
+    fp.prepare()
+    name = next(n[:-len(".attn2.to_q")] for n in fp.layers if n.endswith(".attn2.to_q"))
+    C = fp.sd[name + ".norm2.weight"].shape[0]
+    tok = torch.randn(ctx.shape[0], 16, C, generator=torch.Generator().manual_seed(1)).to(DEV)
+    fp._ctx_pad = None
+    want = fp._tblock(name, tok, ctx)
+    with pytest.raises(TfmqError, match="context_mask"):
+        fp.forward(x, t, ctx, context_mask=lengths(ctx, *[1] * ctx.shape[0]))
+    fp._ctx_pad = None
+    assert torch.equal(fp._tblock(name, tok, ctx), want)

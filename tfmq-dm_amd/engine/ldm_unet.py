@@ -651,6 +651,8 @@ class LdmUNetEngine(DdimUNetEngine):
                 return self._forward(*a, **k)
         except UnitReached:
             return None
+        finally:
+            self._ctx_mask = None       # (a block run on its own takes none, also after a forward that raised)
 
     def _forward(self, x: torch.Tensor, t: Optional[torch.Tensor] = None, context: Optional[torch.Tensor] = None,
                 taps: Optional[dict] = None, pair_prefix: bool = False, context_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -726,5 +728,4 @@ class LdmUNetEngine(DdimUNetEngine):
         for i in range(_n_children(self.sd, "output_blocks")):
             h = self._seq(f"output_blocks.{i}", h, hs.pop(), ctx, rowadd, taps)
         h, _ = self._gn("out.0", h, None, True, None, eps=1e-5, half=self._fp_conv_half_ok(L["out.2"]))
-        self._ctx_mask = None       # (a block run on its own takes none)
         return L["out.2"].run(h, pad=(1, 1, 1, 1), want_stats=False)
