@@ -171,6 +171,7 @@ def test_a_refused_forward_leaves_no_mask_behind(run, golden):
     name = next(n[:-len(".attn2.to_q")] for n in fp.layers if n.endswith(".attn2.to_q"))
     C = fp.sd[name + ".norm2.weight"].shape[0]
     tok = torch.randn(ctx.shape[0], 16, C, generator=torch.Generator().manual_seed(1)).to(DEV)
+    fp.forward(x, t, ctx)          # (the stream's type is that of the last forward)
     fp._ctx_pad = None
     want = fp._tblock(name, tok, ctx)
     with pytest.raises(TfmqError, match="context_mask"):
