@@ -24,8 +24,8 @@ def ops():
     return ops
 
 
-def _exact(q, k, v, go, H, scale, G=None, kv_lens=None, mask=None):
-    """64-bit results and the bounds above."""
+def _exact(q, k, v, go, H, scale, G=None, kv_lens=None, mask=None, late=None):
+    """64-bit results and the bounds above (late: whether D is put right afterwards)."""
     dt = q.dtype
     u = torch.finfo(dt).eps / 2
     half = dt == torch.float16
@@ -60,9 +60,9 @@ def _exact(q, k, v, go, H, scale, G=None, kv_lens=None, mask=None):
             ds, low = p * diff, 2.0 ** -126 * (a + (p * a).sum(-1, keepdim=True))
             und = 2.0 ** -33 * diff.abs() if half else torch.zeros_like(diff)
             Ed = u * ds.abs() + 3 * f * p * (a + A) + low
-            late = 2 * u * (u + 2 * f) * A * p + (u * A * 2.0 ** -25 if half else 0.0) if Tk > 128 else 0.0
+            more = 2 * u * (u + 2 * f) * A * p + (u * A * 2.0 ** -25 if half else 0.0) if (Tk > 128 if late is None else late) else 0.0
             R["dq"][b, :, cq] = scale * ds @ kk
-            E["dq"][b, :, cq] = scale * (Ed + late + und.amax(-1, keepdim=True) + n * 2.0 ** -24 * ds.abs()) @ kk.abs() + tiny
+            E["dq"][b, :, cq] = scale * (Ed + more + und.amax(-1, keepdim=True) + n * 2.0 ** -24 * ds.abs()) @ kk.abs() + tiny
             R["dk"][b, idx, ck] += scale * ds.t() @ qq
             R["dv"][b, idx, ck] += p.t() @ gg
             E["dk"][b, idx, ck] += scale * (Ed + und.amax() + rep * Tq * 2.0 ** -24 * ds.abs()).t() @ qq.abs()
@@ -256,3 +256,89 @@ def test_a_long_tail_of_small_probabilities_counts(ops, Tq, Tk):
     assert float(R["o"].abs().min()) > 2.0 ** -12
     for n in ("o", "lse"):
         _check(n, got[n], R, E)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_too_far_apart_for_32_bit_offsets(ops, dt):
+    """Few states under query, gradient and output rows 2^30 bytes apart: the kernels that address an item's rows with 32 bits leave them to the tiled ones."""
+    B, Tq, Tk, H, d = 1, 3, 20, 2, 64
+    q, k, v, go = _mk(B, Tq, Tk, H, H, d, dt)
+    how = dict(q_lens=torch.tensor([3], dtype=torch.int32, device=DEV), kv_lens=torch.tensor([17], dtype=torch.int32, device=DEV))
+    buf = torch.empty(2 * (1 << 29) + 4 * H * d, dtype=dt, device=DEV)
+
+    def far(t, at):
+        w = torch.as_strided(buf, t.shape, (3 << 29, 1 << 29, 1), at * H * d)
+        w.copy_(t)
+        return w
+    (kd, vd), qd, gd = _fused_dev(k, v), far(q, 0), far(go, 1)
+    o, lse = ops.cross_attention(qd, kd, vd, H, 0.125, want_lse=True, **how)
+    got = dict(zip(("o", "lse", "dq", "dk", "dv"), (o, lse) + tuple(ops.cross_attention_bwd(qd, kd, vd, far(o, 2), lse, gd, H, 0.125, **how))))
+    R, E = _exact(q, k, v, go, H, 0.125, None, torch.tensor([17]), None, late=True)
+    for n, t in got.items():
+        _check(n, t, R, E)
+
+
+@pytest.mark.parametrize("Tk", [50, 200])
+def test_queries_and_states_of_stride_zero(ops, Tk):
+    """One query set for every item, one query row for every token, one state for every key."""
+    B, Tq, H, d = 3, 20, 2, 64
+    q, k, v, go = _dev(*_mk(B, Tq, Tk, H, H, d, torch.float16, fused=False))
+    for qe, ke, ve in ((q[:1].expand(B, -1, -1), k, v), (q[:, :1].expand(-1, Tq, -1), k, v), (q, k[:, :1].expand(-1, Tk, -1), v[:, :1].expand(-1, Tk, -1))):
+        want = ops.cross_attention(qe.contiguous(), ke.contiguous(), ve.contiguous(), H, 0.125, want_lse=True)
+        got = ops.cross_attention(qe, ke, ve, H, 0.125, want_lse=True)
+        grads = zip(ops.cross_attention_bwd(qe, ke, ve, *got, go[:, :1].expand(-1, Tq, -1), H, 0.125),
+                    ops.cross_attention_bwd(qe.contiguous(), ke.contiguous(), ve.contiguous(), *want, go[:, :1].expand(-1, Tq, -1).contiguous(), H, 0.125))
+        assert all(torch.equal(a, b) for a, b in list(zip(got, want)) + list(grads))
+
+
+@pytest.mark.parametrize("Tk", [77, 150])
+def test_more_than_2_to_the_31_outputs(ops, Tk):
+    """The last item of a call whose queries, outputs and gradients pass 2^31 elements equals a call on that item alone."""
+    B, Tq, H, d = 17, 65536, 16, 128
+    g = torch.Generator(device=DEV).manual_seed(Tk)
+    q = torch.empty(B, Tq, H * d, dtype=torch.bfloat16, device=DEV)
+    q[:-1].fill_(0.25)
+    q[-1].normal_(generator=g)
+    kv = torch.randn(B, Tk, 2 * H * d, dtype=torch.bfloat16, device=DEV, generator=g)
+    k, v = kv[..., :H * d], kv[..., H * d:]
+    assert q.numel() > 1 << 31
+    o, lse = ops.cross_attention(q, k, v, H, 0.1, want_lse=True)
+    dq, dk, dv = ops.cross_attention_bwd(q, k, v, o, lse, q, H, 0.1)
+    o1, lse1 = ops.cross_attention(q[-1:], k[-1:], v[-1:], H, 0.1, want_lse=True)
+    dq1, dk1, dv1 = ops.cross_attention_bwd(q[-1:], k[-1:], v[-1:], o1, lse1, q[-1:], H, 0.1)
+    assert torch.equal(o[-1:], o1) and torch.equal(lse[-1:], lse1) and torch.equal(dq[-1:], dq1)
+    for a, b in ((dk, dk1), (dv, dv1)):          # (alone, the rows are cut into other slices: the same but for the order of fp32 sums and one rounding)
+        assert float((a[-1:].double() - b.double()).norm() / b.double().norm()) <= torch.finfo(torch.bfloat16).eps / 2
+
+
+def test_two_threads_at_once(ops):
+    """Calls from two host threads, each on a stream of its own, give what they give one after the other."""
+    import threading
+    sets = [_dev(*_mk(2, 300 + 50 * i, 70 + 100 * i, 4, 2, 64, torch.float16, seed=i, fused=False)) for i in range(2)]
+    pws = [ops.pack_w_fp8(torch.randn(512 + 64 * i, 256, generator=torch.Generator().manual_seed(i)).to(DEV)) for i in range(2)]
+
+    def one(i):
+        q, k, v, go = sets[i]
+        o, lse = ops.cross_attention(q, k, v, 4, 0.125, 2, want_lse=True)
+        y = ops.linear_fp8(o, pws[i])
+        return (o, lse, y) + tuple(ops.cross_attention_bwd(q, k, v, o, lse, go, 4, 0.125, 2)) + tuple(ops.linear_fp8_bwd(o, y, pws[i]))
+    want = [one(0), one(1)]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got[i] = one(i)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:          # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])), i

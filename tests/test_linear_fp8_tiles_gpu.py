@@ -115,3 +115,54 @@ def test_large_products_replayed(ops):
         assert all(torch.equal(p, q) for p, q in zip(out, want[i])), i
         _ = step(xs[0], bs[0])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dx,dg", [(F32, F16), (BF16, F32), (F16, BF16)])
+@pytest.mark.parametrize("M,K,N", [(40, 200, 96), (1333, 1000, 777)])
+def test_gradients_of_mixed_types(ops, M, K, N, dx, dg):
+    """x and gy of different types: gx in gy's, gw in fp32."""
+    x, gy, w = _x(M, K, dx), _x(M, N, dg, 2), _x(N, K, F32, 1)
+    pw = ops.pack_w_fp8(w.to(DEV))
+    gx, gw = ops.linear_fp8_bwd(x.to(DEV), gy.to(DEV), pw)
+    assert gx.dtype == dg and gw.dtype == F32
+    _check_product(gx.cpu(), O.dequant(*O.quant_rows(gy)), O.dequant(*O.quant(w, 128)).t().contiguous(), None, _cdiv(N, 128), dg, "gx")
+    _check_product(gw.cpu(), O.dequant(*O.quant_rows(gy.t().contiguous())), O.dequant(*O.quant_rows(x.t().contiguous())), None, _cdiv(M, 128), F32, "gw")
+
+
+@pytest.mark.parametrize("out", [F16, F32])
+def test_other_output_types_of_large_products(ops, out):
+    for M, K, N in ((1100, 300, 1000), (4100, 300, 1100), (4000, 130, 4090)):
+        x, w = _x(M, K, BF16), _x(N, K, F32, 1)
+        y = ops.linear_fp8(x.to(DEV), ops.pack_w_fp8(w.to(DEV)), out)
+        assert y.dtype == out
+        _check_product(y.cpu(), O.dequant(*O.quant_rows(x)), O.dequant(*O.quant(w, 128)), None, _cdiv(K, 128), out, (M, K, N))
+
+
+def test_more_than_2_to_the_31_elements(ops):
+    """Rows on both sides of 2^31 elements of x, y, gy and gx, and the weight's gradient over all of them."""
+    M, K, N = (1 << 31) // 640 + 1000, 640, 648
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.empty(M, K, dtype=BF16, device=DEV)
+    x[:] = torch.randn(1024, K, device=DEV, generator=g).to(BF16).repeat(_cdiv(M, 1024), 1)[:M]
+    w = torch.randn(N, K, device=DEV, generator=g)
+    pw = ops.pack_w_fp8(w)
+    at = torch.tensor([0, 1000, (1 << 31) // 648, (1 << 31) // 640, (1 << 31) // 640 + 1, M - 1000, M - 1])
+    rows = x[at.to(DEV)].cpu()
+    y = ops.linear_fp8(x, pw)
+    qw = O.dequant(*O.quant(w.cpu(), 128))
+    qx = O.dequant(*O.quant_rows(rows))
+    _check(y[at.to(DEV)], qx @ qw.t(), _terms(qx, qw), 5, BF16)
+    gx, gw = ops.linear_fp8_bwd(x, y, pw)
+    gy = y[at.to(DEV)].cpu()
+    qg = O.dequant(*O.quant_rows(gy))
+    _check(gx[at.to(DEV)], qg @ qw, _terms(qg, qw.t()), 6, BF16)
+    # every block of 128 tokens is one of eight (the rows repeat after 1024), the last one ragged
+    ref, A = torch.zeros(N, K, dtype=torch.float64), torch.zeros(N, K, dtype=torch.float64)
+    full, rest = M // 128, M % 128
+    for i in range(8):
+        for r0, n, times in ((i * 128, 128, (full - i + 7) // 8), (full % 8 * 128, rest, 1 if i == 0 and rest else 0)):
+            if times:
+                gc = O.dequant(*O.quant_rows(y[r0:r0 + n].cpu().t().contiguous()))
+                xc = O.dequant(*O.quant_rows(x[r0:r0 + n].cpu().t().contiguous()))
+                ref, A = ref + times * (gc @ xc.t()), A + times * (gc.abs() @ xc.abs().t())
+    _check(gw, ref, (A, A * 0), _cdiv(M, 128), F32)
