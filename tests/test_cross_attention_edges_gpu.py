@@ -342,3 +342,44 @@ def test_two_threads_at_once(ops):
     assert not errors
     for i in range(2):
         assert all(torch.equal(a, b) for a, b in zip(got[i], want[i])), i
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("Tk,kept", [(16, 16), (100, 20), (200, 16), (300, 300)])
+def test_far_scores_do_not_unbalance_the_gradients(ops, Tk, kept, dt):
+    """Scores near +-100, rows whose softmax is nearly one key.  Recomputed probabilities sum to one only up to the rounding of lse, some 2^-23 |lse|, and that
+    times D is not small against ds = p (dp - D).  All inputs are small integers: scores and dp are exact, a probability is off by
+    e = 2^-21 + 3 2^-24 max|score| relative to the row's others and in common, so ds before its rounding by at most e (|ds| + p sum |ds|) and by the fp32
+    sum D, (n + 4) 2^-24 p (|dp| + sum p |dp|)."""
+    B, Tq, H, d = 1, 64, 1, 32
+    u, half = torch.finfo(dt).eps / 2, dt == torch.float16
+    g = torch.Generator().manual_seed(Tk)
+    q, k, v, go = (torch.zeros(B, T, d) for T in (Tq, Tk, Tk, Tq))
+    q[:, ::2, 0], q[:, 1::2, 0] = 1, -1
+    k[0, :, 0] = torch.randint(80, 94, (Tk,), generator=g).float()
+    mask = torch.zeros(B, Tk, dtype=torch.bool)
+    mask[0, torch.randperm(Tk, generator=g)[:kept]] = True
+    idx = mask[0].nonzero()[:, 0]
+    k[0, idx[0], 0], k[0, idx[1], 0] = 102, 72
+    k[..., 1:] = torch.randint(-2, 3, k[..., 1:].shape, generator=g).float()
+    v[:] = 8 + torch.randint(-3, 4, v.shape, generator=g).float()
+    go[:] = 2 + torch.randint(-2, 3, go.shape, generator=g).float()
+    q, k, v, go = (t.to(dt) for t in (q, k, v, go))
+    got = _all(ops, q, k, v, go, H, 1.0, None, None, mask)
+    R, _ = _exact(q, k, v, go, H, 1.0, None, None, mask)
+    qq, kk, vv, gg = (t[0].double() for t in (q, k[:, idx], v[:, idx], go))
+    s, dp = qq @ kk.t(), gg @ vv.t()
+    p = torch.softmax(s, -1)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    e = 2.0 ** -21 + 3 * 2.0 ** -24 * float(s.abs().max())
+    und = 2.0 ** -33 * (dp - (p * dp).sum(-1, keepdim=True)).abs().amax() if half else 2.0 ** -126
+    A = (p * dp.abs()).sum(-1, keepdim=True)
+    # over many states D starts from the rounded o: the correction is itself rounded twice
+    more = 2 * u * u * (p @ vv.abs() * gg.abs()).sum(-1, keepdim=True) * p if Tk > 128 else 0.0
+    Ed = u * ds.abs() + e * (ds.abs() + p * ds.abs().sum(-1, keepdim=True)) + (kept + 4) * 2.0 ** -24 * p * (dp.abs() + A) + und + more
+    tiny = 2.0 ** -25 if half else 2.0 ** -126
+    E = {"dq": torch.zeros_like(R["dq"]), "dk": torch.zeros_like(R["dk"])}
+    E["dq"][0] = (Ed + kept * 2.0 ** -24 * ds.abs()) @ kk.abs() + u * R["dq"][0].abs() + tiny
+    E["dk"][0, idx] = (Ed + Tq * 2.0 ** -24 * ds.abs()).t() @ qq.abs() + u * R["dk"][0, idx].abs() + tiny
+    for n in E:
+        _check(n, got[n], R, E)

@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
 }
 
 // ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form).  A row's probabilities and dp all
-// stay in registers and D is their own sum of p dp.  From o, which the forward has rounded, D is off by that rounding, and few states leave
+// stay in registers and D is their own mean of dp.  From o, which the forward has rounded, D is off by that rounding, and few states leave
 // ds = p (dp - D) small against D: bf16 gradients of q and k at 18 states, of which a mask and lengths kept about three, were 1.9 times as far from the exact
 // ones as from one rounding, now 1.4 (the ds operand's and the result's).  8 x 4096 x 77, 8 heads of 40: 24 us for 63 MB of q, go and dq; reading o
 // instead of holding the scores, at four waves a SIMD against three, 25.
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
     const bool in = w.row < r_end, ok = any && in && w.i < qlen;
     const unsigned yoff = w.i * yts + w.hi * hs, loff = in && hh == 0 ? static_cast<unsigned>(w.row) * 4 : NOWHERE;
     const float lse2 = ok && lse != -INFINITY ? lse * LOG2E : INFINITY;
-    float dl = 0.0f, hi = -INFINITY, lo = INFINITY;
+    float dl = 0.0f, sum = 0.0f, hi = -INFINITY, lo = INFINITY;
     V8 df[2 * NKT];
     v16f ps[NKT], dps[NKT];
 #pragma unroll
@@ -282,13 +282,17 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
       for (int r = 0; r < 16; ++r) {
         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse2));
         dl = __builtin_fmaf(pr, dp[r], dl);
+        sum += pr;
         if (is_f16<T>()) hi = fmaxf(hi, dp[r]), lo = fminf(lo, dp[r]);          // (a dropped key's dp is a kept one's)
         s[r] = pr;
       }
       ps[kt] = s;
       dps[kt] = dp;
     }
+    // (the p sum to 1 up to the rounding of lse, 2^-23 |lse|; times D that is not small against ds where a row is nearly one key)
+    sum += __shfl_xor(sum, 32, 64);
     dl += __shfl_xor(dl, 32, 64);
+    dl = sum != 0.0f ? dl / sum : 0.0f;
     float f = 1.0f, inv_f = 1.0f;
     if (is_f16<T>()) {
       const float mx = fmaxf(fmaxf(hi, __shfl_xor(hi, 32, 64)) - dl, dl - fminf(lo, __shfl_xor(lo, 32, 64)));
