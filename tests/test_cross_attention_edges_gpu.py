@@ -383,3 +383,13 @@ def test_far_scores_do_not_unbalance_the_gradients(ops, Tk, kept, dt):
     E["dk"][0, idx] = (Ed + Tq * 2.0 ** -24 * ds.abs()).t() @ qq.abs() + u * R["dk"][0, idx].abs() + tiny
     for n in E:
         _check(n, got[n], R, E)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_million_states(ops, dt):
+    Tk, H, d = (1 << 20) + 77, 1, 32
+    q, k, v, go = _mk(1, 2, Tk, H, H, d, dt)
+    lens = torch.tensor([Tk - 100], dtype=torch.int32)
+    R, E = _exact(q, k, v, go, H, d ** -0.5, None, lens)
+    for n, t in _all(ops, q, k, v, go, H, d ** -0.5, None, lens).items():
+        _check(n, t, R, E)

@@ -166,3 +166,19 @@ def test_more_than_2_to_the_31_elements(ops):
                 xc = O.dequant(*O.quant_rows(x[r0:r0 + n].cpu().t().contiguous()))
                 ref, A = ref + times * (gc @ xc.t()), A + times * (gc.abs() @ xc.abs().t())
     _check(gw, ref, (A, A * 0), _cdiv(M, 128), F32)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,K,N", [(20000, 1, 1), (20000, 130, 7), (17000, 64, 33), (40, 1 << 20, 40), (2, 1 << 22, 3)])
+def test_ends_of_the_sizes(ops, M, K, N, dt):
+    """One column or channel under many rows, and the longest reductions."""
+    x, w = _x(M, K, dt), _x(N, K, F32, 1) * K ** -0.5
+    pw = ops.pack_w_fp8(w.to(DEV))
+    y = ops.linear_fp8(x.to(DEV), pw)
+    _check_product(y.cpu(), O.dequant(*O.quant_rows(x)), O.dequant(*O.quant(w, 128)), None, _cdiv(K, 128), dt, (M, K, N))
+    if M * K > 1 << 22:
+        return
+    gy = _x(M, N, dt, 2)
+    gx, gw = ops.linear_fp8_bwd(x.to(DEV), gy.to(DEV), pw)
+    _check_product(gx.cpu(), O.dequant(*O.quant_rows(gy)), O.dequant(*O.quant(w, 128)).t().contiguous(), None, _cdiv(N, 128), dt, "gx")
+    _check_product(gw.cpu(), O.dequant(*O.quant_rows(gy.t().contiguous())), O.dequant(*O.quant_rows(x.t().contiguous())), None, _cdiv(M, 128), F32, "gw")
