@@ -1,11 +1,11 @@
 // Gradients of the cross attention (attention_cross_fwd.hip): with p_ij = exp(scale q_i k_j - lse_i), dp_ij = go_i v_j and
-// D_i = sum_c o_ic go_ic = sum_j p_ij dp_ij,
+// D_i = sum_j p_ij dp_ij = sum_c o_ic go_ic,
 //     ds_ij = p_ij (dp_ij - D_i),   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij go_i.
 //
 // Two kernels recompute p from the saved lse, each with its sums in registers and no atomics: k_xattn_dq walks the keys of 128 rows (a lane owns a row,
 // as in the forward), k_xattn_dkv walks the rows of 128 keys (a lane owns a key; shared key heads sum over their query heads because those are
-// further rows).  Seven products instead of the five of a fused pass, for results that are the same bits every time.  Where few key blocks face
-// many rows -- 77 states under 4096 tokens -- the rows are cut into slices whose fp32 sums are added in order.
+// further rows).  Seven products (eight over more than 128 states) instead of the five of a fused pass, for results that are the same bits every
+// time.  Where few key blocks face many rows -- 77 states under 4096 tokens -- the rows are cut into slices whose fp32 sums are added in order.
 //
 // fp16 range: ds has the size of p go v, which may lie far below fp16's normal numbers (a loss averaged over many tokens, small states) or above its largest
 // (states of thousands).  The ds operand is therefore carried with a power of two by the largest |dp - D| itself -- of the row in dq, of the slice's rows in
@@ -26,12 +26,15 @@ __device__ __forceinline__ int inv_exponent(float a) {
 }
 constexpr int DS_TOP = 13;          // where the operand's largest |dp - D| is put when it is known beforehand: 2^13 ... 2^14
 
-// Three products and the exponentials per score; operand reads run ahead of the products (dealt between them).  One wave a SIMD at d = 128 (315 registers; at
-// 256 it spills).  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 67 us.
+// Four products and the exponentials per score; operand reads run ahead of the products (dealt between them; at d = 160 the registers hold the rows or the
+// transposed tiles).  One wave a SIMD from d = 72 on (d = 128: 409 registers; at two waves 80 and 96 spill 144 - 220 bytes).  4 x 1000 x 1500, 16 heads on 4 of
+// 128, lengths and mask drawn: 75 us, MFMA 16 % busy, 0.66 waves a SIMD on average.
 //
 // D comes from the row's own p dp, as over few states (below), without a walk of its own: the walk starts from the D0 of the rounded o, sums
 // delta = sum_j ds_j = D - D0 in fp32 and B = sum_j p_j k_j beside sum_j ds_j k_j, and dq loses delta B at its end.  (D0's rounding is small against
-// D but not against p (dp - D) where few states hold a row's weight: two kept of 1500, bf16, dq 2.5 ... 3.4 times one rounding's bound.)
+// D but not against p (dp - D) where few states hold a row's weight: two kept of 1500, bf16, dq 2.5 times its roundings' bound.)  The fourth product took this
+// kernel from 67 to 75 us; the whole backward pass of 4 x 1000 x 1500 and 16 heads on 4, bf16, from 113 to 121 at d = 40, 198 to 227 at 80 (two waves a SIMD
+// before), 273 to 291 at 128 and 380 to 417 at 160.
 template <typename T, int D>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
   constexpr float PSHIFT = is_f16<T>() ? 12.0f : 0.0f, UNSHIFT = is_f16<T>() ? 1.0f / 4096.0f : 1.0f;          // p carries 2^PSHIFT
@@ -219,8 +222,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void k_xattn_dq(XattnP p) {
 // ---- dq against up to 128 states: K and V stay in LDS, the waves walk over rows without barriers (k_xattn_short's form).  A row's probabilities and dp all
 // stay in registers and D is their own mean of dp.  From o, which the forward has rounded, D is off by that rounding, and few states leave
 // ds = p (dp - D) small against D: bf16 gradients of q and k at 18 states, of which a mask and lengths kept about three, were 1.9 times as far from the exact
-// ones as from one rounding, now 1.4 (the ds operand's and the result's).  8 x 4096 x 77, 8 heads of 40: 24 us for 63 MB of q, go and dq; reading o
-// instead of holding the scores, at four waves a SIMD against three, 25.
+// ones as from one rounding, now 1.4 (the ds operand's and the result's).  8 x 4096 x 77, 8 heads of 40: 26 us for 63 MB of q, go and dq, VALU 33 % busy, 1.5
+// waves a SIMD.
 constexpr int dq_short_waves(int D, int NKT) { return D <= 64 && NKT <= 2 ? 4 : NKT <= (D <= 32 ? 4 : D <= 64 ? 3 : D <= 96 ? 2 : 0) ? 3 : 2; }
 template <typename T, int D, int NKT>
 __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(XattnP p) {
@@ -326,8 +329,9 @@ __global__ __launch_bounds__(256, dq_short_waves(D, NKT)) void k_xattn_dq_short(
 }
 
 // ---- dk and dv: four products per score, both sums in registers (2 x d fp32 a key).  Staging the next tile costs registers that d = 128 does not have twice:
-// one wave a SIMD (436 registers), two LDS buffers spill (120 -> 400 us).  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 91 us;
-// 8 x 4096 x 77, 8 heads of 40: 27 us, of whose 128 keys a workgroup 77 are there.
+// one wave a SIMD (436 registers), two LDS buffers spill (120 -> 400 us).  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 91 us, MFMA 12 % busy,
+// 0.42 waves a SIMD on average (key blocks behind an item's length leave at once, and the slices are chosen by the stored length); 8 x 4096 x 77, 8 heads
+// of 40: 27 us, of whose 128 keys a workgroup 77 are there.
 template <int D> constexpr int dkv_rows() { return D <= 128 ? 64 : 32; }
 
 template <typename T, int D>

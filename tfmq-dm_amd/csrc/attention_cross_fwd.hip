@@ -13,9 +13,9 @@ using namespace xattn;
 
 namespace {
 
-// Bound by the VALU: a score costs an FMA, an exponential, half a maximum, an addition and half a conversion beside 4 d / 64 matrix cycles per 64 of them.
-// 2 x 4096 x 4096, 16 heads of 64, lengths drawn: 130 us, VALU 70 % busy, three waves a SIMD; four (128 registers) took 127 -> 127 - 130, two LDS buffers
-// spill.  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 39 us.
+// A score costs an FMA, an exponential, half a maximum, an addition and half a conversion beside 4 d / 64 matrix cycles per 64 of them: the VALU is the busier
+// pipe.  2 x 4096 x 4096, 16 heads of 64, lengths drawn: 130 us (mean over six draws); VALU 52 % and MFMA 30 % busy, 2.0 waves a SIMD of the three that
+// fit (the workgroups run in the items' order, whatever their lengths); four (128 registers) took 127 -> 127 - 130, two LDS buffers spill.  4 x 1000 x 1500, 16 heads on 4 of 128, lengths and mask drawn: 39 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void k_xattn_fwd(XattnP p) {
   constexpr int NKS = nks(D), NRT = nrt(D), KS = stride_rows(D), VS = stride_cols(D);

@@ -310,8 +310,8 @@ __device__ __forceinline__ int key_w(int r) { return (r & 3) | ((r >> 2) & 4); }
 // stored.
 // What bounds it: the LDS-DMA of the operands, the fragment reads, the matrix instructions and the VALU that scales every block's result take about as long as
 // each other, and the barrier of a stage lets them overlap only between the two waves of a SIMD.  16384 x 1280 x 10240 fp16 out (256 x 256 tiles, half the
-// operand bytes of 128 x 128): 265 us, 1.6 PFLOP/s, MFMA busy 38 %, VALU 31 %,
-// LDS 28 % and 13 % conflicts of the LDS-DMA's writes with the reads.  Fragments of block b + 1 in registers under the products of
+// operand bytes of 128 x 128): 262 us, 1.6 PFLOP/s, MFMA busy 38 %, VALU 37 %,
+// LDS 32 % and 14 % conflicts of the LDS-DMA's writes with the reads (nothing is full: the steps of a block follow each other).  Fragments of block b + 1 in registers under the products of
 // b: 256 x 128 tiles spill 68 bytes, 177 against 134 us at 8192 x 1280 x 10240; without spills (eight waves of 32 x 64) 44.7 against 41.6 us at
 // 1024 x 5120 x 1280.  8192 x 320 x 2560 (three blocks a tile): 24 us, 42 MB of stores.
 template <int BM, int BN, int WM, int WN, int YDT, bool SBROW, int S>
@@ -798,9 +798,10 @@ int launch_grads(tfmq_handle h, GemmF8P gw, GemmF8P gx, hipStream_t st) {
   return TFMQ_OK;
 }
 
-// ---- which kernel multiplies.  Tiles of 256 x 256 where they fill the card in whole rounds (at least three quarters of all), else 128 x 128.  us, 128^2
-// against 256^2: 16384 x 1280 x 10240 (10 rounds, full) 338 / 288; 6144 x 1280 x 3840 (360 tiles, 70 %) 48.9 / 50.1; 8192 x 320 x 2560 (320 tiles, 62 %)
-// 21.9 / 25.4; 4096 x 1280 x 1280 (80 tiles, 31 %) 16.8 / 24.5.
+// ---- which kernel multiplies.  Tiles of 256 x 256 where they fill the card in whole rounds (at least three quarters of all), else 128 x 128.  us of the
+// product alone, 128^2 / 256^2 in turn on one box, fastest of six, normal values: 16384 x 1280 x 10240 (10 rounds, full) 280 / 242; 8192 x 1280 x 10240 (five,
+// full) 138 / 122; 6144 x 1280 x 3840 (360 tiles, 70 %) 43 / 50; 8192 x 320 x 2560 (320 tiles, 62 %) 19.6 / 23.1; 4096 x 1280 x 1280 (80 tiles, 31 %)
+// 14.6 / 22.3.
 bool big_tiles(tfmq_handle h, long M, int N) {
   const long nt = static_cast<long>(ceil_div(M, 256)) * ceil_div(N, 256), cu = h->cu_count;
   return nt >= cu && nt * 4 >= (nt + cu - 1) / cu * cu * 3;

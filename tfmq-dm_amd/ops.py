@@ -1863,7 +1863,7 @@ def _bias_f32(bias, N: int, d: int, name: str):
 
 def pack_w_fp8(w: torch.Tensor, bias: Optional[torch.Tensor] = None) -> PackedFp8:
     """Quantise a Linear's weight [N, K] (fp32 / fp16 / bf16) to e4m3 with one scale per 128 x 128 block; both orders of the bytes are laid
-    out here, once."""
+    out here, once.  Nothing of w or bias is kept: later changes of them do not reach the packed layer."""
     d = _dev(w)
     _dt_code(w, "pack_w_fp8")
     if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
@@ -2054,8 +2054,9 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
                         scale: float, kv_heads: Optional[int] = None, q_lens: Optional[torch.Tensor] = None,
                         kv_lens: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
     """-> (dq, dk, dv) of cross_attention for the upstream gradient g_o [B, Tq, heads * d], given its o and lse; contiguous, in the operands'
-    type.  dk / dv of shared key heads are summed over their query heads; dropped keys and rows have zeros; a k or v that was expanded over the
-    batch gets its gradient per item.  The same bits on every call."""
+    type.  dk / dv of shared key heads are summed over their query heads; dropped keys and rows have zeros, whatever live rows hold; a k or v that was
+    expanded over the batch gets its gradient per item.  fp16 gradients are finite wherever they fit the type, however large
+    or small the states and g_o are.  The same bits on every call."""
     name = "cross_attention_bwd"
     a = _Xattn(q, k, v, heads, scale, kv_heads, q_lens, kv_lens, mask, name)
     _same_device(a.d_, o, lse, g_o)
