@@ -393,3 +393,17 @@ def test_a_million_states(ops, dt):
     R, E = _exact(q, k, v, go, H, d ** -0.5, None, lens)
     for n, t in _all(ops, q, k, v, go, H, d ** -0.5, None, lens).items():
         _check(n, t, R, E)
+
+
+def test_more_items_than_a_launch_holds_are_refused(ops):
+    """2^24 pairs of item and key head (one query each, every item reading the same rows): refused on the host, nothing launched; half of them run."""
+    B, d = 1 << 18, 8
+    for H in (32, 64):
+        q, k = (torch.ones(1, T, H * d, dtype=torch.float16, device=DEV).expand(B, -1, -1) for T in (1, 2))
+        if H == 32:
+            assert (ops.cross_attention(q, k, k, H, 0.5) == 1).all()
+            continue
+        with pytest.raises(ops.TfmqError, match="too many workgroups"):
+            ops.cross_attention(q, k, k, H, 0.5)
+        with pytest.raises(ops.TfmqError, match="too many workgroups"):
+            ops.cross_attention_bwd(q, k, k, q, torch.zeros(B, H, 1, device=DEV), q, H, 0.5)

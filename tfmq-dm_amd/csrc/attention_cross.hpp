@@ -30,6 +30,7 @@ __device__ __forceinline__ v16f zero16() {
 }
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr long MAX_BLOCKS = (1L << 32) / 256;          // of a launch: its threads (256 a workgroup) are counted in 32 bits
 
 struct View {          // [B][T][heads * d] with unit channel stride; element strides
   const void* p;

@@ -544,7 +544,7 @@ int launch_dq_short(tfmq_handle h, XattnP p, hipStream_t st) {
   const long pairs = static_cast<long>(p.B) * p.G;
   p.rows_per = short_rows(h, pairs, p.R, dq_short_waves(D, NKT));
   p.nrb = ceil_div(p.R, p.rows_per);
-  TFMQ_CHECK_ARG(h, pairs * p.nrb < (1L << 31), "xattn_bwd: too many workgroups");
+  TFMQ_CHECK_ARG(h, pairs * p.nrb < MAX_BLOCKS, "xattn_bwd: too many workgroups");
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(pairs * p.nrb)), dim3(256), smem, st, p);
   TFMQ_LAUNCH_CHECK(h);
   return TFMQ_OK;
@@ -562,7 +562,7 @@ int launch_dq(tfmq_handle h, XattnP p, hipStream_t st) {
   TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
   p.nrb = ceil_div(p.R, 128);
   const long n = static_cast<long>(p.B) * p.G * p.nrb;
-  TFMQ_CHECK_ARG(h, n < (1L << 31), "xattn_bwd: too many workgroups");
+  TFMQ_CHECK_ARG(h, n < MAX_BLOCKS, "xattn_bwd: too many workgroups");
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(n)), dim3(256), smem, st, p);
   TFMQ_LAUNCH_CHECK(h);
   return TFMQ_OK;
@@ -581,7 +581,7 @@ int launch_bwd(tfmq_handle h, XattnP p, hipStream_t st) {
     XattnP c = p;
     c.nrb = ceil_div(p.Tk, 128);
     const long nk = static_cast<long>(p.B) * p.G * c.nrb * p.nsplit;
-    TFMQ_CHECK_ARG(h, nk < (1L << 31), "xattn_bwd: too many workgroups");
+    TFMQ_CHECK_ARG(h, nk < MAX_BLOCKS, "xattn_bwd: too many workgroups");
     hipLaunchKernelGGL(kk, dim3(static_cast<unsigned>(nk)), dim3(256), sk, st, c);
     TFMQ_LAUNCH_CHECK(h);
     if (p.nsplit > 1) {

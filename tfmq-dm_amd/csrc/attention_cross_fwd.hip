@@ -292,7 +292,7 @@ int launch_short(tfmq_handle h, XattnP p, hipStream_t st) {
   const long pairs = static_cast<long>(p.B) * p.G;
   p.rows_per = short_rows(h, pairs, p.R, short_waves(D, NKT));
   p.nrb = ceil_div(p.R, p.rows_per);
-  TFMQ_CHECK_ARG(h, pairs * p.nrb < (1L << 31), "xattn_fwd: too many workgroups");
+  TFMQ_CHECK_ARG(h, pairs * p.nrb < MAX_BLOCKS, "xattn_fwd: too many workgroups");
   hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(pairs * p.nrb)), dim3(256), smem, st, p);
   TFMQ_LAUNCH_CHECK(h);
   return TFMQ_OK;
@@ -315,7 +315,7 @@ int launch_fwd(tfmq_handle h, XattnP p, hipStream_t st) {
     TFMQ_HIP(h, room_kern.ask(h, reinterpret_cast<const void*>(kern), smem));
     p.nrb = ceil_div(p.R, 128);
     const long nb = static_cast<long>(p.B) * p.G * p.nrb * p.nsplit;
-    TFMQ_CHECK_ARG(h, nb < (1L << 31), "xattn_fwd: too many workgroups");
+    TFMQ_CHECK_ARG(h, nb < MAX_BLOCKS, "xattn_fwd: too many workgroups");
     hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(nb)), dim3(256), smem, st, p);
     TFMQ_LAUNCH_CHECK(h);
     if (p.nsplit > 1) {
